@@ -448,6 +448,96 @@ int pp_lion_step_f32(int count, float* const* p, const float* const* g, float* c
                      const long* numel, float lr, float beta1, float beta2, float weight_decay,
                      int sparse, void* stream);
 
+/* ---- Sequence-model operators in 32- and 16-bit types (no counterpart in the reference) ----
+ * Element type of the tensors passed as void*; everything is computed in fp32.  Pointers are
+ * aligned to their element, not more; strides count elements and are free (a row of channels or
+ * classes is contiguous), so slices of wider tensors are read in place. */
+enum { PP_F32 = 0, PP_BF16 = 1, PP_F16 = 2 };
+
+/* Gated linear recurrence beside the selective scan (csrc/pp_recurrence.hip):
+ *   a = sigmoid(f_t);  h_t = a h_{t-1} + (1 - a) z_t;  y_t = h_t          per channel, h in fp32
+ * z, f: [b][l][d] with strides (zb, zl), (fb, fl) over batch and time;  y: [b][l][d] contiguous;
+ * h0: [b][d] or NULL (zeros);  h_last: [b][d].  lengths: [b] int32 or NULL: steps from
+ * lengths[i] on (clamped to [0, l]) are not read, y is 0 there and h_last is the state before
+ * them.  reset: [b][l] bytes or NULL: non-zero drops the state before that step.
+ * starts: NULL, or [b][pp_gated_recurrence_starts(l)][d] fp32, the states that the backward needs.
+ * Backward: gy [b][l][d] with strides (gb, gl), gh_last [b][d] or NULL (zeros); writes gz, gf
+ * [b][l][d] contiguous and gh0 [b][d] unless NULL.  Scratch: pp_gated_recurrence_workspace_bytes
+ * for either direction (0: none needed), contents undefined on entry and exit; calls that may run
+ * at the same time need one each.  b <= 65535.  Bitwise reproducible.
+ * The step form takes one token for b running sequences: z, f [b][d] with row strides zb, fb; h
+ * [b][d] fp32 with row stride hb is replaced by the new state, y [b][d] contiguous receives it. */
+#define PP_RECURRENCE_STEPS 16
+int pp_gated_recurrence_starts(int l);
+size_t pp_gated_recurrence_workspace_bytes(int b, int l, int d);
+int pp_gated_recurrence_fwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
+                            int64_t fl, int dtype, const float* h0, const int32_t* lengths,
+                            const uint8_t* reset, void* y, float* h_last, float* starts,
+                            void* workspace, size_t workspace_bytes, int b, int l, int d,
+                            void* stream);
+int pp_gated_recurrence_bwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
+                            int64_t fl, int dtype, const int32_t* lengths, const uint8_t* reset,
+                            const float* starts, const void* gy, int64_t gb, int64_t gl,
+                            const float* gh_last, void* gz, void* gf, float* gh0, void* workspace,
+                            size_t workspace_bytes, int b, int l, int d, void* stream);
+int pp_gated_recurrence_step(const void* z, int64_t zb, const void* f, int64_t fb, int dtype,
+                             float* h, int64_t hb, void* y, int b, int d, void* stream);
+
+/* Log-probability of given tokens and the clipped policy loss beside the cross entropy
+ * (csrc/pp_policy.hip).  logits: [b][t][v] with strides (lb, lt);  tokens: [b][t] int64;  mask:
+ * [b][t] bytes or NULL (all count).  A masked token is not read at all; a token that counts and
+ * lies outside [0, v) makes its log-probability, and a loss, NaN.
+ *   lp = logits[token] - logsumexp(logits)                                     (0 where masked)
+ * stats: NULL, or [b][t][2] floats for the backward, which writes
+ *   grad = gout[0] * coef[b][t] * (onehot(token) - softmax)     (zeros where masked; gout NULL: 1)
+ * with the logits' strides; where those leave gaps, the gaps are not written.  done_if_one: grad
+ * holds the result for gout = 1 already.
+ *   rho = exp(lp - old);  k = exp(ref - lp) - (ref - lp) - 1
+ *   loss = mean(-min(rho adv, clip(rho, 1 - clip_low, 1 + clip_high) adv) + kl_coef k)
+ * out[0] = loss, out[1] = mean k (ref NULL: 0, and no such term), out[2] = share of the tokens whose
+ * ratio was clipped.  The mean is over the tokens that count, or (by_sequence) over the means of
+ * the sequences that have any; nothing counts: 0.  old, ref: [b][t] fp32; adv: fp32 with strides
+ * (ab, at), 0 where it is shared.  stats, coef ([b][t] floats: dloss/dlp) and grad (dloss/dlogits,
+ * the logits' strides and alignment to 16 bytes) are written unless stats / grad are NULL.
+ * Bitwise reproducible. */
+int pp_token_log_probs_fwd(const void* logits, int64_t lb, int64_t lt, int dtype,
+                           const int64_t* tokens, const uint8_t* mask, float* lp, float* stats,
+                           int b, int t, int v, void* stream);
+int pp_token_log_probs_bwd(const void* logits, int64_t lb, int64_t lt, int dtype,
+                           const int64_t* tokens, const uint8_t* mask, const float* stats,
+                           const float* coef, const float* gout, int done_if_one, void* grad, int b,
+                           int t, int v, void* stream);
+size_t pp_clipped_policy_loss_workspace_bytes(int b, int t);
+int pp_clipped_policy_loss_fwd(const void* logits, int64_t lb, int64_t lt, int dtype,
+                               const int64_t* tokens, const uint8_t* mask, const float* old_lp,
+                               const float* adv, int64_t ab, int64_t at, const float* ref_lp,
+                               float clip_low, float clip_high, float kl_coef, int by_sequence,
+                               float* out, float* stats, float* coef, void* grad, void* workspace,
+                               size_t workspace_bytes, int b, int t, int v, void* stream);
+
+/* AdamW beside Lion (csrc/pp_adamw.hip), `count` <= PP_OPT_MAX_TENSORS tensors in one launch:
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+ *   w = w (1 - lr wd) - lr / (1 - b1^s) * m / (sqrt(v) / sqrt(1 - b2^s) + eps)
+ * g is multiplied by *grad_scale first (device scalar; NULL: 1).  dtype: type of p and g; PP_F32:
+ * w is p and master is NULL, 16-bit: w is master[t] (fp32) and p receives w rounded to nearest.
+ * moment_bits 32: m, v fp32, m_exp and v_exp NULL.  8: codes of one byte and one exponent byte for
+ * every 256 entries (pp_moment_blocks), all zero at first; stochastic rounding from (seed, s,
+ * first_index + t, entry).  pp_decode_moment: their values as `dtype`.
+ * step: host array of step numbers s >= 1; or step_dev, an array of device counters of which s is
+ * read when the kernel runs (pp_count_step adds 1 to each; a graph that holds both calls counts its
+ * replays).  Host arrays of `count` entries; tensors are `numel[t]` elements in one order, updated
+ * in place, each in the list once. */
+int64_t pp_moment_blocks(int64_t numel);
+int pp_count_step(int count, int64_t* const* step, void* stream);
+int pp_adamw_step(int count, int dtype, int moment_bits, void* const* p, const void* const* g,
+                  float* const* master, void* const* m, void* const* v, uint8_t* const* m_exp,
+                  uint8_t* const* v_exp, const int64_t* numel, const int64_t* step,
+                  const int64_t* const* step_dev, double lr, double beta1, double beta2, double eps,
+                  double weight_decay, const float* grad_scale, uint32_t seed, uint32_t first_index,
+                  void* stream);
+int pp_decode_moment(const uint8_t* codes, const uint8_t* exponents, void* out, int dtype,
+                     int is_signed, int64_t numel, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

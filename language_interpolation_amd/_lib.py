@@ -8,7 +8,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_long, c_size_t, c_void_p
+from ctypes import (c_double, c_float, c_int, c_int64, c_long, c_size_t, c_uint32,
+                    c_void_p)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpphip.so")
@@ -122,6 +123,25 @@ SIGNATURES = {
     "pp_cross_entropy_bwd_f32": (c_int, [_P, _P, _P, _P, c_int, c_int, _P]),
     "pp_selective_scan_fwd_f32": (c_int, [_P] * 8 + [c_int] * 4 + [_P]),
     "pp_selective_scan_bwd_f32": (c_int, [_P] * 14 + [c_int] * 4 + [_P]),
+    "pp_gated_recurrence_starts": (c_int, [c_int]),
+    "pp_gated_recurrence_workspace_bytes": (c_size_t, [c_int] * 3),
+    "pp_gated_recurrence_fwd": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, c_int] + [_P] * 7 +
+                                [c_size_t] + [c_int] * 3 + [_P]),
+    "pp_gated_recurrence_bwd": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, c_int] + [_P] * 4 +
+                                [c_int64, c_int64] + [_P] * 5 + [c_size_t] + [c_int] * 3 + [_P]),
+    "pp_gated_recurrence_step": (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int64, _P, c_int,
+                                         c_int, _P]),
+    "pp_token_log_probs_fwd": (c_int, [_P, c_int64, c_int64, c_int] + [_P] * 4 + [c_int] * 3 + [_P]),
+    "pp_token_log_probs_bwd": (c_int, [_P, c_int64, c_int64, c_int] + [_P] * 5 + [c_int, _P] +
+                               [c_int] * 3 + [_P]),
+    "pp_clipped_policy_loss_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "pp_clipped_policy_loss_fwd": (c_int, [_P, c_int64, c_int64, c_int] + [_P] * 4 +
+                                   [c_int64, c_int64, _P] + [c_float] * 3 + [c_int] + [_P] * 5 +
+                                   [c_size_t] + [c_int] * 3 + [_P]),
+    "pp_moment_blocks": (c_int64, [c_int64]),
+    "pp_count_step": (c_int, [c_int, _P, _P]),
+    "pp_adamw_step": (c_int, [c_int] * 3 + [_P] * 10 + [c_double] * 5 + [_P, c_uint32, c_uint32, _P]),
+    "pp_decode_moment": (c_int, [_P, _P, _P, c_int, c_int, c_int64, _P]),
     "pp_transpose_w_f32": (c_int, [_P, _P, c_int, c_int, c_int, _P]),
     "pp_transpose_wt_f32": (c_int, [_P, _P, c_int, c_int, c_int, _P]),
 }

@@ -868,4 +868,188 @@ int pp_lion_step_f32(int count, float* const* p, const float* const* g, float* c
                                (hipStream_t)stream));
 }
 
+// ---- sequence-model operators ----
+static bool aligned_to(const void* p, size_t n) { return ((size_t)p & (n - 1)) == 0; }
+static int elem_ok(int dtype) { return dtype == PP_F32 || dtype == PP_BF16 || dtype == PP_F16; }
+static size_t elem_size(int dtype) { return dtype == PP_F32 ? 4 : 2; }
+static int rec_args_ok(int dtype, int b, int l, int d) {
+  if (!elem_ok(dtype)) return PP_ERR_METHOD;
+  if (b < 1 || l < 1 || d < 1 || b > 65535) return PP_ERR_SHAPE;
+  if ((int64_t)b * l >= (1LL << 31) || (int64_t)l + 4096 >= (1LL << 31) || d > (1 << 24))
+    return PP_ERR_RANGE;
+  return PP_OK;
+}
+
+int pp_gated_recurrence_starts(int l) {
+  return l > 0 ? (int)(((int64_t)l + PP_RECURRENCE_STEPS - 1) / PP_RECURRENCE_STEPS) : 0;
+}
+
+size_t pp_gated_recurrence_workspace_bytes(int b, int l, int d) {
+  return b > 0 && l > 0 && d > 0 ? pp_rec_workspace_bytes(b, l, d) : 0;
+}
+
+int pp_gated_recurrence_fwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
+                            int64_t fl, int dtype, const float* h0, const int32_t* lengths,
+                            const uint8_t* reset, void* y, float* h_last, float* starts,
+                            void* workspace, size_t workspace_bytes, int b, int l, int d,
+                            void* stream) {
+  if (!z || !f || !y || !h_last) return PP_ERR_NULL;
+  int rc = rec_args_ok(dtype, b, l, d);
+  if (rc != PP_OK) return rc;
+  const size_t s = elem_size(dtype);
+  if (!aligned_to(z, s) || !aligned_to(f, s) || !aligned_to(y, s) || !aligned_to(h0, 4) ||
+      !aligned_to(h_last, 4) || !aligned_to(lengths, 4) || !aligned_to(starts, 4))
+    return PP_ERR_ALIGN;
+  const size_t need = pp_rec_workspace_bytes(b, l, d);
+  if (need && (!workspace || workspace_bytes < need)) return PP_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return PP_ERR_ALIGN;
+  return hip_rc(pp_launch_rec_fwd(z, zb, zl, f, fb, fl, dtype, h0, lengths, reset, y, h_last, starts,
+                                  workspace, b, l, d, (hipStream_t)stream));
+}
+
+int pp_gated_recurrence_bwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
+                            int64_t fl, int dtype, const int32_t* lengths, const uint8_t* reset,
+                            const float* starts, const void* gy, int64_t gb, int64_t gl,
+                            const float* gh_last, void* gz, void* gf, float* gh0, void* workspace,
+                            size_t workspace_bytes, int b, int l, int d, void* stream) {
+  if (!z || !f || !starts || !gy || !gz || !gf) return PP_ERR_NULL;
+  int rc = rec_args_ok(dtype, b, l, d);
+  if (rc != PP_OK) return rc;
+  const size_t s = elem_size(dtype);
+  if (!aligned_to(z, s) || !aligned_to(f, s) || !aligned_to(gy, s) || !aligned_to(gz, s) ||
+      !aligned_to(gf, s) || !aligned_to(gh_last, 4) || !aligned_to(gh0, 4) ||
+      !aligned_to(lengths, 4) || !aligned_to(starts, 4))
+    return PP_ERR_ALIGN;
+  const size_t need = pp_rec_workspace_bytes(b, l, d);
+  if (need && (!workspace || workspace_bytes < need)) return PP_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return PP_ERR_ALIGN;
+  return hip_rc(pp_launch_rec_bwd(z, zb, zl, f, fb, fl, dtype, lengths, reset, starts, gy, gb, gl,
+                                  gh_last, gz, gf, gh0, workspace, b, l, d, (hipStream_t)stream));
+}
+
+int pp_gated_recurrence_step(const void* z, int64_t zb, const void* f, int64_t fb, int dtype,
+                             float* h, int64_t hb, void* y, int b, int d, void* stream) {
+  if (!z || !f || !h || !y) return PP_ERR_NULL;
+  int rc = rec_args_ok(dtype, b, 1, d);
+  if (rc != PP_OK) return rc;
+  if (hb < d && b > 1) return PP_ERR_SHAPE;  // two sequences would share a state
+  const size_t s = elem_size(dtype);
+  if (!aligned_to(z, s) || !aligned_to(f, s) || !aligned_to(y, s) || !aligned_to(h, 4))
+    return PP_ERR_ALIGN;
+  return hip_rc(pp_launch_rec_step(z, zb, f, fb, dtype, h, hb, y, b, d, (hipStream_t)stream));
+}
+
+static int pol_args_ok(int dtype, int b, int t, int v) {
+  if (!elem_ok(dtype)) return PP_ERR_METHOD;
+  if (b < 1 || t < 1 || v < 1) return PP_ERR_SHAPE;
+  if ((int64_t)b * t >= (1LL << 30) || v > (1 << 30)) return PP_ERR_RANGE;
+  return PP_OK;
+}
+
+int pp_token_log_probs_fwd(const void* logits, int64_t lb, int64_t lt, int dtype,
+                           const int64_t* tokens, const uint8_t* mask, float* lp, float* stats,
+                           int b, int t, int v, void* stream) {
+  if (!logits || !tokens || !lp) return PP_ERR_NULL;
+  int rc = pol_args_ok(dtype, b, t, v);
+  if (rc != PP_OK) return rc;
+  if (!aligned_to(logits, elem_size(dtype)) || !aligned_to(tokens, 8) || !aligned_to(lp, 4) ||
+      !aligned_to(stats, 8))
+    return PP_ERR_ALIGN;
+  return hip_rc(pp_launch_token_lp(logits, lb, lt, dtype, tokens, mask, lp, stats, b, t, v,
+                                   (hipStream_t)stream));
+}
+
+int pp_token_log_probs_bwd(const void* logits, int64_t lb, int64_t lt, int dtype,
+                           const int64_t* tokens, const uint8_t* mask, const float* stats,
+                           const float* coef, const float* gout, int done_if_one, void* grad, int b,
+                           int t, int v, void* stream) {
+  if (!logits || !tokens || !stats || !coef || !grad) return PP_ERR_NULL;
+  int rc = pol_args_ok(dtype, b, t, v);
+  if (rc != PP_OK) return rc;
+  if (!aligned_to(logits, elem_size(dtype)) || !aligned_to(tokens, 8) || !aligned_to(coef, 4) ||
+      !aligned_to(stats, 8) || (((size_t)logits ^ (size_t)grad) & 15))
+    return PP_ERR_ALIGN;
+  return hip_rc(pp_launch_token_lp_bwd(logits, lb, lt, dtype, tokens, mask, stats, coef, gout,
+                                       done_if_one, grad, b, t, v, (hipStream_t)stream));
+}
+
+size_t pp_clipped_policy_loss_workspace_bytes(int b, int t) {
+  return b > 0 && t > 0 ? pp_policy_workspace_bytes(b, t) : 0;
+}
+
+int pp_clipped_policy_loss_fwd(const void* logits, int64_t lb, int64_t lt, int dtype,
+                               const int64_t* tokens, const uint8_t* mask, const float* old_lp,
+                               const float* adv, int64_t ab, int64_t at, const float* ref_lp,
+                               float clip_low, float clip_high, float kl_coef, int by_sequence,
+                               float* out, float* stats, float* coef, void* grad, void* workspace,
+                               size_t workspace_bytes, int b, int t, int v, void* stream) {
+  if (!logits || !tokens || !old_lp || !adv || !out || (stats && !coef)) return PP_ERR_NULL;
+  int rc = pol_args_ok(dtype, b, t, v);
+  if (rc != PP_OK) return rc;
+  if (!(clip_low >= 0.0f) || !(clip_high >= 0.0f)) return PP_ERR_SHAPE;
+  if (!aligned_to(logits, elem_size(dtype)) || !aligned_to(tokens, 8) || !aligned_to(old_lp, 4) ||
+      !aligned_to(adv, 4) || !aligned_to(ref_lp, 4) || !aligned_to(out, 4) || !aligned_to(coef, 4) ||
+      !aligned_to(stats, 8) || (grad && (((size_t)logits ^ (size_t)grad) & 15)))
+    return PP_ERR_ALIGN;
+  if (!workspace || workspace_bytes < pp_policy_workspace_bytes(b, t)) return PP_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return PP_ERR_ALIGN;
+  return hip_rc(pp_launch_policy(logits, lb, lt, dtype, tokens, mask, old_lp, adv, ab, at, ref_lp,
+                                 clip_low, clip_high, kl_coef, by_sequence, out, stats, coef, grad,
+                                 workspace, b, t, v, (hipStream_t)stream));
+}
+
+int64_t pp_moment_blocks(int64_t numel) { return numel > 0 ? (numel + 255) / 256 : 0; }
+
+int pp_count_step(int count, int64_t* const* step, void* stream) {
+  if (count < 1 || count > PP_OPT_MAX_TENSORS) return PP_ERR_SHAPE;
+  if (!step) return PP_ERR_NULL;
+  for (int i = 0; i < count; ++i) {
+    if (!step[i]) return PP_ERR_NULL;
+    if (!aligned_to(step[i], 8)) return PP_ERR_ALIGN;
+    for (int j = 0; j < i; ++j)
+      if (step[j] == step[i]) return PP_ERR_SHAPE;  // the two additions would race
+  }
+  return hip_rc(pp_launch_count_step(count, step, (hipStream_t)stream));
+}
+
+int pp_adamw_step(int count, int dtype, int moment_bits, void* const* p, const void* const* g,
+                  float* const* master, void* const* m, void* const* v, uint8_t* const* m_exp,
+                  uint8_t* const* v_exp, const int64_t* numel, const int64_t* step,
+                  const int64_t* const* step_dev, double lr, double beta1, double beta2, double eps,
+                  double weight_decay, const float* grad_scale, uint32_t seed, uint32_t first_index,
+                  void* stream) {
+  if (count < 1 || count > PP_OPT_MAX_TENSORS) return PP_ERR_SHAPE;
+  if (!elem_ok(dtype) || (moment_bits != 8 && moment_bits != 32)) return PP_ERR_METHOD;
+  if (!p || !g || !m || !v || !numel || (!step && !step_dev)) return PP_ERR_NULL;
+  if ((dtype != PP_F32 && !master) || (moment_bits == 8 && (!m_exp || !v_exp))) return PP_ERR_NULL;
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return PP_ERR_SHAPE;
+  const size_t s = elem_size(dtype), ms = moment_bits / 8;
+  if (!aligned_to(grad_scale, 4)) return PP_ERR_ALIGN;
+  for (int t = 0; t < count; ++t) {
+    if (!p[t] || !g[t] || !m[t] || !v[t] || (dtype != PP_F32 && !master[t]) ||
+        (moment_bits == 8 && (!m_exp[t] || !v_exp[t])) || (step_dev && !step_dev[t]))
+      return PP_ERR_NULL;
+    if (numel[t] < 1 || (!step_dev && step[t] < 1)) return PP_ERR_SHAPE;
+    if (numel[t] > (1LL << 36)) return PP_ERR_RANGE;
+    if (!aligned_to(p[t], s) || !aligned_to(g[t], s) || !aligned_to(m[t], ms) ||
+        !aligned_to(v[t], ms) || (dtype != PP_F32 && !aligned_to(master[t], 4)) ||
+        (step_dev && !aligned_to(step_dev[t], 8)))
+      return PP_ERR_ALIGN;
+  }
+  return hip_rc(pp_launch_adamw(count, dtype, moment_bits, p, g, master, m, v, m_exp, v_exp, numel,
+                                step, step_dev, lr, beta1, beta2, eps, weight_decay, grad_scale,
+                                seed, first_index, (hipStream_t)stream));
+}
+
+int pp_decode_moment(const uint8_t* codes, const uint8_t* exponents, void* out, int dtype,
+                     int is_signed, int64_t numel, void* stream) {
+  if (!codes || !exponents || !out) return PP_ERR_NULL;
+  if (!elem_ok(dtype)) return PP_ERR_METHOD;
+  if (numel < 1) return PP_ERR_SHAPE;
+  if (numel > (1LL << 36)) return PP_ERR_RANGE;
+  if (!aligned_to(out, elem_size(dtype))) return PP_ERR_ALIGN;
+  return hip_rc(pp_launch_decode_moment(codes, exponents, out, dtype, is_signed, numel,
+                                        (hipStream_t)stream));
+}
+
 }  // extern "C"

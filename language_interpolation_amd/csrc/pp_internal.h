@@ -177,3 +177,43 @@ hipError_t pp_launch_bwd_w_h2_ln(const float* x, const float* gy, const float* y
                                  const float* rstd, const float* rowstats, int ntile, float* g_out,
                                  float* gwt, void* ws, const PPShape& sh, const BasisTab& tab,
                                  hipStream_t st);
+
+// ---- gated linear recurrence (pp_recurrence.hip) ----
+size_t pp_rec_workspace_bytes(int b, int l, int d);
+hipError_t pp_launch_rec_fwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
+                             int64_t fl, int dtype, const float* h0, const int32_t* lengths,
+                             const uint8_t* reset, void* y, float* h_last, float* starts, void* ws,
+                             int b, int l, int d, hipStream_t st);
+hipError_t pp_launch_rec_bwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
+                             int64_t fl, int dtype, const int32_t* lengths, const uint8_t* reset,
+                             const float* starts, const void* gy, int64_t gb, int64_t gl,
+                             const float* gh_last, void* gz, void* gf, float* gh0, void* ws, int b,
+                             int l, int d, hipStream_t st);
+hipError_t pp_launch_rec_step(const void* z, int64_t zb, const void* f, int64_t fb, int dtype,
+                              float* h, int64_t hb, void* y, int b, int d, hipStream_t st);
+
+// ---- token log-probabilities and the clipped policy loss (pp_policy.hip) ----
+hipError_t pp_launch_token_lp(const void* logits, int64_t lb, int64_t lt, int dtype,
+                              const int64_t* tokens, const uint8_t* mask, float* lp, float* stats,
+                              int b, int t, int v, hipStream_t st);
+hipError_t pp_launch_token_lp_bwd(const void* logits, int64_t lb, int64_t lt, int dtype,
+                                  const int64_t* tokens, const uint8_t* mask, const float* stats,
+                                  const float* coef, const float* gout, int done_if_one, void* grad,
+                                  int b, int t, int v, hipStream_t st);
+size_t pp_policy_workspace_bytes(int b, int t);
+hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtype,
+                            const int64_t* tokens, const uint8_t* mask, const float* old,
+                            const float* adv, int64_t ab, int64_t at, const float* ref, float low,
+                            float high, float beta, int by_sequence, float* out, float* stats,
+                            float* coef, void* grad, void* ws, int b, int t, int v, hipStream_t st);
+
+// ---- AdamW over many tensors (pp_adamw.hip) ----
+hipError_t pp_launch_count_step(int count, int64_t* const* step, hipStream_t st);
+hipError_t pp_launch_adamw(int count, int dtype, int bits, void* const* p, const void* const* g,
+                           float* const* master, void* const* m, void* const* v,
+                           uint8_t* const* m_exp, uint8_t* const* v_exp, const int64_t* numel,
+                           const int64_t* step, const int64_t* const* step_dev, double lr,
+                           double beta1, double beta2, double eps, double wd,
+                           const float* grad_scale, uint32_t seed, uint32_t index, hipStream_t st);
+hipError_t pp_launch_decode_moment(const uint8_t* code, const uint8_t* exps, void* out, int dtype,
+                                   int is_signed, int64_t n, hipStream_t st);

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from ctypes import c_void_p
 from dataclasses import dataclass, field
 from typing import Optional, Tuple
 
@@ -1015,3 +1016,469 @@ class RMSNormFunction(torch.autograd.Function):
 
 def rms_norm(x, weight, eps: float = 1e-5):
     return RMSNormFunction.apply(x, weight, eps)
+
+
+# ---------------------------------------------------------------------------
+# Sequence-model operators in fp32, bf16 and fp16 (no counterpart in the reference): the gated
+# linear recurrence beside the selective scan, the clipped policy loss beside the cross entropy,
+# the AdamW step beside Lion (csrc/pp_recurrence.hip, pp_policy.hip, pp_adamw.hip)
+# ---------------------------------------------------------------------------
+_ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PP_F32, PP_BF16, PP_F16
+
+
+def _require_element(t, name: str, like=None) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}: this operator runs on MI355X (HIP) only; "
+                           "there is no CPU path in this package")
+    if t.dtype not in _ELEMENT:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise TypeError(f"{name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+
+
+def _require_aux(t, name: str, shape, dtypes, device) -> None:
+    """A tensor of the given shape, one of the dtypes, on the device of the main operand."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+
+
+def _bytes_of(mask: Optional[torch.Tensor]):
+    """A bool or uint8 mask as contiguous bytes."""
+    return None if mask is None else mask.contiguous().view(torch.uint8)
+
+
+def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class GatedRecurrenceFunction(torch.autograd.Function):
+    """(y, h_last) of gated_recurrence; keeps z, f and the state at the start of every
+    PP_RECURRENCE_STEPS steps, the backward recomputes the states in between."""
+
+    @staticmethod
+    def forward(ctx, z, f, h0, lengths, reset):
+        lib = _lib.load()
+        ctx.set_materialize_grads(False)
+        z, f = _last_contiguous(z), _last_contiguous(f)
+        b, l, d = z.shape
+        y = torch.empty(b, l, d, device=z.device, dtype=z.dtype)
+        h0 = None if h0 is None else h0.contiguous()
+        starts = None
+        if z.numel() == 0:  # no step: the state stays as it is
+            h = torch.zeros(b, d, device=z.device) if h0 is None else h0.clone()
+        else:
+            h = torch.empty(b, d, device=z.device, dtype=torch.float32)
+            if any(ctx.needs_input_grad):
+                starts = torch.empty(b, lib.pp_gated_recurrence_starts(l), d, device=z.device)
+            nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
+            ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
+            with torch.cuda.device(z.device):
+                rc = lib.pp_gated_recurrence_fwd(
+                    _ptr(z), z.stride(0), z.stride(1), _ptr(f), f.stride(0), f.stride(1),
+                    _ELEMENT[z.dtype], _ptr(h0), _ptr(lengths), _ptr(reset), _ptr(y), _ptr(h),
+                    _ptr(starts), _ptr(ws), nbytes, b, l, d, _stream(z.device))
+            _lib.check(rc, "pp_gated_recurrence_fwd")
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(z, f, starts, lengths, reset)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy, gh):
+        lib = _lib.load()
+        z, f, starts, lengths, reset = ctx.saved_tensors
+        b, l, d = z.shape
+        gz = torch.empty(b, l, d, device=z.device, dtype=z.dtype)
+        gf = torch.empty_like(gz)
+        gh = None if gh is None else gh.contiguous()
+        if z.numel() == 0:
+            return gz, gf, gh if ctx.needs_input_grad[2] else None, None, None
+        gy = torch.zeros_like(gz) if gy is None else _last_contiguous(gy)
+        gh0 = torch.empty(b, d, device=z.device) if ctx.needs_input_grad[2] else None
+        nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
+        ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
+        with torch.cuda.device(z.device):
+            rc = lib.pp_gated_recurrence_bwd(
+                _ptr(z), z.stride(0), z.stride(1), _ptr(f), f.stride(0), f.stride(1),
+                _ELEMENT[z.dtype], _ptr(lengths), _ptr(reset), _ptr(starts), _ptr(gy),
+                gy.stride(0), gy.stride(1), _ptr(gh), _ptr(gz), _ptr(gf), _ptr(gh0), _ptr(ws),
+                nbytes, b, l, d, _stream(z.device))
+        _lib.check(rc, "pp_gated_recurrence_bwd")
+        return gz, gf, gh0, None, None
+
+
+def gated_recurrence(z, f, h0=None, lengths=None, reset=None):
+    """(y, h_last) of the gated linear recurrence along dim 1 of z, f [b, l, d]:
+
+        a_t = sigmoid(f_t);   h_t = a_t * h_{t-1} + (1 - a_t) * z_t;   y_t = h_t
+
+    z, f: fp32, bf16 or fp16 on the GPU, read in place if their last dim is contiguous (the halves of
+    one projection are).  h0: the state before the first step, fp32 [b, d] (default zeros).
+    lengths: int [b], the steps of each row that exist (y is 0 behind them, h_last is the state
+    before them); reset: bool [b, l], steps before which the state is dropped (a new document in a
+    packed row).  y has z's dtype, h_last is fp32.  Differentiable in z, f and h0."""
+    _require_element(z, "z")
+    _require_element(f, "f", like=z)
+    if z.dim() != 3 or f.shape != z.shape:
+        raise ValueError(f"gated_recurrence: z, f [b, l, d], got {tuple(z.shape)}, {tuple(f.shape)}")
+    b, l, d = z.shape
+    if h0 is not None:
+        _require_aux(h0, "h0", (b, d), (torch.float32,), z.device)
+    if lengths is not None:
+        _require_aux(lengths, "lengths", (b,), (torch.int32, torch.int64), z.device)
+        lengths = lengths.clamp(0, l).to(torch.int32) if lengths.dtype == torch.int64 else \
+            lengths.contiguous()
+    if reset is not None:
+        _require_aux(reset, "reset", (b, l), (torch.bool, torch.uint8), z.device)
+        reset = _bytes_of(reset)
+    return GatedRecurrenceFunction.apply(z, f, h0, lengths, reset)
+
+
+def gated_recurrence_step(z, f, h):
+    """One token of b running sequences: z, f [b, d]; h [b, d] fp32 is replaced by the new state,
+    which is returned in z's dtype.  No backward: gated_recurrence has one."""
+    _require_element(z, "z")
+    _require_element(f, "f", like=z)
+    if z.dim() != 2 or f.shape != z.shape:
+        raise ValueError(f"gated_recurrence_step: z, f [b, d], got {tuple(z.shape)}, {tuple(f.shape)}")
+    b, d = z.shape
+    _require_aux(h, "h", (b, d), (torch.float32,), z.device)
+    if (d > 1 and h.stride(1) != 1) or (b > 1 and h.stride(0) < d):
+        raise ValueError("gated_recurrence_step: the rows of h must be contiguous and not overlap")
+    if torch.is_grad_enabled() and (z.requires_grad or f.requires_grad or h.requires_grad):
+        raise RuntimeError("gated_recurrence_step has no backward; call it under torch.no_grad(), "
+                           "or gated_recurrence on [b, 1, d]")
+    y = torch.empty(b, d, device=z.device, dtype=z.dtype)
+    if z.numel() == 0:
+        return y
+    z, f = _last_contiguous(z), _last_contiguous(f)
+    lib = _lib.load()
+    with torch.cuda.device(z.device):
+        rc = lib.pp_gated_recurrence_step(_ptr(z), z.stride(0), _ptr(f), f.stride(0),
+                                          _ELEMENT[z.dtype], _ptr(h), max(h.stride(0), d), _ptr(y),
+                                          b, d, _stream(z.device))
+    _lib.check(rc, "pp_gated_recurrence_step")
+    torch._C._increment_version([h])
+    return y
+
+
+def _class_rows(logits):
+    """(logits usable in place, strides over batch and time, buffer for their gradient): [b, t, v]
+    with contiguous classes and rows that do not overlap is read as it is, anything else copied."""
+    b, t, v = logits.shape
+    lt = logits.stride(1) if t > 1 else max(v, logits.stride(1))
+    lb = logits.stride(0) if b > 1 else max(1, t) * lt
+    if (logits.stride(2) != 1 and v > 1) or lt < v or lb < (t - 1) * lt + v:
+        logits = logits.contiguous()
+        lt, lb = v, t * v
+    return logits, lb, lt
+
+
+def _class_grad(logits, lb, lt):
+    """An empty gradient with the strides of the logits and their offset within 16 bytes."""
+    b, t, v = logits.shape
+    off = logits.data_ptr() % 16 // logits.element_size()
+    if off == 0 and logits.is_contiguous():
+        return torch.empty_like(logits)
+    span = (b - 1) * lb + (t - 1) * lt + v
+    buf = torch.empty(off + span, device=logits.device, dtype=logits.dtype)
+    return buf.as_strided((b, t, v), (lb, lt, 1), off)
+
+
+def _check_classes(logits, tokens, mask):
+    _require_element(logits, "logits")
+    if logits.dim() != 3 or logits.shape[2] < 1:
+        raise ValueError(f"logits must be [b, t, classes], got {tuple(logits.shape)}")
+    _require_aux(tokens, "tokens", logits.shape[:2], (torch.int64, torch.int32), logits.device)
+    if mask is not None:
+        _require_aux(mask, "mask", logits.shape[:2], (torch.bool, torch.uint8), logits.device)
+    return tokens.long().contiguous(), _bytes_of(mask)
+
+
+class TokenLogProbsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask):
+        lib = _lib.load()
+        b, t, v = logits.shape
+        logits, lb, lt = _class_rows(logits)
+        lp = torch.empty(b, t, device=logits.device, dtype=torch.float32)
+        stats = torch.empty(b, t, 2, device=logits.device) if ctx.needs_input_grad[0] else None
+        if lp.numel():
+            with torch.cuda.device(logits.device):
+                rc = lib.pp_token_log_probs_fwd(
+                    _ptr(logits), lb, lt, _ELEMENT[logits.dtype], _ptr(tokens), _ptr(mask), _ptr(lp),
+                    _ptr(stats), b, t, v, _stream(logits.device))
+            _lib.check(rc, "pp_token_log_probs_fwd")
+        if stats is not None:
+            ctx.save_for_backward(logits, tokens, mask, stats)
+            ctx.strides = (lb, lt)
+        return lp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, glp):
+        logits, tokens, mask, stats = ctx.saved_tensors
+        grad = _class_grad(logits, *ctx.strides)
+        _class_backward(logits, tokens, mask, stats, glp.float().contiguous(), None, 0, grad, ctx.strides)
+        return grad, None, None
+
+
+def _class_backward(logits, tokens, mask, stats, coef, gout, done_if_one, grad, strides):
+    """grad = gout * coef * (onehot(token) - softmax(logits)), row by row."""
+    b, t, v = logits.shape
+    if b * t == 0:
+        return
+    lib = _lib.load()
+    with torch.cuda.device(logits.device):
+        rc = lib.pp_token_log_probs_bwd(
+            _ptr(logits), strides[0], strides[1], _ELEMENT[logits.dtype], _ptr(tokens), _ptr(mask),
+            _ptr(stats), _ptr(coef), _ptr(gout), done_if_one, _ptr(grad), b, t, v,
+            _stream(logits.device))
+    _lib.check(rc, "pp_token_log_probs_bwd")
+
+
+def token_log_probs(logits, tokens, mask=None):
+    """log softmax(logits)[token] as fp32: logits [b, t, v] (or [n, v]) in fp32, bf16 or fp16, tokens
+    int [b, t] (or [n]).  mask: bool, False where a token does not count: 0 there, its logits are not
+    read, its token may be anything (-100).  A token that counts and is no class gives NaN.
+    Differentiable in the logits."""
+    if isinstance(logits, torch.Tensor) and logits.dim() == 2:
+        return token_log_probs(logits[None], tokens[None], None if mask is None else mask[None])[0]
+    tokens, mask = _check_classes(logits, tokens, mask)
+    return TokenLogProbsFunction.apply(logits, tokens, mask)
+
+
+class ClippedPolicyLossFunction(torch.autograd.Function):
+    """(loss, kl, clipped).  When a gradient is needed the forward writes it for an upstream gradient
+    of 1 while the row is on the chip: one read and one write of the logits' size for both
+    directions.  The backward hands it out, or, where the upstream gradient is not 1 or it was
+    handed out before, computes it again from the logits."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, old, adv, ref, low, high, beta, by_sequence):
+        lib = _lib.load()
+        b, t, v = logits.shape
+        logits, lb, lt = _class_rows(logits)
+        out = torch.empty(3, device=logits.device, dtype=torch.float32)
+        stats = coef = grad = None
+        if ctx.needs_input_grad[0]:
+            stats = torch.empty(b, t, 2, device=logits.device)
+            coef = torch.empty(b, t, device=logits.device)
+            grad = _class_grad(logits, lb, lt)
+        if b * t:
+            nbytes = lib.pp_clipped_policy_loss_workspace_bytes(b, t)
+            ws = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
+            with torch.cuda.device(logits.device):
+                rc = lib.pp_clipped_policy_loss_fwd(
+                    _ptr(logits), lb, lt, _ELEMENT[logits.dtype], _ptr(tokens), _ptr(mask), _ptr(old),
+                    _ptr(adv), adv.stride(0), adv.stride(1), _ptr(ref), low, high, beta, by_sequence,
+                    _ptr(out), _ptr(stats), _ptr(coef), _ptr(grad), _ptr(ws), nbytes, b, t, v,
+                    _stream(logits.device))
+            _lib.check(rc, "pp_clipped_policy_loss_fwd")
+        else:
+            out.zero_()
+        if grad is not None:
+            ctx.save_for_backward(logits, tokens, mask, stats, coef)
+            ctx.grad, ctx.strides = grad, (lb, lt)
+        loss, kl, clipped = out[0], out[1], out[2]
+        ctx.mark_non_differentiable(kl, clipped)
+        return loss, kl, clipped
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gloss, _gkl, _gclipped):
+        logits, tokens, mask, stats, coef = ctx.saved_tensors
+        grad, ctx.grad = ctx.grad, None
+        done = int(grad is not None)
+        if grad is None:
+            grad = _class_grad(logits, *ctx.strides)
+        gout = gloss.reshape(1).to(torch.float32).contiguous()
+        _class_backward(logits, tokens, mask, stats, coef, gout, done, grad, ctx.strides)
+        return (grad,) + (None,) * 9
+
+
+def clipped_policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, mask=None,
+                        clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="token"):
+    """(loss, kl, clipped) of the clipped policy loss with a KL term, logits [b, t, v]:
+
+        lp = log softmax(logits)[token];   rho = exp(lp - old_logp)
+        loss = mean(-min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef k)
+        k = exp(ref_logp - lp) - (ref_logp - lp) - 1
+
+    tokens int [b, t]; old_logp, ref_logp fp32 [b, t]; advantages fp32 [b, t], or [b]: one a sequence.
+    mask: bool [b, t], False where a token does not count (nothing of it is read).  The mean is over
+    the tokens that count (reduction "token"), or over the means of the sequences that have any
+    ("sequence"); if none counts, all three are 0.  kl: mean k (0 without ref_logp); clipped: share
+    of the tokens whose ratio was clipped.  Differentiable in the logits; old_logp, advantages and
+    ref_logp are constants."""
+    tokens, mask = _check_classes(logits, tokens, mask)
+    b, t, _ = logits.shape
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"reduction must be 'token' or 'sequence', got {reduction!r}")
+    if not (clip_low >= 0 and clip_high >= 0):
+        raise ValueError(f"clip_low and clip_high must not be negative, got {clip_low}, {clip_high}")
+    if kl_coef != 0 and ref_logp is None:
+        raise ValueError("kl_coef needs ref_logp")
+    _require_aux(old_logp, "old_logp", (b, t), (torch.float32,), logits.device)
+    if isinstance(advantages, torch.Tensor) and advantages.dim() == 1:
+        _require_aux(advantages, "advantages", (b,), (torch.float32,), logits.device)
+        advantages = advantages[:, None].expand(b, t)
+    else:
+        _require_aux(advantages, "advantages", (b, t), (torch.float32,), logits.device)
+    if ref_logp is not None:
+        _require_aux(ref_logp, "ref_logp", (b, t), (torch.float32,), logits.device)
+        ref_logp = ref_logp.detach().contiguous()
+    return ClippedPolicyLossFunction.apply(
+        logits, tokens, mask, old_logp.detach().contiguous(), advantages.detach(), ref_logp,
+        float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"))
+
+
+def dense_storage(t: torch.Tensor) -> bool:
+    """The tensor's elements fill numel() consecutive storage slots (any permutation of a
+    contiguous tensor does)."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for st, sz in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if st != expect:
+            return False
+        expect *= sz
+    return True
+
+
+def moment_blocks(numel: int) -> int:
+    """Exponent bytes of an 8-bit moment of numel entries."""
+    return _lib.load().pp_moment_blocks(numel)
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8,
+               weight_decay=1e-2, masters=None, avg_exponents=None, sq_exponents=None, seed=0,
+               grad_scale=None):
+    """One AdamW step (decoupled weight decay) of many tensors in place, a launch for every
+    PP_OPT_MAX_TENSORS of them:
+
+        m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2
+        p = p (1 - lr wd) - lr / (1 - b1^s) * m / (sqrt(v) / sqrt(1 - b2^s) + eps)
+
+    Lists of equal length; params and grads of one dtype.  fp32 params are updated as they are;
+    bf16 and fp16 params need `masters`, fp32 tensors that hold the weights, and receive them
+    rounded.  exp_avgs, exp_avg_sqs: fp32, or uint8 codes with avg_exponents and sq_exponents, uint8
+    [moment_blocks(numel)] (all zero at first); their rounding is stochastic, drawn from `seed`, the
+    step and the place.  Every tensor has the strides of its param, which may be any dense order.
+    steps: the number of this step (1, 2, ...) or a device int64 counter that is advanced by the call
+    (under graph capture), for all or a list of one each.  grad_scale: device fp32 scalar that the
+    gradients are multiplied by."""
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    n = len(params)
+    if not n:
+        return
+    eight = avg_exponents is not None or sq_exponents is not None
+    if eight and (avg_exponents is None or sq_exponents is None):
+        raise ValueError("adamw_step: 8-bit moments need avg_exponents and sq_exponents")
+    lists = [("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs)]
+    for name, x in (("masters", masters), ("avg_exponents", avg_exponents), ("sq_exponents", sq_exponents)):
+        if x is not None:
+            lists.append((name, list(x)))
+    for name, x in lists:
+        if len(x) != n:
+            raise ValueError(f"adamw_step: {len(x)} {name} for {n} params")
+    steps = list(steps) if isinstance(steps, (list, tuple)) else [steps] * n
+    counted = isinstance(steps[0], torch.Tensor)
+    if len(steps) != n or any(isinstance(s, torch.Tensor) != counted for s in steps):
+        raise ValueError("adamw_step: steps is one number or counter, or a list of one each")
+    b1, b2 = betas
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+        raise ValueError(f"adamw_step: betas must lie in [0, 1), got {betas}")
+    first = params[0]
+    _require_element(first, "params[0]")
+    dtype, device = first.dtype, first.device
+    if (masters is not None) != (dtype != torch.float32):
+        raise ValueError("adamw_step: masters belong to bfloat16 and float16 params, and these need them")
+    moment = torch.uint8 if eight else torch.float32
+    wanted = {"grads": dtype, "exp_avgs": moment, "exp_avg_sqs": moment, "masters": torch.float32}
+    for i, p in enumerate(params):
+        if p.dtype != dtype or p.device != device:
+            raise TypeError(f"adamw_step: params[{i}] is {p.dtype} on {p.device}, params[0] {dtype} on {device}")
+        stride = p.stride()
+        if not p.is_contiguous() and not dense_storage(p):
+            raise ValueError(f"adamw_step: params[{i}] has gaps or overlaps (strides {stride})")
+        for name, x in lists:
+            t = x[i]
+            if name in wanted:
+                ok = t.dtype == wanted[name] and t.shape == p.shape and t.stride() == stride
+            else:
+                ok = t.dtype == torch.uint8 and t.is_contiguous() and t.numel() == -(-p.numel() // 256)
+            if not ok or t.device != device:
+                raise ValueError(f"adamw_step: {name}[{i}] ({t.dtype}, {tuple(t.shape)}, strides {t.stride()}, "
+                                 f"{t.device}) does not fit params[{i}] ({dtype}, {tuple(p.shape)}, {stride}, {device})")
+    ptrs = [p.data_ptr() for p in params]
+    if len({q for q, p in zip(ptrs, params) if p.numel()}) < sum(p.numel() > 0 for p in params):
+        raise ValueError("adamw_step: a param is in the list twice")
+    if grad_scale is not None:
+        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != device:
+            raise ValueError("adamw_step: grad_scale is one float32 on the device of the params")
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        stream = _stream(device)
+        if counted:
+            unique = list({s.data_ptr(): s for s in steps}.values())
+            for s in unique:
+                if s.dtype != torch.int64 or s.numel() != 1 or s.device != device:
+                    raise ValueError("adamw_step: a step counter is one int64 on the device of the params")
+            for lo in range(0, len(unique), _lib.OPT_MAX_TENSORS):
+                part = unique[lo:lo + _lib.OPT_MAX_TENSORS]
+                rc = lib.pp_count_step(len(part), (c_void_p * len(part))(*[s.data_ptr() for s in part]), stream)
+                _lib.check(rc, "pp_count_step")
+            torch._C._increment_version(unique)
+        elif min(steps) < 1:
+            raise ValueError("adamw_step: steps are counted from 1")
+        table = {name: [t.data_ptr() for t in x] for name, x in lists}
+        live = [i for i in range(n) if params[i].numel()]
+        for lo in range(0, len(live), _lib.OPT_MAX_TENSORS):
+            part = live[lo:lo + _lib.OPT_MAX_TENSORS]
+            k = len(part)
+
+            def array(values, kind=c_void_p):
+                return None if values is None else (kind * k)(*[values[i] for i in part])
+
+            rc = lib.pp_adamw_step(
+                k, _ELEMENT[dtype], 8 if eight else 32, array(ptrs), array(table["grads"]),
+                array(table.get("masters")), array(table["exp_avgs"]), array(table["exp_avg_sqs"]),
+                array(table.get("avg_exponents")), array(table.get("sq_exponents")),
+                array([p.numel() for p in params], ctypes.c_int64),
+                None if counted else array(steps, ctypes.c_int64),
+                array([s.data_ptr() for s in steps]) if counted else None,
+                lr, b1, b2, eps, weight_decay, _ptr(grad_scale), seed & 0xFFFFFFFF, lo, stream)
+            _lib.check(rc, "pp_adamw_step")
+    # written through raw pointers: tell autograd and the pre-split weight cache
+    torch._C._increment_version(params + [t for name, x in lists if name != "grads" for t in x])
+
+
+def decode_moment(codes, exponents, signed: bool, dtype=torch.float32):
+    """The values of an 8-bit moment (adamw_step): codes uint8 in any dense order, exponents uint8
+    [moment_blocks(numel)]; signed for the first moment, unsigned for the second."""
+    if not isinstance(codes, torch.Tensor) or not codes.is_cuda:
+        raise RuntimeError("decode_moment: codes must be on the GPU")
+    if dtype not in _ELEMENT:
+        raise TypeError(f"decode_moment: float32, bfloat16 or float16, got {dtype}")
+    if codes.dtype != torch.uint8 or not dense_storage(codes):
+        raise ValueError("decode_moment: codes must be uint8 without gaps")
+    _require_aux(exponents, "exponents", (-(-codes.numel() // 256),), (torch.uint8,), codes.device)
+    out = torch.empty_like(codes, dtype=dtype)
+    if codes.numel():
+        lib = _lib.load()
+        exponents = exponents.contiguous()
+        with torch.cuda.device(codes.device):
+            rc = lib.pp_decode_moment(_ptr(codes), _ptr(exponents), _ptr(out), _ELEMENT[dtype],
+                                      int(signed), codes.numel(), _stream(codes.device))
+        _lib.check(rc, "pp_decode_moment")
+    return out

@@ -10,7 +10,7 @@ examples/high_order_interpolation.py) reduced to what feeds the hot path:
                       ``${a.b}`` interpolation, with PyYAML only;
 * ``select_network``  ``net.model_type`` ``high_order`` and ``high_order_input``;
 * ``ASCIIPredictionNet``  cross-entropy + accuracy = mean(argmax == y), optimizers
-                      ``adam`` / ``lion`` / ``sparse_lion``;
+                      ``adam`` / ``adamw`` / ``adamw_8bit`` / ``lion`` / ``sparse_lion``;
 * ``CharWindows``     text -> uint8 buffer ON THE DEVICE -> windows gathered on the GPU,
                       ``x = (c - 64 + 0.5)/64`` (single_text_dataset.py:15-16, :102-123
                       builds the same windows as Python lists);
@@ -275,6 +275,104 @@ class Lion(torch.optim.Optimizer):
         return loss
 
 
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with the whole step of a parameter group in one launch for every
+    PP_OPT_MAX_TENSORS tensors (functional.adamw_step).  GPU parameters in fp32, or in bf16 / fp16 with
+    an fp32 master in the state; dense in any order (the layers' parameters are permuted leaves).
+
+    moment_bits=8 keeps both moments in one byte an entry (tensors under MIN_8BIT entries stay in 32
+    bits: they are most of the tensors and none of the memory); `seed` is that of their rounding.
+    capturable: the step numbers are device counters, so that a captured step counts its replays.
+    step(grad_scale=t): gradients are multiplied by the device scalar t first."""
+
+    MIN_8BIT = 4096
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 moment_bits=32, capturable=False, seed=0):
+        if moment_bits not in (8, 32):
+            raise ValueError(f"moment_bits must be 8 or 32, got {moment_bits}")
+        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"AdamW: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      moment_bits=moment_bits, capturable=capturable, seed=seed))
+
+    def _init_state(self, p, group):
+        st = self.state[p]
+        if not p.is_cuda:
+            raise RuntimeError(f"AdamW: a parameter is on {p.device}; the step runs on MI355X (HIP) only")
+        if not PF.dense_storage(p):
+            raise ValueError(f"AdamW: a parameter has gaps or overlaps (strides {p.stride()})")
+        st["step"] = torch.zeros((), dtype=torch.int64, device=p.device) if group["capturable"] else 0
+        eight = group["moment_bits"] == 8 and p.numel() >= self.MIN_8BIT
+        for name in ("exp_avg", "exp_avg_sq"):
+            st[name] = torch.zeros_like(p, dtype=torch.uint8 if eight else torch.float32)
+            if eight:
+                st[name + "_exponent"] = torch.zeros(PF.moment_blocks(p.numel()), dtype=torch.uint8,
+                                                     device=p.device)
+        if p.dtype != torch.float32:
+            st["master"] = p.detach().float()
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for index, group in enumerate(self.param_groups):
+            if not group["capturable"] and torch.cuda.is_available() and \
+                    torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a step that is captured into a graph needs capturable=True "
+                                   "(the step number would be frozen)")
+            kinds = {}
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("AdamW: sparse gradients are not supported")
+                st = self.state[p] or self._init_state(p, group)
+                if not group["capturable"]:
+                    st["step"] += 1
+                if g.stride() != p.stride():  # one order for all that belongs to a parameter
+                    g = torch.empty_like(p).copy_(g)
+                kinds.setdefault((p.device, p.dtype, "exp_avg_exponent" in st), []).append((p, g, st))
+            for k, ((_, dtype, eight), todo) in enumerate(kinds.items()):
+                PF.adamw_step(
+                    [p for p, _, _ in todo], [g for _, g, _ in todo],
+                    [st["exp_avg"] for _, _, st in todo], [st["exp_avg_sq"] for _, _, st in todo],
+                    [st["step"] for _, _, st in todo], lr=group["lr"], betas=group["betas"],
+                    eps=group["eps"], weight_decay=group["weight_decay"],
+                    masters=None if dtype == torch.float32 else [st["master"] for _, _, st in todo],
+                    avg_exponents=[st["exp_avg_exponent"] for _, _, st in todo] if eight else None,
+                    sq_exponents=[st["exp_avg_sq_exponent"] for _, _, st in todo] if eight else None,
+                    seed=group["seed"] + 8191 * index + k, grad_scale=grad_scale)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As the base class, but the state keeps its own types (the base class would cast codes,
+        moments and masters to the parameter's) and its own order of the entries."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [(p, g) for g in self.param_groups for p in g["params"]]
+        for i, (p, group) in zip(saved, mine):
+            old = state_dict["state"].get(i)
+            if not old:
+                continue
+            st = {}
+            for name, x in old.items():
+                if name == "step":
+                    x = int(x)
+                    st[name] = torch.tensor(x, device=p.device) if group["capturable"] else x
+                elif x.shape == p.shape and not name.endswith("_exponent"):
+                    if x.dtype == torch.uint8 and x.stride() != p.stride():
+                        raise ValueError("AdamW: 8-bit moments belong to another order of the entries")
+                    st[name] = torch.empty_like(p, dtype=x.dtype).copy_(x)
+                else:
+                    st[name] = x.to(p.device, copy=True)
+            self.state[p] = st
+
+
 class ASCIIPredictionNet(nn.Module):
     """`ASCIIPredictionNet` without Lightning: ``self.model`` + cross entropy."""
 
@@ -302,6 +400,9 @@ class ASCIIPredictionNet(nn.Module):
             return Lion(self.parameters(), lr=opt.lr, weight_decay=0.0)
         if opt.name == "sparse_lion":
             return Lion(self.parameters(), lr=opt.lr, weight_decay=0.0, sparse=True)
+        if opt.name in ("adamw", "adamw_8bit"):
+            return AdamW(self.parameters(), lr=opt.lr, weight_decay=opt.get("weight_decay", 1e-2),
+                         moment_bits=8 if opt.name == "adamw_8bit" else 32, capturable=capturable)
         raise ValueError(f"Optimizer {opt.name} not recognized")
 
 
@@ -466,10 +567,10 @@ class GraphedTrainStep:
         with torch.no_grad():
             for p, q in zip(module.parameters(), saved):
                 p.copy_(q)
-            for st in optimizer.state.values():
-                for v in st.values():
+            for p, st in optimizer.state.items():
+                for k, v in st.items():
                     if torch.is_tensor(v):
-                        v.zero_()
+                        v.copy_(p) if k == "master" else v.zero_()
         optimizer.zero_grad(set_to_none=True)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
