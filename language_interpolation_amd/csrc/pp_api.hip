@@ -875,7 +875,8 @@ static size_t elem_size(int dtype) { return dtype == PP_F32 ? 4 : 2; }
 static int rec_args_ok(int dtype, int b, int l, int d) {
   if (!elem_ok(dtype)) return PP_ERR_METHOD;
   if (b < 1 || l < 1 || d < 1 || b > 65535) return PP_ERR_SHAPE;
-  if ((int64_t)b * l >= (1LL << 31) || (int64_t)l + 4096 >= (1LL << 31) || d > (1 << 24))
+  if ((int64_t)b * l >= (1LL << 31) || (int64_t)l + 4096 >= (1LL << 31) || d > (1 << 24) ||
+      (int64_t)b * ((l + 127) / 128) * ((d + 63) / 64) >= (1LL << 31))  // workgroups
     return PP_ERR_RANGE;
   return PP_OK;
 }

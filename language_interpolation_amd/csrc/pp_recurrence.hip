@@ -1,17 +1,33 @@
 // Gated linear recurrence, forward and backward, and its single-token step.
 //
-//   a_t = sigmoid(f_t);   h_t = a_t h_{t-1} + (1 - a_t) z_t = z_t + a_t (h_{t-1} - z_t)
+//   a_t = sigmoid(f_t);   h_t = a_t h_{t-1} + (1 - a_t) z_t
 //
 // per channel, z and f [b][l][d] in fp32, bf16 or fp16, the state in fp32.  reset[b][t] != 0 drops
 // the state before step t (h_{t-1} := 0: a new document); steps from lengths[b] on do not exist
 // (y = 0, gradients 0, nothing read), the state stays as it is.  Backward, with e_t = dL/dh_t:
 //
-//   e_t = gy_t + a_{t+1} e_{t+1}  (a := 0 at a reset, gh_last arrives behind the last step)
+//   e_t = gy_t + u_t;  u_{t-1} = a_t e_t  (0 at a reset; u = gh_last behind the last step)
 //   gz_t = e_t (1 - a_t);   gf_t = e_t a_t (1 - a_t) (h_{t-1} - z_t);   gh0 = a_0 e_0
 //
-// 1 - a is computed as sigmoid(-f), so neither gate loses its small end to cancellation.
-// The forward of a training step keeps h at the start of every kSteps steps in fp32 (the states
-// in between are recomputed from it; y, rounded to 16 bits, would not do for the differences).
+// 1 - a is sigmoid(-f), so neither gate loses its small end to cancellation; a step keeps the
+// smaller of the two, with its sign telling which it is, and the other is 1 minus it.
+//
+// Split of the length.  A step is linear in the state, so a stretch of steps is h_out = P h_in + H
+// with P the product of its a and H its result from 0.  A wave takes kSteps steps x 64 V channels:
+// it loads them once (16 loads of each input in flight), keeps gates and candidates in registers,
+// computes (P, H), and, once h_in is known, walks the steps again from registers.  The waves of a
+// workgroup are consecutive stretches, joined through LDS; the workgroups of a row (chunks) are
+// joined through global memory: each publishes its (P, H) as soon as it has it, then looks back for
+// the nearest chunk whose final state is known and applies the (P, H) of those in between, in
+// order -- the same fma of each chunk whoever applies it, so results do not depend on timing.
+//   Waiting is safe: a workgroup draws its chunk from a counter, chunks in the order of the chain,
+// so it waits only for workgroups that are running already and that publish before they wait.
+//   The published words carry their own readiness (all ones = not yet, the fill before the launch),
+// read and written with device-scope atomics; no other data travels between workgroups, so no fence
+// (on this chip a release would write back an XCD's L2) is needed.
+//   A reset makes P = -0.0, which no product of gates is: it cuts even a state that is NaN.
+// The forward of a training step keeps h at the start of every kSteps steps in fp32 (the states in
+// between are recomputed from it; y, rounded to 16 bits, would not do for the differences).
 #include <algorithm>
 
 #include "pp_device.h"
@@ -19,130 +35,581 @@
 
 namespace {
 
-constexpr int kSteps = PP_RECURRENCE_STEPS;  // steps between two kept states
+constexpr int kSteps = PP_RECURRENCE_STEPS;  // steps of a wave, and between two kept states
+constexpr int kWaves = 8;                    // waves (stretches) of a workgroup
+constexpr int kChunk = kSteps * kWaves;
+constexpr uint32_t kNotYet = 0xffffffffu;
 
 struct RecArgs {
   int64_t zb, zl, fb, fl, gb, gl;  // strides in elements of z, f and gy over batch and time
   int b, l, d;
+  int nchunk, ngroup;  // chunks of a row, groups of 64 V channels
   const float* h0;
   const int32_t* lengths;
   const uint8_t* reset;
+  uint32_t* ticket;
+  unsigned long long* part;  // [chain][chunk][64 V]: (P, H) of a chunk
+  uint32_t* done;            // [chain][chunk][64 V]: state behind it
 };
 
-__device__ __forceinline__ void gates(float f, float& a, float& r) {
-  const float x = expf(-fabsf(f));  // in (0, 1]: neither gate overflows
-  const float big = 1.0f / (1.0f + x), small = x * big;
-  a = f >= 0.0f ? big : small;
-  r = f >= 0.0f ? small : big;
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void pp_rec_fwd_kernel(const T* __restrict__ z,
-                                                        const T* __restrict__ f, T* __restrict__ y,
-                                                        float* __restrict__ h_last,
-                                                        float* __restrict__ starts, RecArgs p) {
-  const int ch = blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-  if (ch >= p.d) return;
-  const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
-  const int nchunk = (p.l + kSteps - 1) / kSteps;
-  float h = p.h0 ? p.h0[(int64_t)b * p.d + ch] : 0.0f;
-  for (int t = 0; t < p.l; ++t) {
-    if (starts && t % kSteps == 0) starts[((int64_t)b * nchunk + t / kSteps) * p.d + ch] = h;
-    float out = 0.0f;
-    if (t < len) {
-      float a, r;
-      gates((float)f[b * p.fb + t * p.fl + ch], a, r);
-      if (p.reset && p.reset[(int64_t)b * p.l + t]) h = 0.0f;
-      h = fmaf(a, h, r * (float)z[b * p.zb + t * p.zl + ch]);
-      out = h;
-    }
-    y[((int64_t)b * p.l + t) * p.d + ch] = (T)out;
+// The smaller gate with a sign: r = sigmoid(-f) for f >= 0, -a for f < 0.
+template <bool EXACT>
+__device__ __forceinline__ float gate_code(float f) {
+  const float s = -fabsf(f);
+  float x;
+  if (EXACT) {  // the rounding of s log2(e) is made good: matters for |f| >> 1 in fp32
+    const float hi = s * 1.44269502f;
+    const float lo = fmaf(s, 1.92596299e-8f, fmaf(s, 1.44269502f, -hi));
+    x = __builtin_amdgcn_exp2f(hi);
+    x = fmaf(x * 0.693147182f, lo, x);
+    x = s < -200.0f ? 0.0f : x;  // (also -inf, whose lo is NaN)
+  } else {
+    x = __builtin_amdgcn_exp2f(s * 1.44269502f);
   }
-  h_last[(int64_t)b * p.d + ch] = h;
+  const float small = x * __builtin_amdgcn_rcpf(1.0f + x);
+  return f >= 0.0f ? small : (f < 0.0f ? -small : f);  // NaN stays NaN
+}
+__device__ __forceinline__ void gates(float q, float& a, float& r) {
+  const float small = fabsf(q), big = 1.0f - small;
+  // (q = -0.0 is the open gate's underflow: a = 0)
+  const bool neg = __float_as_uint(q) >> 31;
+  a = neg ? small : big;
+  r = neg ? big : small;
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void pp_rec_bwd_kernel(
+// state behind a stretch (P, H) from the state before it
+__device__ __forceinline__ float through(float P, float H, float h) {
+  return __float_as_uint(P) == 0x80000000u ? H : fmaf(P, h, H);
+}
+
+__device__ __forceinline__ uint32_t word_of(float x) {
+  return x != x ? 0x7fc00000u : __float_as_uint(x);  // one NaN: never kNotYet
+}
+
+// The state behind chunk `last` of a chain that begins with chunk `first` (which publishes its state
+// without waiting); one wave, V channels a lane, kWindow chunks looked at together.
+template <int kWindow, int V>
+__device__ __forceinline__ void look_back(const RecArgs& p, int64_t chain, int first, int last,
+                                          float (&h)[V]) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t* done = p.done + chain * p.nchunk * (64 * V) + lane;
+  const unsigned long long* part = p.part + chain * p.nchunk * (64 * V) + lane;
+  int k = last;
+  for (bool found = false; !found;) {  // the nearest chunk whose state is known
+    uint32_t w[kWindow][V];
+#pragma unroll
+    for (int j = 0; j < kWindow; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        w[j][v] = __hip_atomic_load(done + (int64_t)max(k - j, first) * (64 * V) + v * 64, __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int j = 0; j < kWindow; ++j) {
+      if (found) continue;
+      bool ready = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) ready = ready && w[j][v] != kNotYet;
+      if (__all(ready)) {
+        found = true;
+        k = max(k - j, first);
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = __uint_as_float(w[j][v]);
+      }
+    }
+    if (!found) {
+      if (k - kWindow < first) {  // not even the first: wait and start again from the near end
+        __builtin_amdgcn_s_sleep(2);
+        k = last;
+      } else {
+        k -= kWindow;
+      }
+    }
+  }
+  while (k < last) {  // ... and on from there, chunk by chunk
+    const int n = min(kWindow, last - k);
+    unsigned long long w[kWindow][V];
+#pragma unroll
+    for (int j = 0; j < kWindow; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        w[j][v] = __hip_atomic_load(part + (int64_t)min(k + 1 + j, last) * (64 * V) + v * 64,
+                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int used = 0;
+#pragma unroll
+    for (int j = 0; j < kWindow; ++j) {
+      bool ready = j < n && used == j;
+#pragma unroll
+      for (int v = 0; v < V; ++v) ready = ready && (uint32_t)w[j][v] != kNotYet;
+      if (__all(ready)) {
+        used = j + 1;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          h[v] = through(__uint_as_float((uint32_t)w[j][v]), __uint_as_float((uint32_t)(w[j][v] >> 32)), h[v]);
+      }
+    }
+    k += used;
+    if (!used) __builtin_amdgcn_s_sleep(1);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void publish_part(const RecArgs& p, int64_t chain, int c, const float (&P)[V],
+                                             const float (&H)[V]) {
+  unsigned long long* at = p.part + (chain * p.nchunk + c) * (64 * V) + (threadIdx.x & 63);
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    __hip_atomic_store(at + v * 64, (unsigned long long)word_of(P[v]) | (unsigned long long)word_of(H[v]) << 32,
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <int V>
+__device__ __forceinline__ void publish_done(const RecArgs& p, int64_t chain, int c, const float (&h)[V]) {
+  uint32_t* at = p.done + (chain * p.nchunk + c) * (64 * V) + (threadIdx.x & 63);
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    __hip_atomic_store(at + v * 64, word_of(h[v]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__global__ __launch_bounds__(256) void pp_rec_fill_kernel(uint32_t* __restrict__ ws, int64_t words) {
+  const int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (i + j * 256 < words) ws[i + j * 256] = i + j * 256 < 4 ? 0u : kNotYet;  // the counter, then the rest
+}
+
+// bits j: step t0 + j starts a document
+__device__ __forceinline__ uint32_t reset_bits(const uint8_t* reset, int64_t row, int t0, int n) {
+  if (!reset) return 0u;
+  const int lane = threadIdx.x & 63;
+  const bool on = lane < n && reset[row + t0 + lane] != 0;
+  return (uint32_t)__ballot(on);
+}
+
+// this workgroup's chunk (counted along the chain), channel group and row
+__device__ __forceinline__ void draw_tile(const RecArgs& p, int* shared, int& c, int& g, int& b) {
+  int id = blockIdx.x;
+  if (p.nchunk > 1) {
+    if (threadIdx.x == 0) *shared = (int)atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    id = __builtin_amdgcn_readfirstlane(*shared);
+  }
+  const int chains = p.ngroup * p.b;
+  c = id / chains;
+  b = (id % chains) / p.ngroup;
+  g = id % p.ngroup;
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_fwd_kernel(const T* __restrict__ z,
+                                                                 const T* __restrict__ f,
+                                                                 T* __restrict__ y,
+                                                                 float* __restrict__ h_last,
+                                                                 float* __restrict__ starts, RecArgs p) {
+  typedef PPElems<T, V> E;
+  __shared__ float2 part[kWaves][V][64];
+  __shared__ float carry[V][64];
+  __shared__ int drawn;
+  int c, g, b;
+  draw_tile(p, &drawn, c, g, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int ch = (g * 64 + lane) * V;
+  const bool live = ch < p.d;
+  const int chl = live ? ch : 0;  // a lane without channels reads some and writes nothing
+  const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
+  const int t0 = c * kChunk + wave * kSteps;
+  const int n = max(0, min(kSteps, len - t0));        // steps of this wave that exist
+  const int rows = max(0, min(kSteps, p.l - t0));     // rows of y to write
+  const int64_t chain = (int64_t)b * p.ngroup + g;
+  const int64_t row0 = (int64_t)b * p.l + t0;
+
+  float q[kSteps][V];
+  typename E::raw zr[kSteps];
+  float P[V], H[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    P[v] = 1.0f;
+    H[v] = 0.0f;
+  }
+  uint32_t cut = 0;
+  if (n > 0) {
+    cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
+    const T* zp = z + b * p.zb + t0 * p.zl + chl;
+    const T* fp = f + b * p.fb + t0 * p.fl + chl;
+    typename E::raw fr[kSteps];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      const int64_t t = min(j, n - 1);
+      fr[j] = E::load(fp + t * p.fl);
+      zr[j] = E::load(zp + t * p.zl);
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      float fv[V], zv[V];
+      E::get(fr[j], fv);
+      E::get(zr[j], zv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        q[j][v] = gate_code<sizeof(T) == 4>(fv[v]);
+        float a, r;
+        gates(q[j][v], a, r);
+        if (j < n) {
+          if (cut >> j & 1) {
+            P[v] = -0.0f;
+            H[v] = 0.0f;
+          }
+          H[v] = fmaf(a, H[v], r * zv[v]);
+          P[v] *= a;
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) part[wave][v][lane] = make_float2(P[v], H[v]);
+  __syncthreads();
+  const bool alone = p.nchunk == 1;
+  if (wave == 0) {  // the state before this chunk
+    float h[V];
+    if (c == 0 || c * kChunk >= len) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = p.h0 && live ? p.h0[(int64_t)b * p.d + ch + v] : 0.0f;
+    }
+    if (c * kChunk < len && !alone) {
+      const bool more = (c + 1) * kChunk < len;  // someone waits for it
+      float CP[V], CH[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        CP[v] = part[0][v][lane].x;
+        CH[v] = part[0][v][lane].y;
+        for (int w = 1; w < waves; ++w) {
+          const float2 s = part[w][v][lane];
+          CH[v] = through(s.x, s.y, CH[v]);
+          CP[v] = __float_as_uint(s.x) == 0x80000000u ? s.x : CP[v] * s.x;
+        }
+      }
+      if (c > 0) {
+        if (more) publish_part<V>(p, chain, c, CP, CH);
+        look_back<8, V>(p, chain, 0, c - 1, h);
+      }
+      if (more) {
+        float out[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] = through(CP[v], CH[v], h[v]);
+        publish_done<V>(p, chain, c, out);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v][lane] = h[v];
+  }
+  __syncthreads();
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    h[v] = carry[v][lane];
+    for (int w = 0; w < wave; ++w) h[v] = through(part[w][v][lane].x, part[w][v][lane].y, h[v]);
+  }
+  if (!live) return;
+  if (starts && n > 0) {
+    float* at = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d + ch;
+#pragma unroll
+    for (int v = 0; v < V; ++v) at[v] = h[v];
+  }
+  T* yp = y + row0 * p.d + ch;
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    float out[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = 0.0f;
+    if (j < n) {
+      float zv[V];
+      E::get(zr[j], zv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float a, r;
+        gates(q[j][v], a, r);
+        if (cut >> j & 1) h[v] = 0.0f;
+        h[v] = fmaf(a, h[v], r * zv[v]);
+        out[v] = h[v];
+      }
+    }
+    if (j < rows) E::store(yp + (int64_t)j * p.d, E::put(out));
+  }
+  if ((n > 0 && t0 + n == len) || (len == 0 && c == 0 && wave == 0)) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) h_last[(int64_t)b * p.d + ch + v] = h[v];
+  }
+}
+
+// Chunks are counted from the end of the (allocated) row: chunk c of the chain is row chunk
+// nchunk - 1 - c; those behind the end of a shorter row only write zeros.
+template <typename T, int V>
+__global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_bwd_kernel(
     const T* __restrict__ z, const T* __restrict__ f, const float* __restrict__ starts,
     const T* __restrict__ gy, const float* __restrict__ gh, T* __restrict__ gz, T* __restrict__ gf,
     float* __restrict__ gh0, RecArgs p) {
-  const int ch = blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-  if (ch >= p.d) return;
+  typedef PPElems<T, V> E;
+  __shared__ float2 part[kWaves][V][64];
+  __shared__ float carry[V][64];
+  __shared__ int drawn;
+  int c, g, b;
+  draw_tile(p, &drawn, c, g, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int ch = (g * 64 + lane) * V;
+  const bool live = ch < p.d;
+  const int chl = live ? ch : 0;
   const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
-  const int nchunk = (p.l + kSteps - 1) / kSteps;
-  float u = gh ? gh[(int64_t)b * p.d + ch] : 0.0f;  // a_{t+1} e_{t+1}
-  for (int c = nchunk - 1; c >= 0; --c) {
-    const int t0 = c * kSteps;
-    float prev[kSteps];
-    float h = starts[((int64_t)b * nchunk + c) * p.d + ch];
+  const int chunk0 = (p.nchunk - 1 - c) * kChunk;  // first step of the chunk
+  const int t0 = chunk0 + wave * kSteps;
+  const int n = max(0, min(kSteps, len - t0));
+  const int rows = max(0, min(kSteps, p.l - t0));
+  const int64_t chain = (int64_t)b * p.ngroup + g;
+  const int64_t row0 = (int64_t)b * p.l + t0;
+
+  float q[kSteps][V], gap[kSteps][V];  // gates, h_{t-1} - z_t
+  typename E::raw gr[kSteps];
+  float P[V], G[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    P[v] = 1.0f;
+    G[v] = 0.0f;
+  }
+  uint32_t cut = 0;
+  if (n > 0) {
+    cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
+    const T* zp = z + b * p.zb + t0 * p.zl + chl;
+    const T* fp = f + b * p.fb + t0 * p.fl + chl;
+    const T* gp = gy + b * p.gb + t0 * p.gl + chl;
+    const float* sp = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d + chl;
+    typename E::raw fr[kSteps], zr[kSteps];
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = sp[v];
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
-      const int t = t0 + j;
-      prev[j] = 0.0f;
-      if (t < len) {
+      const int64_t t = min(j, n - 1);
+      fr[j] = E::load(fp + t * p.fl);
+      zr[j] = E::load(zp + t * p.zl);
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) gr[j] = E::load(gp + (int64_t)min(j, n - 1) * p.gl);
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      float fv[V], zv[V];
+      E::get(fr[j], fv);
+      E::get(zr[j], zv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        q[j][v] = gate_code<sizeof(T) == 4>(fv[v]);
         float a, r;
-        gates((float)f[b * p.fb + t * p.fl + ch], a, r);
-        if (p.reset && p.reset[(int64_t)b * p.l + t]) h = 0.0f;
-        prev[j] = h;
-        h = fmaf(a, h, r * (float)z[b * p.zb + t * p.zl + ch]);
+        gates(q[j][v], a, r);
+        if (cut >> j & 1) h[v] = 0.0f;
+        gap[j][v] = h[v] - zv[v];
+        h[v] = fmaf(a, h[v], r * zv[v]);
       }
     }
 #pragma unroll
     for (int j = kSteps - 1; j >= 0; --j) {
-      const int t = t0 + j;
-      if (t >= p.l) continue;
-      const int64_t at = ((int64_t)b * p.l + t) * p.d + ch;
-      float oz = 0.0f, of = 0.0f;
-      if (t < len) {
+      if (j >= n) continue;
+      float gv[V];
+      E::get(gr[j], gv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
         float a, r;
-        gates((float)f[b * p.fb + t * p.fl + ch], a, r);
-        const float e = (float)gy[b * p.gb + t * p.gl + ch] + u;
-        oz = e * r;
-        of = e * (a * r) * (prev[j] - (float)z[b * p.zb + t * p.zl + ch]);
-        u = p.reset && p.reset[(int64_t)b * p.l + t] ? 0.0f : a * e;
+        gates(q[j][v], a, r);
+        G[v] = a * (gv[v] + G[v]);
+        P[v] *= a;
+        if (cut >> j & 1) {
+          P[v] = -0.0f;
+          G[v] = 0.0f;
+        }
       }
-      gz[at] = (T)oz;
-      gf[at] = (T)of;
     }
   }
-  if (gh0) gh0[(int64_t)b * p.d + ch] = u;
+#pragma unroll
+  for (int v = 0; v < V; ++v) part[wave][v][lane] = make_float2(P[v], G[v]);
+  __syncthreads();
+  if (wave == 0) {  // the gradient that arrives behind this chunk
+    float u[V];
+    const int first = p.nchunk - (len + kChunk - 1) / kChunk;  // the chain's chunk with the last step
+    if (c <= first) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) u[v] = gh && live ? gh[(int64_t)b * p.d + ch + v] : 0.0f;
+    }
+    if (chunk0 < len && p.nchunk > 1) {
+      const bool more = chunk0 > 0;
+      float CP[V], CG[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        CP[v] = part[waves - 1][v][lane].x;
+        CG[v] = part[waves - 1][v][lane].y;
+        for (int w = waves - 2; w >= 0; --w) {
+          const float2 s = part[w][v][lane];
+          CG[v] = through(s.x, s.y, CG[v]);
+          CP[v] = __float_as_uint(s.x) == 0x80000000u ? s.x : CP[v] * s.x;
+        }
+      }
+      if (c > first) {
+        if (more) publish_part<V>(p, chain, c, CP, CG);
+        look_back<4, V>(p, chain, first, c - 1, u);
+      }
+      if (more) {
+        float out[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) out[v] = through(CP[v], CG[v], u[v]);
+        publish_done<V>(p, chain, c, out);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v][lane] = u[v];
+  }
+  __syncthreads();
+  float u[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    u[v] = carry[v][lane];
+    for (int w = waves - 1; w > wave; --w) u[v] = through(part[w][v][lane].x, part[w][v][lane].y, u[v]);
+  }
+  if (!live) return;
+  T* gzp = gz + row0 * p.d + ch;
+  T* gfp = gf + row0 * p.d + ch;
+#pragma unroll
+  for (int j = kSteps - 1; j >= 0; --j) {
+    float oz[V], of[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) oz[v] = of[v] = 0.0f;
+    if (j < n) {
+      float gv[V];
+      E::get(gr[j], gv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float a, r;
+        gates(q[j][v], a, r);
+        const float e = gv[v] + u[v];
+        oz[v] = e * r;
+        of[v] = (e * gap[j][v]) * (a * r);
+        u[v] = cut >> j & 1 ? 0.0f : a * e;
+      }
+    }
+    if (j < rows) {
+      E::store(gzp + (int64_t)j * p.d, E::put(oz));
+      E::store(gfp + (int64_t)j * p.d, E::put(of));
+    }
+  }
+  if (gh0 && chunk0 == 0 && wave == 0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) gh0[(int64_t)b * p.d + ch + v] = u[v];
+  }
 }
 
-template <typename T>
+template <typename T, int V>
 __global__ __launch_bounds__(256) void pp_rec_step_kernel(const T* __restrict__ z, int64_t zb,
                                                           const T* __restrict__ f, int64_t fb,
                                                           float* __restrict__ h, int64_t hb,
                                                           T* __restrict__ y, int b, int d) {
-  const int ch = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
-  if (ch >= d) return;
-  float a, r;
-  gates((float)f[row * fb + ch], a, r);
-  const float n = fmaf(a, h[row * hb + ch], r * (float)z[row * zb + ch]);
-  h[row * hb + ch] = n;
-  y[(int64_t)row * d + ch] = (T)n;
+  typedef PPElems<T, V> E;
+  typedef PPElems<float, V> EH;
+  const int wide = d / V;  // (V divides d)
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)b * wide) return;
+  const int64_t row = i / wide;
+  const int ch = (int)(i % wide) * V;
+  float zv[V], fv[V], hv[V];
+  E::get(E::load(z + row * zb + ch), zv);
+  E::get(E::load(f + row * fb + ch), fv);
+  EH::get(EH::load(h + row * hb + ch), hv);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float a, r;
+    gates(gate_code<sizeof(T) == 4>(fv[v]), a, r);
+    hv[v] = fmaf(a, hv[v], r * zv[v]);
+  }
+  EH::store(h + row * hb + ch, EH::put(hv));
+  E::store(y + row * d + ch, E::put(hv));
+}
+
+// V elements from every address that `strides` steps away from `at` are one aligned access
+bool fits(int v, size_t size, std::initializer_list<const void*> at, std::initializer_list<int64_t> strides) {
+  for (const void* q : at)
+    if ((size_t)q % (v * size)) return false;
+  for (int64_t s : strides)
+    if (s % v) return false;
+  return true;
+}
+
+int plan(RecArgs& p, int v, void* ws) {  // returns the waves of a workgroup
+  p.ngroup = (p.d + 64 * v - 1) / (64 * v);
+  p.nchunk = (p.l + kChunk - 1) / kChunk;
+  p.ticket = static_cast<uint32_t*>(ws);
+  const int64_t n = (int64_t)p.b * p.nchunk * p.ngroup * 64 * v;
+  p.part = reinterpret_cast<unsigned long long*>(p.ticket + 4);
+  p.done = reinterpret_cast<uint32_t*>(p.part + n);
+  return p.nchunk > 1 ? kWaves : (p.l + kSteps - 1) / kSteps;
+}
+
+void fill(const RecArgs& p, int v, hipStream_t st) {
+  if (p.nchunk == 1) return;
+  const int64_t words = 4 + (int64_t)p.b * p.nchunk * p.ngroup * 64 * v * 3;
+  hipLaunchKernelGGL(pp_rec_fill_kernel, dim3((unsigned)((words + 1023) / 1024)), dim3(256), 0, st,
+                     p.ticket, words);
+}
+
+template <typename T, int V>
+void run_fwd(const void* z, const void* f, void* y, float* h_last, float* starts, RecArgs p, void* ws,
+             hipStream_t st) {
+  const int waves = plan(p, V, ws);
+  fill(p, V, st);
+  hipLaunchKernelGGL((pp_rec_fwd_kernel<T, V>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
+                     dim3(64 * waves), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
+                     static_cast<T*>(y), h_last, starts, p);
+}
+template <typename T, int V>
+void run_bwd(const void* z, const void* f, const float* starts, const void* gy, const float* gh,
+             void* gz, void* gf, float* gh0, RecArgs p, void* ws, hipStream_t st) {
+  const int waves = plan(p, V, ws);
+  fill(p, V, st);
+  hipLaunchKernelGGL((pp_rec_bwd_kernel<T, V>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
+                     dim3(64 * waves), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
+                     starts, static_cast<const T*>(gy), gh, static_cast<T*>(gz), static_cast<T*>(gf),
+                     gh0, p);
+}
+template <typename T, int V>
+void run_step(const void* z, int64_t zb, const void* f, int64_t fb, float* h, int64_t hb, void* y, int b,
+              int d, hipStream_t st) {
+  const int64_t n = (int64_t)b * (d / V);
+  hipLaunchKernelGGL((pp_rec_step_kernel<T, V>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st,
+                     static_cast<const T*>(z), zb, static_cast<const T*>(f), fb, h, hb,
+                     static_cast<T*>(y), b, d);
 }
 
 }  // namespace
 
-#define PP_REC_TYPES(CALL)                 \
-  do {                                     \
-    if (dtype == PP_F32) CALL(float);      \
+#define PP_REC_TYPES(CALL)                    \
+  do {                                        \
+    if (dtype == PP_F32) CALL(float);         \
     else if (dtype == PP_BF16) CALL(pp_bf16); \
-    else CALL(pp_f16);                     \
-    return hipGetLastError();              \
+    else CALL(pp_f16);                        \
+    return hipGetLastError();                 \
   } while (0)
 
-size_t pp_rec_workspace_bytes(int b, int l, int d) { return 0; }
+size_t pp_rec_workspace_bytes(int b, int l, int d) {
+  const int64_t nchunk = ((int64_t)l + kChunk - 1) / kChunk;
+  if (nchunk == 1) return 0;
+  return 16 + (size_t)b * nchunk * (((size_t)d + 255) / 256 * 256) * 12;
+}
 
 hipError_t pp_launch_rec_fwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
                              int64_t fl, int dtype, const float* h0, const int32_t* lengths,
                              const uint8_t* reset, void* y, float* h_last, float* starts, void* ws,
                              int b, int l, int d, hipStream_t st) {
-  const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, h0, lengths, reset};
-#define PP_CALL(T)                                                                             \
-  hipLaunchKernelGGL((pp_rec_fwd_kernel<T>), dim3((d + 63) / 64, b), dim3(64), 0, st,          \
-                     static_cast<const T*>(z), static_cast<const T*>(f), static_cast<T*>(y),   \
-                     h_last, starts, p)
+  const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, 0, 0, h0, lengths, reset, nullptr, nullptr, nullptr};
+  const size_t s = dtype == PP_F32 ? 4 : 2;
+  int v = 2;
+  while (v > 1 && !fits(v, s, {z, f, y}, {zb, zl, fb, fl, (int64_t)d})) v /= 2;
+#define PP_CALL(T)                                                             \
+  do {                                                                         \
+    if (v == 2)                                                           \
+      run_fwd<T, 2>(z, f, y, h_last, starts, p, ws, st);                       \
+    else                                                                       \
+      run_fwd<T, 1>(z, f, y, h_last, starts, p, ws, st);                       \
+  } while (0)
   PP_REC_TYPES(PP_CALL);
 #undef PP_CALL
 }
@@ -152,22 +619,31 @@ hipError_t pp_launch_rec_bwd(const void* z, int64_t zb, int64_t zl, const void* 
                              const float* starts, const void* gy, int64_t gb, int64_t gl,
                              const float* gh_last, void* gz, void* gf, float* gh0, void* ws, int b,
                              int l, int d, hipStream_t st) {
-  const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, nullptr, lengths, reset};
-#define PP_CALL(T)                                                                              \
-  hipLaunchKernelGGL((pp_rec_bwd_kernel<T>), dim3((d + 63) / 64, b), dim3(64), 0, st,           \
-                     static_cast<const T*>(z), static_cast<const T*>(f), starts,                \
-                     static_cast<const T*>(gy), gh_last, static_cast<T*>(gz),                   \
-                     static_cast<T*>(gf), gh0, p)
+  const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, 0, 0, nullptr, lengths, reset, nullptr, nullptr, nullptr};
+  const size_t s = dtype == PP_F32 ? 4 : 2;
+  const bool two = s == 2 && fits(2, s, {z, f, gy, gz, gf}, {zb, zl, fb, fl, gb, gl, (int64_t)d});
+#define PP_CALL(T)                                                           \
+  do {                                                                       \
+    if (sizeof(T) == 2 && two)                                               \
+      run_bwd<T, sizeof(T) == 2 ? 2 : 1>(z, f, starts, gy, gh_last, gz, gf, gh0, p, ws, st); \
+    else                                                                     \
+      run_bwd<T, 1>(z, f, starts, gy, gh_last, gz, gf, gh0, p, ws, st);      \
+  } while (0)
   PP_REC_TYPES(PP_CALL);
 #undef PP_CALL
 }
 
 hipError_t pp_launch_rec_step(const void* z, int64_t zb, const void* f, int64_t fb, int dtype,
                               float* h, int64_t hb, void* y, int b, int d, hipStream_t st) {
-#define PP_CALL(T)                                                                              \
-  hipLaunchKernelGGL((pp_rec_step_kernel<T>), dim3((d + 255) / 256, b), dim3(256), 0, st,       \
-                     static_cast<const T*>(z), zb, static_cast<const T*>(f), fb, h, hb,         \
-                     static_cast<T*>(y), b, d)
+  const size_t s = dtype == PP_F32 ? 4 : 2;
+  const bool two = fits(2, s, {z, f, y}, {zb, fb, (int64_t)d}) && fits(2, 4, {h}, {hb});
+#define PP_CALL(T)                                       \
+  do {                                                   \
+    if (two)                                             \
+      run_step<T, 2>(z, zb, f, fb, h, hb, y, b, d, st);  \
+    else                                                 \
+      run_step<T, 1>(z, zb, f, fb, h, hb, y, b, d, st);  \
+  } while (0)
   PP_REC_TYPES(PP_CALL);
 #undef PP_CALL
 }
