@@ -50,15 +50,19 @@ struct PPRaw<2> { typedef uint16_t type; };
 template <>
 struct PPRaw<4> { typedef uint32_t type; };
 template <>
-struct PPRaw<8> { typedef uint2 type; };
+struct PPRaw<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
 template <>
-struct PPRaw<16> { typedef uint4 type; };
+struct PPRaw<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
 
 template <typename T, int N>
 struct PPElems {
   typedef typename PPRaw<N * sizeof(T)>::type raw;
   static __device__ __forceinline__ raw load(const T* p) { return *reinterpret_cast<const raw*>(p); }
   static __device__ __forceinline__ void store(T* p, raw r) { *reinterpret_cast<raw*>(p) = r; }
+  // what no kernel reads soon: past the caches
+  static __device__ __forceinline__ void stream(T* p, raw r) {
+    __builtin_nontemporal_store(r, reinterpret_cast<raw*>(p));
+  }
   static __device__ __forceinline__ void get(const raw& r, float (&v)[N]) {
     if constexpr (sizeof(T) == 4) {
       struct S { float x[N]; };

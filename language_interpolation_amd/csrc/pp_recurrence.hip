@@ -9,8 +9,8 @@
 //   e_t = gy_t + u_t;  u_{t-1} = a_t e_t  (0 at a reset; u = gh_last behind the last step)
 //   gz_t = e_t (1 - a_t);   gf_t = e_t a_t (1 - a_t) (h_{t-1} - z_t);   gh0 = a_0 e_0
 //
-// 1 - a is sigmoid(-f), so neither gate loses its small end to cancellation; a step keeps the
-// smaller of the two, with its sign telling which it is, and the other is 1 minus it.
+// With x = e^-f: a = 1 / (1 + x) and 1 - a = x a, so neither gate loses its small end to
+// cancellation, and h_t = z_t + a_t (h_{t-1} - z_t).
 //
 // Split of the length.  A step is linear in the state, so a stretch of steps is h_out = P h_in + H
 // with P the product of its a and H its result from 0.  A wave takes kSteps steps x 64 V channels:
@@ -36,14 +36,14 @@
 namespace {
 
 constexpr int kSteps = PP_RECURRENCE_STEPS;  // steps of a wave, and between two kept states
-constexpr int kWaves = 8;                    // waves (stretches) of a workgroup
-constexpr int kChunk = kSteps * kWaves;
+constexpr int kMostWaves = 16;               // waves (stretches) of a workgroup
 constexpr uint32_t kNotYet = 0xffffffffu;
 
 struct RecArgs {
   int64_t zb, zl, fb, fl, gb, gl;  // strides in elements of z, f and gy over batch and time
   int b, l, d;
   int nchunk, ngroup;  // chunks of a row, groups of 64 V channels
+  int chunk;           // steps of a chunk
   const float* h0;
   const int32_t* lengths;
   const uint8_t* reset;
@@ -52,29 +52,43 @@ struct RecArgs {
   uint32_t* done;            // [chain][chunk][64 V]: state behind it
 };
 
-// The smaller gate with a sign: r = sigmoid(-f) for f >= 0, -a for f < 0.
+// e^-f (infinity where f is far below 0: then 1 / (1 + x) is 0, as it should be)
+template <bool EXACT>
+__device__ __forceinline__ float gate_exp(float f) {
+  const float hi = f * -1.44269502f;
+  const float x = __builtin_amdgcn_exp2f(hi);
+  if (!EXACT) return x;
+  // the rounding of f log2(e) is made good: matters for |f| >> 1 in fp32
+  const float lo = fmaf(f, -1.92596299e-8f, fmaf(f, -1.44269502f, -hi));
+  return fabsf(hi) < 126.0f ? fmaf(x * 0.693147182f, lo, x) : x;
+}
+template <bool EXACT>
+__device__ __forceinline__ float gate(float f) {
+  return __builtin_amdgcn_rcpf(1.0f + gate_exp<EXACT>(f));
+}
+// Both gates in one register for later walks: the smaller of the two, its sign telling which it is
+// (1 - a for f >= 0, -a else); the other is 1 minus it.
 template <bool EXACT>
 __device__ __forceinline__ float gate_code(float f) {
-  const float s = -fabsf(f);
-  float x;
-  if (EXACT) {  // the rounding of s log2(e) is made good: matters for |f| >> 1 in fp32
-    const float hi = s * 1.44269502f;
-    const float lo = fmaf(s, 1.92596299e-8f, fmaf(s, 1.44269502f, -hi));
-    x = __builtin_amdgcn_exp2f(hi);
-    x = fmaf(x * 0.693147182f, lo, x);
-    x = s < -200.0f ? 0.0f : x;  // (also -inf, whose lo is NaN)
-  } else {
-    x = __builtin_amdgcn_exp2f(s * 1.44269502f);
-  }
-  const float small = x * __builtin_amdgcn_rcpf(1.0f + x);
-  return f >= 0.0f ? small : (f < 0.0f ? -small : f);  // NaN stays NaN
+  const float x = gate_exp<EXACT>(fabsf(f));
+  return copysignf(x * __builtin_amdgcn_rcpf(1.0f + x), f);
 }
 __device__ __forceinline__ void gates(float q, float& a, float& r) {
   const float small = fabsf(q), big = 1.0f - small;
-  // (q = -0.0 is the open gate's underflow: a = 0)
-  const bool neg = __float_as_uint(q) >> 31;
+  const bool neg = __float_as_int(q) < 0;  // (also -0.0, a closed gate)
   a = neg ? small : big;
   r = neg ? big : small;
+}
+
+// Holds a value in this very form: without it the compiler keeps what the value was made from, or
+// both gates of an earlier walk, in registers of their own, at the cost of half the resident waves.
+__device__ __forceinline__ void keep(float& x) { asm volatile("" : "+v"(x)); }
+template <int V>
+__device__ __forceinline__ void keep_all(float (&q)[kSteps][V]) {
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+    for (int v = 0; v < V; ++v) keep(q[j][v]);
 }
 
 // state behind a stretch (P, H) from the state before it
@@ -91,9 +105,9 @@ __device__ __forceinline__ uint32_t word_of(float x) {
 template <int kWindow, int V>
 __device__ __forceinline__ void look_back(const RecArgs& p, int64_t chain, int first, int last,
                                           float (&h)[V]) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t* done = p.done + chain * p.nchunk * (64 * V) + lane;
-  const unsigned long long* part = p.part + chain * p.nchunk * (64 * V) + lane;
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t* done = p.done + chain * p.nchunk * (64 * V);
+  const unsigned long long* part = p.part + chain * p.nchunk * (64 * V);
   int k = last;
   for (bool found = false; !found;) {  // the nearest chunk whose state is known
     uint32_t w[kWindow][V];
@@ -101,7 +115,7 @@ __device__ __forceinline__ void look_back(const RecArgs& p, int64_t chain, int f
     for (int j = 0; j < kWindow; ++j)
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        w[j][v] = __hip_atomic_load(done + (int64_t)max(k - j, first) * (64 * V) + v * 64, __ATOMIC_RELAXED,
+        w[j][v] = __hip_atomic_load(done + (int64_t)max(k - j, first) * (64 * V) + v * 64 + lane, __ATOMIC_RELAXED,
                                     __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
     for (int j = 0; j < kWindow; ++j) {
@@ -132,7 +146,7 @@ __device__ __forceinline__ void look_back(const RecArgs& p, int64_t chain, int f
     for (int j = 0; j < kWindow; ++j)
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        w[j][v] = __hip_atomic_load(part + (int64_t)min(k + 1 + j, last) * (64 * V) + v * 64,
+        w[j][v] = __hip_atomic_load(part + (int64_t)min(k + 1 + j, last) * (64 * V) + v * 64 + lane,
                                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     int used = 0;
 #pragma unroll
@@ -199,30 +213,31 @@ __device__ __forceinline__ void draw_tile(const RecArgs& p, int* shared, int& c,
 }
 
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_fwd_kernel(const T* __restrict__ z,
+__global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T* __restrict__ z,
                                                                  const T* __restrict__ f,
                                                                  T* __restrict__ y,
                                                                  float* __restrict__ h_last,
                                                                  float* __restrict__ starts, RecArgs p) {
   typedef PPElems<T, V> E;
-  __shared__ float2 part[kWaves][V][64];
+  __shared__ float2 part[kMostWaves][V][64];
   __shared__ float carry[V][64];
   __shared__ int drawn;
   int c, g, b;
   draw_tile(p, &drawn, c, g, b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ch = (g * 64 + lane) * V;
   const bool live = ch < p.d;
-  const int chl = live ? ch : 0;  // a lane without channels reads some and writes nothing
+  const uint32_t chl = live ? ch : 0;  // a lane without channels reads some and writes nothing
   const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
-  const int t0 = c * kChunk + wave * kSteps;
+  const int t0 = c * p.chunk + wave * kSteps;
   const int n = max(0, min(kSteps, len - t0));        // steps of this wave that exist
   const int rows = max(0, min(kSteps, p.l - t0));     // rows of y to write
   const int64_t chain = (int64_t)b * p.ngroup + g;
   const int64_t row0 = (int64_t)b * p.l + t0;
 
-  float q[kSteps][V];
-  typename E::raw zr[kSteps];
+  // of each step: the state from 0 at the start of the stretch, and the product of its a until then
+  float hl[kSteps][V] = {}, pl[kSteps][V] = {};
   float P[V], H[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -232,33 +247,36 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_fwd_kernel(const T* __r
   uint32_t cut = 0;
   if (n > 0) {
     cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
-    const T* zp = z + b * p.zb + t0 * p.zl + chl;
-    const T* fp = f + b * p.fb + t0 * p.fl + chl;
-    typename E::raw fr[kSteps];
+    const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
+    const T* fp = f + b * p.fb + t0 * p.fl;
+    typename E::raw fr[kSteps], zr[kSteps];
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
       const int64_t t = min(j, n - 1);
-      fr[j] = E::load(fp + t * p.fl);
-      zr[j] = E::load(zp + t * p.zl);
+      fr[j] = E::load(fp + t * p.fl + chl);
+      zr[j] = E::load(zp + t * p.zl + chl);
     }
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
       float fv[V], zv[V];
       E::get(fr[j], fv);
       E::get(zr[j], zv);
+      if (j < n) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        q[j][v] = gate_code<sizeof(T) == 4>(fv[v]);
-        float a, r;
-        gates(q[j][v], a, r);
-        if (j < n) {
+        for (int v = 0; v < V; ++v) {
+          const float a = gate<sizeof(T) == 4>(fv[v]);
           if (cut >> j & 1) {
             P[v] = -0.0f;
             H[v] = 0.0f;
           }
-          H[v] = fmaf(a, H[v], r * zv[v]);
+          H[v] = fmaf(a, H[v] - zv[v], zv[v]);
           P[v] *= a;
         }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        hl[j][v] = H[v];
+        pl[j][v] = P[v];
       }
     }
   }
@@ -268,12 +286,12 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_fwd_kernel(const T* __r
   const bool alone = p.nchunk == 1;
   if (wave == 0) {  // the state before this chunk
     float h[V];
-    if (c == 0 || c * kChunk >= len) {
+    if (c == 0 || c * p.chunk >= len) {
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = p.h0 && live ? p.h0[(int64_t)b * p.d + ch + v] : 0.0f;
     }
-    if (c * kChunk < len && !alone) {
-      const bool more = (c + 1) * kChunk < len;  // someone waits for it
+    if (c * p.chunk < len && !alone) {
+      const bool more = (c + 1) * p.chunk < len;  // someone waits for it
       float CP[V], CH[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -308,55 +326,44 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_fwd_kernel(const T* __r
   }
   if (!live) return;
   if (starts && n > 0) {
-    float* at = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d + ch;
+    float* at = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d;
 #pragma unroll
-    for (int v = 0; v < V; ++v) at[v] = h[v];
+    for (int v = 0; v < V; ++v) at[chl + v] = h[v];
   }
-  T* yp = y + row0 * p.d + ch;
+  T* yp = y + row0 * p.d;
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
     float out[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = 0.0f;
-    if (j < n) {
-      float zv[V];
-      E::get(zr[j], zv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a, r;
-        gates(q[j][v], a, r);
-        if (cut >> j & 1) h[v] = 0.0f;
-        h[v] = fmaf(a, h[v], r * zv[v]);
-        out[v] = h[v];
-      }
-    }
-    if (j < rows) E::store(yp + (int64_t)j * p.d, E::put(out));
+    for (int v = 0; v < V; ++v) out[v] = j < n ? through(pl[j][v], hl[j][v], h[v]) : 0.0f;
+    if (j < rows) E::stream(yp + (int64_t)j * p.d + chl, E::put(out));
   }
   if ((n > 0 && t0 + n == len) || (len == 0 && c == 0 && wave == 0)) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) h_last[(int64_t)b * p.d + ch + v] = h[v];
+    for (int v = 0; v < V; ++v) h_last[(int64_t)b * p.d + ch + v] = through(P[v], H[v], h[v]);
   }
 }
 
 // Chunks are counted from the end of the (allocated) row: chunk c of the chain is row chunk
 // nchunk - 1 - c; those behind the end of a shorter row only write zeros.
 template <typename T, int V>
-__global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_bwd_kernel(
+__global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
     const T* __restrict__ z, const T* __restrict__ f, const float* __restrict__ starts,
     const T* __restrict__ gy, const float* __restrict__ gh, T* __restrict__ gz, T* __restrict__ gf,
     float* __restrict__ gh0, RecArgs p) {
   typedef PPElems<T, V> E;
-  __shared__ float2 part[kWaves][V][64];
+  __shared__ float2 part[kMostWaves][V][64];
   __shared__ float carry[V][64];
   __shared__ int drawn;
   int c, g, b;
   draw_tile(p, &drawn, c, g, b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ch = (g * 64 + lane) * V;
   const bool live = ch < p.d;
-  const int chl = live ? ch : 0;
+  const uint32_t chl = live ? ch : 0;
   const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
-  const int chunk0 = (p.nchunk - 1 - c) * kChunk;  // first step of the chunk
+  const int chunk0 = (p.nchunk - 1 - c) * p.chunk;  // first step of the chunk
   const int t0 = chunk0 + wave * kSteps;
   const int n = max(0, min(kSteps, len - t0));
   const int rows = max(0, min(kSteps, p.l - t0));
@@ -374,22 +381,22 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_bwd_kernel(
   uint32_t cut = 0;
   if (n > 0) {
     cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
-    const T* zp = z + b * p.zb + t0 * p.zl + chl;
-    const T* fp = f + b * p.fb + t0 * p.fl + chl;
-    const T* gp = gy + b * p.gb + t0 * p.gl + chl;
-    const float* sp = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d + chl;
+    const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
+    const T* fp = f + b * p.fb + t0 * p.fl;
+    const T* gp = gy + b * p.gb + t0 * p.gl;
+    const float* sp = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d;
     typename E::raw fr[kSteps], zr[kSteps];
     float h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = sp[v];
+    for (int v = 0; v < V; ++v) h[v] = sp[chl + v];
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
       const int64_t t = min(j, n - 1);
-      fr[j] = E::load(fp + t * p.fl);
-      zr[j] = E::load(zp + t * p.zl);
+      fr[j] = E::load(fp + t * p.fl + chl);
+      zr[j] = E::load(zp + t * p.zl + chl);
     }
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) gr[j] = E::load(gp + (int64_t)min(j, n - 1) * p.gl);
+    for (int j = 0; j < kSteps; ++j) gr[j] = E::load(gp + (int64_t)min(j, n - 1) * p.gl + chl);
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
       float fv[V], zv[V];
@@ -402,7 +409,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_bwd_kernel(
         gates(q[j][v], a, r);
         if (cut >> j & 1) h[v] = 0.0f;
         gap[j][v] = h[v] - zv[v];
-        h[v] = fmaf(a, h[v], r * zv[v]);
+        h[v] = fmaf(a, gap[j][v], zv[v]);
+        keep(q[j][v]);
+        keep(gap[j][v]);
       }
     }
 #pragma unroll
@@ -428,7 +437,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_bwd_kernel(
   __syncthreads();
   if (wave == 0) {  // the gradient that arrives behind this chunk
     float u[V];
-    const int first = p.nchunk - (len + kChunk - 1) / kChunk;  // the chain's chunk with the last step
+    const int first = p.nchunk - (len + p.chunk - 1) / p.chunk;  // the chain's chunk with the last step
     if (c <= first) {
 #pragma unroll
       for (int v = 0; v < V; ++v) u[v] = gh && live ? gh[(int64_t)b * p.d + ch + v] : 0.0f;
@@ -468,8 +477,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_bwd_kernel(
     for (int w = waves - 1; w > wave; --w) u[v] = through(part[w][v][lane].x, part[w][v][lane].y, u[v]);
   }
   if (!live) return;
-  T* gzp = gz + row0 * p.d + ch;
-  T* gfp = gf + row0 * p.d + ch;
+  keep_all<V>(q);
+  T* gzp = gz + row0 * p.d;
+  T* gfp = gf + row0 * p.d;
 #pragma unroll
   for (int j = kSteps - 1; j >= 0; --j) {
     float oz[V], of[V];
@@ -489,8 +499,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void pp_rec_bwd_kernel(
       }
     }
     if (j < rows) {
-      E::store(gzp + (int64_t)j * p.d, E::put(oz));
-      E::store(gfp + (int64_t)j * p.d, E::put(of));
+      E::stream(gzp + (int64_t)j * p.d + chl, E::put(oz));
+      E::stream(gfp + (int64_t)j * p.d + chl, E::put(of));
     }
   }
   if (gh0 && chunk0 == 0 && wave == 0) {
@@ -517,9 +527,8 @@ __global__ __launch_bounds__(256) void pp_rec_step_kernel(const T* __restrict__ 
   EH::get(EH::load(h + row * hb + ch), hv);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    float a, r;
-    gates(gate_code<sizeof(T) == 4>(fv[v]), a, r);
-    hv[v] = fmaf(a, hv[v], r * zv[v]);
+    const float a = gate<sizeof(T) == 4>(fv[v]);
+    hv[v] = fmaf(a, hv[v] - zv[v], zv[v]);
   }
   EH::store(h + row * hb + ch, EH::put(hv));
   E::store(y + row * d + ch, E::put(hv));
@@ -534,14 +543,14 @@ bool fits(int v, size_t size, std::initializer_list<const void*> at, std::initia
   return true;
 }
 
-int plan(RecArgs& p, int v, void* ws) {  // returns the waves of a workgroup
+void plan(RecArgs& p, int v, void* ws) {
   p.ngroup = (p.d + 64 * v - 1) / (64 * v);
-  p.nchunk = (p.l + kChunk - 1) / kChunk;
+  p.chunk = kSteps * std::min(kMostWaves, (p.l + kSteps - 1) / kSteps);  // a short row is one chunk
+  p.nchunk = (p.l + p.chunk - 1) / p.chunk;
   p.ticket = static_cast<uint32_t*>(ws);
   const int64_t n = (int64_t)p.b * p.nchunk * p.ngroup * 64 * v;
   p.part = reinterpret_cast<unsigned long long*>(p.ticket + 4);
   p.done = reinterpret_cast<uint32_t*>(p.part + n);
-  return p.nchunk > 1 ? kWaves : (p.l + kSteps - 1) / kSteps;
 }
 
 void fill(const RecArgs& p, int v, hipStream_t st) {
@@ -551,22 +560,24 @@ void fill(const RecArgs& p, int v, hipStream_t st) {
                      p.ticket, words);
 }
 
-template <typename T, int V>
+// One channel a lane in the forward, whatever the type: 60 registers, twice the waves of two channels a
+// lane (114).  bf16 [8, 2048, 2048]: 55 against 59 us, [1, 100003, 640]: 112 against 120 us.
+template <typename T>
 void run_fwd(const void* z, const void* f, void* y, float* h_last, float* starts, RecArgs p, void* ws,
              hipStream_t st) {
-  const int waves = plan(p, V, ws);
-  fill(p, V, st);
-  hipLaunchKernelGGL((pp_rec_fwd_kernel<T, V>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
-                     dim3(64 * waves), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
+  plan(p, 1, ws);
+  fill(p, 1, st);
+  hipLaunchKernelGGL((pp_rec_fwd_kernel<T, 1>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
+                     dim3(4 * p.chunk), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
                      static_cast<T*>(y), h_last, starts, p);
 }
 template <typename T, int V>
 void run_bwd(const void* z, const void* f, const float* starts, const void* gy, const float* gh,
              void* gz, void* gf, float* gh0, RecArgs p, void* ws, hipStream_t st) {
-  const int waves = plan(p, V, ws);
+  plan(p, V, ws);
   fill(p, V, st);
   hipLaunchKernelGGL((pp_rec_bwd_kernel<T, V>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
-                     dim3(64 * waves), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
+                     dim3(4 * p.chunk), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
                      starts, static_cast<const T*>(gy), gh, static_cast<T*>(gz), static_cast<T*>(gf),
                      gh0, p);
 }
@@ -590,26 +601,17 @@ void run_step(const void* z, int64_t zb, const void* f, int64_t fb, float* h, in
   } while (0)
 
 size_t pp_rec_workspace_bytes(int b, int l, int d) {
-  const int64_t nchunk = ((int64_t)l + kChunk - 1) / kChunk;
-  if (nchunk == 1) return 0;
-  return 16 + (size_t)b * nchunk * (((size_t)d + 255) / 256 * 256) * 12;
+  if (l <= kMostWaves * kSteps) return 0;
+  const size_t chunk = kMostWaves * kSteps, nchunk = ((size_t)l + chunk - 1) / chunk;
+  return 16 + (size_t)b * nchunk * (((size_t)d + 127) / 128 * 128) * 12;
 }
 
 hipError_t pp_launch_rec_fwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,
                              int64_t fl, int dtype, const float* h0, const int32_t* lengths,
                              const uint8_t* reset, void* y, float* h_last, float* starts, void* ws,
                              int b, int l, int d, hipStream_t st) {
-  const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, 0, 0, h0, lengths, reset, nullptr, nullptr, nullptr};
-  const size_t s = dtype == PP_F32 ? 4 : 2;
-  int v = 2;
-  while (v > 1 && !fits(v, s, {z, f, y}, {zb, zl, fb, fl, (int64_t)d})) v /= 2;
-#define PP_CALL(T)                                                             \
-  do {                                                                         \
-    if (v == 2)                                                           \
-      run_fwd<T, 2>(z, f, y, h_last, starts, p, ws, st);                       \
-    else                                                                       \
-      run_fwd<T, 1>(z, f, y, h_last, starts, p, ws, st);                       \
-  } while (0)
+  const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, 0, 0, 0, h0, lengths, reset, nullptr, nullptr, nullptr};
+#define PP_CALL(T) run_fwd<T>(z, f, y, h_last, starts, p, ws, st)
   PP_REC_TYPES(PP_CALL);
 #undef PP_CALL
 }
@@ -619,8 +621,10 @@ hipError_t pp_launch_rec_bwd(const void* z, int64_t zb, int64_t zl, const void* 
                              const float* starts, const void* gy, int64_t gb, int64_t gl,
                              const float* gh_last, void* gz, void* gf, float* gh0, void* ws, int b,
                              int l, int d, hipStream_t st) {
-  const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, 0, 0, nullptr, lengths, reset, nullptr, nullptr, nullptr};
+  const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, 0, 0, 0, nullptr, lengths, reset, nullptr, nullptr, nullptr};
   const size_t s = dtype == PP_F32 ? 4 : 2;
+  // Two channels a lane in 16-bit types: with one, the 2-byte accesses of five tensors are the limit
+  // (bf16 [1, 100003, 640]: 154 against 201 us).  In fp32 two would need more registers than there are.
   const bool two = s == 2 && fits(2, s, {z, f, gy, gz, gf}, {zb, zl, fb, fl, gb, gl, (int64_t)d});
 #define PP_CALL(T)                                                           \
   do {                                                                       \
