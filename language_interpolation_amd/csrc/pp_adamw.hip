@@ -39,6 +39,7 @@ struct AdamWDescs {
   int64_t n[PP_OPT_MAX_TENSORS];
   int first[PP_OPT_MAX_TENSORS + 1];        // first workgroup of each tensor
   uint32_t number[PP_OPT_MAX_TENSORS];
+  uint32_t wide;                            // bit t: four entries of every list of tensor t are one access
   float c1[PP_OPT_MAX_TENSORS];             // lr / (1 - b1^t)
   float c2[PP_OPT_MAX_TENSORS];             // 1 / sqrt(1 - b2^t)
 };
@@ -119,36 +120,65 @@ __global__ __launch_bounds__(256) void pp_adamw_kernel(AdamWDescs d, AdamWArgs a
   const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
   const uint32_t key = EIGHT ? mix32(mix32(mix32(number) ^ a.seed) + a.index + (uint32_t)t) : 0u;
   const int64_t first = (int64_t)((int)blockIdx.x - d.first[t]) * per_block;
+  const bool wide = d.wide >> t & 1;
+  void* __restrict__ mp = d.m[t];
+  void* __restrict__ vp = d.v[t];
+  typedef PPElems<T, 4> ET;
+  typedef PPElems<float, 4> EF;
+  typedef PPElems<uint8_t, 4> E8;
   for (int it = 0; it < per_block; it += 1024) {
     const int64_t e0 = first + it + (int64_t)threadIdx.x * 4;
     if (first + it + (threadIdx.x & ~63) * 4 >= n) return;  // the whole wave is behind the end
     float gv[4], wv[4], mv[4], vv[4];
+    uint32_t mc[4], vc[4];
     int Em = 0, Ev = 0;
-    uint8_t* m8 = static_cast<uint8_t*>(d.m[t]);
-    uint8_t* v8 = static_cast<uint8_t*>(d.v[t]);
-    float* m32 = static_cast<float*>(d.m[t]);
-    float* v32 = static_cast<float*>(d.v[t]);
     if (EIGHT) {
       Em = d.me[t][e0 / kBlk];
       Ev = d.ve[t][e0 / kBlk];
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t e = e0 + j;
-      const bool live = e < n;
-      gv[j] = live ? (float)g[e] : 0.0f;
-      wv[j] = live ? w[e] : 0.0f;
+    const bool whole = wide && e0 + 4 <= n;
+    if (whole) {
+      const typename ET::raw gr = ET::take(g + e0);
+      const typename EF::raw wr = EF::take(w + e0);
       if (EIGHT) {
-        mv[j] = live ? decode8<14, true>(m8[e], Em) : 0.0f;
-        vv[j] = live ? decode8<30, false>(v8[e], Ev) : 0.0f;
+        const uint32_t mr = E8::load(static_cast<const uint8_t*>(mp) + e0);
+        const uint32_t vr = E8::load(static_cast<const uint8_t*>(vp) + e0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mc[j] = mr >> (8 * j) & 255u;
+          vc[j] = vr >> (8 * j) & 255u;
+        }
       } else {
-        mv[j] = live ? m32[e] : 0.0f;
-        vv[j] = live ? v32[e] : 0.0f;
+        const typename EF::raw mr = EF::take(static_cast<const float*>(mp) + e0);
+        const typename EF::raw vr = EF::take(static_cast<const float*>(vp) + e0);
+        EF::get(mr, mv);
+        EF::get(vr, vv);
+      }
+      ET::get(gr, gv);
+      EF::get(wr, wv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t e = e0 + j;
+        const bool live = e < n;
+        gv[j] = live ? (float)g[e] : 0.0f;
+        wv[j] = live ? w[e] : 0.0f;
+        if (EIGHT) {
+          mc[j] = live ? static_cast<const uint8_t*>(mp)[e] : 0u;
+          vc[j] = live ? static_cast<const uint8_t*>(vp)[e] : 0u;
+        } else {
+          mv[j] = live ? static_cast<const float*>(mp)[e] : 0.0f;
+          vv[j] = live ? static_cast<const float*>(vp)[e] : 0.0f;
+        }
       }
     }
     float tm = 0.0f, tv = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      if (EIGHT) {
+        mv[j] = decode8<14, true>(mc[j], Em);
+        vv[j] = decode8<30, false>(vc[j], Ev);
+      }
       const float gg = gv[j] * gs;
       mv[j] = mv[j] * a.b1 + gg * a.nb1;
       vv[j] = vv[j] * a.b2 + (gg * gg) * a.nb2;
@@ -158,45 +188,72 @@ __global__ __launch_bounds__(256) void pp_adamw_kernel(AdamWDescs d, AdamWArgs a
         tv = fmaxf(tv, finite_size(vv[j]));
       }
     }
-    uint32_t bm = 0, bv = 0;
     if (EIGHT) {
       Em = (int)(__float_as_uint(wave_max_nonneg(tm)) >> 23);
       Ev = (int)(__float_as_uint(wave_max_nonneg(tv)) >> 23);
       const uint32_t q = key + 2u * (uint32_t)(e0 >> 2);
-      bm = mix32(q);
-      bv = mix32(q + 1u);
+      const uint32_t bm = mix32(q), bv = mix32(q + 1u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mc[j] = encode8<14, true>(mv[j], Em, (bm >> (8 * j)) & 255u);
+        vc[j] = encode8<30, false>(vv[j], Ev, (bv >> (8 * j)) & 255u);
+      }
       if ((threadIdx.x & 63) == 0) {
         d.me[t][e0 / kBlk] = (uint8_t)Em;
         d.ve[t][e0 / kBlk] = (uint8_t)Ev;
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t e = e0 + j;
-      if (e >= n) break;
-      w[e] = wv[j];
-      if (sizeof(T) == 2) p[e] = (T)wv[j];
+    if (whole) {
+      EF::stream(w + e0, EF::put(wv));
+      if (sizeof(T) == 2) ET::stream(p + e0, ET::put(wv));
       if (EIGHT) {
-        m8[e] = (uint8_t)encode8<14, true>(mv[j], Em, (bm >> (8 * j)) & 255u);
-        v8[e] = (uint8_t)encode8<30, false>(vv[j], Ev, (bv >> (8 * j)) & 255u);
+        E8::store(static_cast<uint8_t*>(mp) + e0, mc[0] | mc[1] << 8 | mc[2] << 16 | mc[3] << 24);
+        E8::store(static_cast<uint8_t*>(vp) + e0, vc[0] | vc[1] << 8 | vc[2] << 16 | vc[3] << 24);
       } else {
-        m32[e] = mv[j];
-        v32[e] = vv[j];
+        EF::stream(static_cast<float*>(mp) + e0, EF::put(mv));
+        EF::stream(static_cast<float*>(vp) + e0, EF::put(vv));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t e = e0 + j;
+        if (e >= n) break;
+        w[e] = wv[j];
+        if (sizeof(T) == 2) p[e] = (T)wv[j];
+        if (EIGHT) {
+          static_cast<uint8_t*>(mp)[e] = (uint8_t)mc[j];
+          static_cast<uint8_t*>(vp)[e] = (uint8_t)vc[j];
+        } else {
+          static_cast<float*>(mp)[e] = mv[j];
+          static_cast<float*>(vp)[e] = vv[j];
+        }
       }
     }
   }
 }
 
+// Eight codes a thread: 8 bytes in, 16 or 32 out.
 template <typename O, bool SIGNED>
 __global__ __launch_bounds__(256) void pp_decode_moment_kernel(const uint8_t* __restrict__ code,
                                                                const uint8_t* __restrict__ exps,
-                                                               O* __restrict__ out, int64_t n) {
-  const int64_t e0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+                                                               O* __restrict__ out, int64_t n, int wide) {
+  constexpr int kPer = 16 / sizeof(O);  // entries of a store
+  const int64_t e0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e0 >= n) return;
+  const int E = exps[e0 / kBlk];
+  if (wide && e0 + 8 <= n) {
+    const typename PPRaw<8>::type c = PPElems<uint8_t, 8>::load(code + e0);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t e = e0 + j;
-    if (e < n) out[e] = (O)decode8<SIGNED ? 14 : 30, SIGNED>(code[e], exps[e / kBlk]);
+    for (int i = 0; i < 8; i += kPer) {
+      float x[kPer];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        x[j] = decode8<SIGNED ? 14 : 30, SIGNED>(c[(i + j) / 4] >> (8 * (j & 3)) & 255u, E);
+      PPElems<O, kPer>::stream(out + e0 + i, PPElems<O, kPer>::put(x));
+    }
+    return;
   }
+  for (int64_t e = e0; e < n && e < e0 + 8; ++e) out[e] = (O)decode8<SIGNED ? 14 : 30, SIGNED>(code[e], E);
 }
 
 struct StepCounters {
@@ -228,8 +285,9 @@ hipError_t pp_launch_adamw(int count, int dtype, int bits, void* const* p, const
   a.eps = (float)eps; a.decay = (float)(1.0 - lr * wd);
   a.lr = lr; a.beta1 = beta1; a.beta2 = beta2;
   a.seed = seed; a.index = index; a.grad_scale = grad_scale; a.count = count;
-  const int per_block = 1024;
+  const int per_block = bits == 8 ? 2048 : 1024;
   int64_t blocks = 0;
+  d.wide = 0;
   for (int t = 0; t < count; ++t) {
     d.p[t] = p[t]; d.g[t] = g[t]; d.m[t] = m[t]; d.v[t] = v[t];
     d.w[t] = dtype == PP_F32 ? static_cast<float*>(p[t]) : master[t];
@@ -241,6 +299,9 @@ hipError_t pp_launch_adamw(int count, int dtype, int bits, void* const* p, const
     d.number[t] = (uint32_t)s;
     d.c1[t] = (float)(lr / (1.0 - int_power(beta1, s)));
     d.c2[t] = (float)(1.0 / std::sqrt(1.0 - int_power(beta2, s)));
+    const size_t es = dtype == PP_F32 ? 4 : 2, ms = bits / 8;
+    if ((((size_t)p[t] | (size_t)g[t]) % (4 * es) | (size_t)d.w[t] % 16 | ((size_t)m[t] | (size_t)v[t]) % (4 * ms)) == 0)
+      d.wide |= 1u << t;
     d.first[t] = (int)blocks;
     blocks += (numel[t] + per_block - 1) / per_block;
   }
@@ -262,17 +323,18 @@ hipError_t pp_launch_adamw(int count, int dtype, int bits, void* const* p, const
 
 hipError_t pp_launch_decode_moment(const uint8_t* code, const uint8_t* exps, void* out, int dtype,
                                    int is_signed, int64_t n, hipStream_t st) {
-  const int64_t blocks = (n + 1023) / 1024;
+  const int64_t blocks = (n + 2047) / 2048;
   if (blocks >= (1LL << 31)) return hipErrorInvalidValue;
+  const int wide = (size_t)code % 8 == 0 && (size_t)out % 16 == 0;
   const dim3 grid((unsigned)blocks), block(256);
 #define PP_DECODE(T)                                                                             \
   do {                                                                                           \
     if (is_signed)                                                                               \
       hipLaunchKernelGGL((pp_decode_moment_kernel<T, true>), grid, block, 0, st, code, exps,     \
-                         static_cast<T*>(out), n);                                               \
+                         static_cast<T*>(out), n, wide);                                               \
     else                                                                                         \
       hipLaunchKernelGGL((pp_decode_moment_kernel<T, false>), grid, block, 0, st, code, exps,    \
-                         static_cast<T*>(out), n);                                               \
+                         static_cast<T*>(out), n, wide);                                               \
   } while (0)
   if (dtype == PP_F32) PP_DECODE(float);
   else if (dtype == PP_BF16) PP_DECODE(pp_bf16);

@@ -59,7 +59,10 @@ struct PPElems {
   typedef typename PPRaw<N * sizeof(T)>::type raw;
   static __device__ __forceinline__ raw load(const T* p) { return *reinterpret_cast<const raw*>(p); }
   static __device__ __forceinline__ void store(T* p, raw r) { *reinterpret_cast<raw*>(p) = r; }
-  // what no kernel reads soon: past the caches
+  // what is read or written once: no place in the caches for it
+  static __device__ __forceinline__ raw take(const T* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const raw*>(p));
+  }
   static __device__ __forceinline__ void stream(T* p, raw r) {
     __builtin_nontemporal_store(r, reinterpret_cast<raw*>(p));
   }

@@ -1026,6 +1026,23 @@ def rms_norm(x, weight, eps: float = 1e-5):
 _ELEMENT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PP_F32, PP_BF16, PP_F16
 
 
+def _launch(name: str, device: torch.device, *args) -> None:
+    """An entry point on the current stream of `device`; addresses are passed as integers or None."""
+    fn = getattr(_lib.load(), name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
 def _require_element(t, name: str, like=None) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
@@ -1080,12 +1097,9 @@ class GatedRecurrenceFunction(torch.autograd.Function):
                 starts = torch.empty(b, lib.pp_gated_recurrence_starts(l), d, device=z.device)
             nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
             ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
-            with torch.cuda.device(z.device):
-                rc = lib.pp_gated_recurrence_fwd(
-                    _ptr(z), z.stride(0), z.stride(1), _ptr(f), f.stride(0), f.stride(1),
-                    _ELEMENT[z.dtype], _ptr(h0), _ptr(lengths), _ptr(reset), _ptr(y), _ptr(h),
-                    _ptr(starts), _ptr(ws), nbytes, b, l, d, _stream(z.device))
-            _lib.check(rc, "pp_gated_recurrence_fwd")
+            _launch("pp_gated_recurrence_fwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
+                    f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(h0), _at(lengths), _at(reset),
+                    _at(y), _at(h), _at(starts), _at(ws), nbytes, b, l, d)
         if any(ctx.needs_input_grad):
             ctx.save_for_backward(z, f, starts, lengths, reset)
         return y, h
@@ -1105,13 +1119,10 @@ class GatedRecurrenceFunction(torch.autograd.Function):
         gh0 = torch.empty(b, d, device=z.device) if ctx.needs_input_grad[2] else None
         nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
         ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
-        with torch.cuda.device(z.device):
-            rc = lib.pp_gated_recurrence_bwd(
-                _ptr(z), z.stride(0), z.stride(1), _ptr(f), f.stride(0), f.stride(1),
-                _ELEMENT[z.dtype], _ptr(lengths), _ptr(reset), _ptr(starts), _ptr(gy),
-                gy.stride(0), gy.stride(1), _ptr(gh), _ptr(gz), _ptr(gf), _ptr(gh0), _ptr(ws),
-                nbytes, b, l, d, _stream(z.device))
-        _lib.check(rc, "pp_gated_recurrence_bwd")
+        _launch("pp_gated_recurrence_bwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
+                f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(lengths), _at(reset), _at(starts),
+                _at(gy), gy.stride(0), gy.stride(1), _at(gh), _at(gz), _at(gf), _at(gh0), _at(ws),
+                nbytes, b, l, d)
         return gz, gf, gh0, None, None
 
 
@@ -1160,12 +1171,8 @@ def gated_recurrence_step(z, f, h):
     if z.numel() == 0:
         return y
     z, f = _last_contiguous(z), _last_contiguous(f)
-    lib = _lib.load()
-    with torch.cuda.device(z.device):
-        rc = lib.pp_gated_recurrence_step(_ptr(z), z.stride(0), _ptr(f), f.stride(0),
-                                          _ELEMENT[z.dtype], _ptr(h), max(h.stride(0), d), _ptr(y),
-                                          b, d, _stream(z.device))
-    _lib.check(rc, "pp_gated_recurrence_step")
+    _launch("pp_gated_recurrence_step", z.device, _at(z), z.stride(0), _at(f), f.stride(0),
+            _ELEMENT[z.dtype], _at(h), max(h.stride(0), d), _at(y), b, d)
     torch._C._increment_version([h])
     return y
 
@@ -1206,17 +1213,13 @@ def _check_classes(logits, tokens, mask):
 class TokenLogProbsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask):
-        lib = _lib.load()
         b, t, v = logits.shape
         logits, lb, lt = _class_rows(logits)
         lp = torch.empty(b, t, device=logits.device, dtype=torch.float32)
         stats = torch.empty(b, t, 2, device=logits.device) if ctx.needs_input_grad[0] else None
         if lp.numel():
-            with torch.cuda.device(logits.device):
-                rc = lib.pp_token_log_probs_fwd(
-                    _ptr(logits), lb, lt, _ELEMENT[logits.dtype], _ptr(tokens), _ptr(mask), _ptr(lp),
-                    _ptr(stats), b, t, v, _stream(logits.device))
-            _lib.check(rc, "pp_token_log_probs_fwd")
+            _launch("pp_token_log_probs_fwd", logits.device, _at(logits), lb, lt,
+                    _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(lp), _at(stats), b, t, v)
         if stats is not None:
             ctx.save_for_backward(logits, tokens, mask, stats)
             ctx.strides = (lb, lt)
@@ -1236,13 +1239,9 @@ def _class_backward(logits, tokens, mask, stats, coef, gout, done_if_one, grad, 
     b, t, v = logits.shape
     if b * t == 0:
         return
-    lib = _lib.load()
-    with torch.cuda.device(logits.device):
-        rc = lib.pp_token_log_probs_bwd(
-            _ptr(logits), strides[0], strides[1], _ELEMENT[logits.dtype], _ptr(tokens), _ptr(mask),
-            _ptr(stats), _ptr(coef), _ptr(gout), done_if_one, _ptr(grad), b, t, v,
-            _stream(logits.device))
-    _lib.check(rc, "pp_token_log_probs_bwd")
+    _launch("pp_token_log_probs_bwd", logits.device, _at(logits), strides[0], strides[1],
+            _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(stats), _at(coef), _at(gout),
+            done_if_one, _at(grad), b, t, v)
 
 
 def token_log_probs(logits, tokens, mask=None):
@@ -1276,13 +1275,10 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         if b * t:
             nbytes = lib.pp_clipped_policy_loss_workspace_bytes(b, t)
             ws = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
-            with torch.cuda.device(logits.device):
-                rc = lib.pp_clipped_policy_loss_fwd(
-                    _ptr(logits), lb, lt, _ELEMENT[logits.dtype], _ptr(tokens), _ptr(mask), _ptr(old),
-                    _ptr(adv), adv.stride(0), adv.stride(1), _ptr(ref), low, high, beta, by_sequence,
-                    _ptr(out), _ptr(stats), _ptr(coef), _ptr(grad), _ptr(ws), nbytes, b, t, v,
-                    _stream(logits.device))
-            _lib.check(rc, "pp_clipped_policy_loss_fwd")
+            _launch("pp_clipped_policy_loss_fwd", logits.device, _at(logits), lb, lt,
+                    _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(old), _at(adv), adv.stride(0),
+                    adv.stride(1), _at(ref), low, high, beta, by_sequence, _at(out), _at(stats),
+                    _at(coef), _at(grad), _at(ws), nbytes, b, t, v)
         else:
             out.zero_()
         if grad is not None:
@@ -1377,90 +1373,92 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     steps: the number of this step (1, 2, ...) or a device int64 counter that is advanced by the call
     (under graph capture), for all or a list of one each.  grad_scale: device fp32 scalar that the
     gradients are multiplied by."""
-    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    params = list(params)
     n = len(params)
-    if not n:
-        return
     eight = avg_exponents is not None or sq_exponents is not None
     if eight and (avg_exponents is None or sq_exponents is None):
         raise ValueError("adamw_step: 8-bit moments need avg_exponents and sq_exponents")
-    lists = [("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs)]
-    for name, x in (("masters", masters), ("avg_exponents", avg_exponents), ("sq_exponents", sq_exponents)):
-        if x is not None:
-            lists.append((name, list(x)))
-    for name, x in lists:
-        if len(x) != n:
-            raise ValueError(f"adamw_step: {len(x)} {name} for {n} params")
-    steps = list(steps) if isinstance(steps, (list, tuple)) else [steps] * n
-    counted = isinstance(steps[0], torch.Tensor)
-    if len(steps) != n or any(isinstance(s, torch.Tensor) != counted for s in steps):
-        raise ValueError("adamw_step: steps is one number or counter, or a list of one each")
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
         raise ValueError(f"adamw_step: betas must lie in [0, 1), got {betas}")
-    first = params[0]
-    _require_element(first, "params[0]")
-    dtype, device = first.dtype, first.device
+    lists = {"grads": list(grads), "exp_avgs": list(exp_avgs), "exp_avg_sqs": list(exp_avg_sqs)}
+    for name, x in (("masters", masters), ("avg_exponents", avg_exponents), ("sq_exponents", sq_exponents)):
+        if x is not None:
+            lists[name] = list(x)
+    for name, x in lists.items():
+        if len(x) != n:
+            raise ValueError(f"adamw_step: {len(x)} {name} for {n} params")
+    steps = list(steps) if isinstance(steps, (list, tuple)) else [steps] * n
+    if len(steps) != n:
+        raise ValueError(f"adamw_step: {len(steps)} steps for {n} params")
+    if not n:
+        return
+    counted = isinstance(steps[0], torch.Tensor)
+    if any(isinstance(s, torch.Tensor) != counted for s in steps):
+        raise ValueError("adamw_step: steps are all numbers or all counters")
+    _require_element(params[0], "params[0]")
+    dtype, device = params[0].dtype, params[0].device
     if (masters is not None) != (dtype != torch.float32):
         raise ValueError("adamw_step: masters belong to bfloat16 and float16 params, and these need them")
-    moment = torch.uint8 if eight else torch.float32
-    wanted = {"grads": dtype, "exp_avgs": moment, "exp_avg_sqs": moment, "masters": torch.float32}
+    sizes, at = [], {"params": []}
     for i, p in enumerate(params):
         if p.dtype != dtype or p.device != device:
             raise TypeError(f"adamw_step: params[{i}] is {p.dtype} on {p.device}, params[0] {dtype} on {device}")
-        stride = p.stride()
-        if not p.is_contiguous() and not dense_storage(p):
-            raise ValueError(f"adamw_step: params[{i}] has gaps or overlaps (strides {stride})")
-        for name, x in lists:
-            t = x[i]
-            if name in wanted:
-                ok = t.dtype == wanted[name] and t.shape == p.shape and t.stride() == stride
-            else:
-                ok = t.dtype == torch.uint8 and t.is_contiguous() and t.numel() == -(-p.numel() // 256)
-            if not ok or t.device != device:
-                raise ValueError(f"adamw_step: {name}[{i}] ({t.dtype}, {tuple(t.shape)}, strides {t.stride()}, "
-                                 f"{t.device}) does not fit params[{i}] ({dtype}, {tuple(p.shape)}, {stride}, {device})")
-    ptrs = [p.data_ptr() for p in params]
-    if len({q for q, p in zip(ptrs, params) if p.numel()}) < sum(p.numel() > 0 for p in params):
-        raise ValueError("adamw_step: a param is in the list twice")
-    if grad_scale is not None:
-        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != device:
-            raise ValueError("adamw_step: grad_scale is one float32 on the device of the params")
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        stream = _stream(device)
-        if counted:
-            unique = list({s.data_ptr(): s for s in steps}.values())
-            for s in unique:
-                if s.dtype != torch.int64 or s.numel() != 1 or s.device != device:
-                    raise ValueError("adamw_step: a step counter is one int64 on the device of the params")
-            for lo in range(0, len(unique), _lib.OPT_MAX_TENSORS):
-                part = unique[lo:lo + _lib.OPT_MAX_TENSORS]
-                rc = lib.pp_count_step(len(part), (c_void_p * len(part))(*[s.data_ptr() for s in part]), stream)
-                _lib.check(rc, "pp_count_step")
-            torch._C._increment_version(unique)
-        elif min(steps) < 1:
-            raise ValueError("adamw_step: steps are counted from 1")
-        table = {name: [t.data_ptr() for t in x] for name, x in lists}
-        live = [i for i in range(n) if params[i].numel()]
-        for lo in range(0, len(live), _lib.OPT_MAX_TENSORS):
-            part = live[lo:lo + _lib.OPT_MAX_TENSORS]
-            k = len(part)
-
-            def array(values, kind=c_void_p):
-                return None if values is None else (kind * k)(*[values[i] for i in part])
-
-            rc = lib.pp_adamw_step(
-                k, _ELEMENT[dtype], 8 if eight else 32, array(ptrs), array(table["grads"]),
-                array(table.get("masters")), array(table["exp_avgs"]), array(table["exp_avg_sqs"]),
-                array(table.get("avg_exponents")), array(table.get("sq_exponents")),
-                array([p.numel() for p in params], ctypes.c_int64),
-                None if counted else array(steps, ctypes.c_int64),
-                array([s.data_ptr() for s in steps]) if counted else None,
-                lr, b1, b2, eps, weight_decay, _ptr(grad_scale), seed & 0xFFFFFFFF, lo, stream)
-            _lib.check(rc, "pp_adamw_step")
+        if not dense_storage(p):
+            raise ValueError(f"adamw_step: params[{i}] has gaps or overlaps (strides {p.stride()})")
+        sizes.append(p.numel())
+        at["params"].append(p.data_ptr())
+    shapes, strides = [p.shape for p in params], [p.stride() for p in params]
+    moment = torch.uint8 if eight else torch.float32
+    wanted = {"grads": dtype, "exp_avgs": moment, "exp_avg_sqs": moment, "masters": torch.float32}
+    for name, x in lists.items():
+        if name in wanted:
+            kind = wanted[name]
+            bad = [i for i, t in enumerate(x) if t.dtype != kind or t.shape != shapes[i] or
+                   t.stride() != strides[i] or t.device != device]
+        else:
+            bad = [i for i, t in enumerate(x) if t.dtype != torch.uint8 or t.numel() != -(-sizes[i] // 256) or
+                   not t.is_contiguous() or t.device != device]
+        if bad:
+            i, t = bad[0], x[bad[0]]
+            raise ValueError(f"adamw_step: {name}[{i}] ({t.dtype}, {tuple(t.shape)}, strides {t.stride()}, {t.device}) "
+                             f"does not fit params[{i}] ({dtype}, {tuple(shapes[i])}, strides {strides[i]}, {device})")
+        at[name] = [t.data_ptr() for t in x]
+    live = range(n) if min(sizes) else [i for i in range(n) if sizes[i]]
+    for name, x in at.items():  # two updates of the same memory would race
+        if name != "grads" and len({x[i] for i in live}) < len(live):
+            raise ValueError(f"adamw_step: a tensor is twice in {name}")
+    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or
+                                   grad_scale.device != device):
+        raise ValueError("adamw_step: grad_scale is one float32 on the device of the params")
+    most = _lib.OPT_MAX_TENSORS
+    if counted:
+        unique = list({s.data_ptr(): s for s in steps}.values())
+        for s in unique:
+            if s.dtype != torch.int64 or s.numel() != 1 or s.device != device:
+                raise ValueError("adamw_step: a step counter is one int64 on the device of the params")
+        for lo in range(0, len(unique), most):
+            part = unique[lo:lo + most]
+            _launch("pp_count_step", device, len(part), (c_void_p * len(part))(*[s.data_ptr() for s in part]))
+        torch._C._increment_version(unique)
+    elif min(steps) < 1:
+        raise ValueError("adamw_step: steps are counted from 1")
+    for lo in range(0, len(live), most):
+        part = live[lo:lo + most]
+        k = len(part)
+        pointers, numbers = c_void_p * k, ctypes.c_int64 * k
+        p, g, w, m, v, me, ve = (
+            pointers(*[at[name][i] for i in part]) if name in at else None
+            for name in ("params", "grads", "masters", "exp_avgs", "exp_avg_sqs", "avg_exponents", "sq_exponents"))
+        _launch("pp_adamw_step", device, k, _ELEMENT[dtype], 8 if eight else 32, p, g, w, m, v, me, ve,
+                numbers(*[sizes[i] for i in part]), None if counted else numbers(*[steps[i] for i in part]),
+                pointers(*[steps[i].data_ptr() for i in part]) if counted else None, lr, b1, b2, eps,
+                weight_decay, _at(grad_scale), seed & 0xFFFFFFFF, lo)
     # written through raw pointers: tell autograd and the pre-split weight cache
-    torch._C._increment_version(params + [t for name, x in lists if name != "grads" for t in x])
+    for name, x in lists.items():
+        if name != "grads":
+            params = params + x
+    torch._C._increment_version(params)
 
 
 def decode_moment(codes, exponents, signed: bool, dtype=torch.float32):
@@ -1475,10 +1473,7 @@ def decode_moment(codes, exponents, signed: bool, dtype=torch.float32):
     _require_aux(exponents, "exponents", (-(-codes.numel() // 256),), (torch.uint8,), codes.device)
     out = torch.empty_like(codes, dtype=dtype)
     if codes.numel():
-        lib = _lib.load()
         exponents = exponents.contiguous()
-        with torch.cuda.device(codes.device):
-            rc = lib.pp_decode_moment(_ptr(codes), _ptr(exponents), _ptr(out), _ELEMENT[dtype],
-                                      int(signed), codes.numel(), _stream(codes.device))
-        _lib.check(rc, "pp_decode_moment")
+        _launch("pp_decode_moment", codes.device, _at(codes), _at(exponents), _at(out), _ELEMENT[dtype],
+                int(signed), codes.numel())
     return out
