@@ -8,12 +8,21 @@
 // Row statistics are kept as (max, log of the sum of exp(x - max)) in fp32: lp = (x - max) - log sum
 // is a difference of small numbers, where x - logsumexp would lose the digits of a large max.
 // A masked token's logits, token, old, ref and advantage are not read; its gradient row is zeros.
+//
+// Bound: the logits are read once and the gradient written once.  A row that fits is therefore held
+// in registers, as it came, between the statistics and the gradient (pp_policy_fused_kernel: a wave,
+// 256 or 1024 threads a row, up to kMostVecs 16-byte vectors a thread); a longer one is read twice
+// (pp_row_terms_kernel, then pp_row_grad_kernel, which are also the score and the backward alone).
+// Rows start anywhere: up to 7 elements before the first 16-byte boundary and behind the last are
+// taken one by one ("edge"), all others as aligned vectors.
 #include <algorithm>
 
 #include "pp_device.h"
 #include "pp_lowp.h"
 
 namespace {
+
+constexpr float kLog2e = 1.44269504f;
 
 struct PolArgs {
   const int64_t* tokens;
@@ -25,97 +34,335 @@ struct PolTerms {
   const float* old;
   const float* adv;
   const float* ref;
-  int64_t ab, at;  // strides of adv
+  int64_t ab, at;       // strides of adv
   float low, high, beta;
+  const float* weight;  // of a token, by sequence; NULL: `every`
+  float every;
+  float* terms;         // [3][padded rows]: weighted loss, kl, clipped
+  int padded;
 };
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = red[0];
-  for (int i = 1; i < (int)blockDim.x / 64; ++i) r = fmaxf(r, red[i]);
-  __syncthreads();
-  return r;
+// Vectors and edge elements of a row at x.
+template <typename T>
+struct Span {
+  static constexpr int kVec = 16 / sizeof(T);
+  int head, vecs, edge;
+  __device__ __forceinline__ Span(const T* x, int v) {
+    const int off = (int)((size_t)x & 15) / (int)sizeof(T);
+    head = min(v, off ? kVec - off : 0);
+    vecs = (v - head) / kVec;
+    edge = v - vecs * kVec;  // head and tail
+  }
+  // element number of edge i < edge
+  __device__ __forceinline__ int edge_at(int i) const { return i < head ? i : i + vecs * kVec; }
+};
+
+// max / sum over the THREADS lanes that share a row; red: one float a wave of the workgroup
+template <int THREADS>
+__device__ __forceinline__ float row_max(float v, float* red) {
+  v = pp_dpp_max<0x128>(v);
+  v = pp_dpp_max<0x124>(v);
+  v = pp_dpp_max<0x122>(v);
+  v = pp_dpp_max<0x121>(v);
+  v = fmaxf(fmaxf(pp_readlane_f(v, 0), pp_readlane_f(v, 16)), fmaxf(pp_readlane_f(v, 32), pp_readlane_f(v, 48)));
+  if (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) v = fmaxf(v, red[i]);
+    __syncthreads();
+  }
+  return v;
 }
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = 0.0f;
-  for (int i = 0; i < (int)blockDim.x / 64; ++i) r += red[i];
-  __syncthreads();
-  return r;
+template <int THREADS>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = pp_wave_sum(v);
+  if (THREADS > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; ++i) v += red[i];
+    __syncthreads();
+  }
+  return v;
 }
 
-// (max, log sum) of a row
-template <typename T>
-__device__ __forceinline__ float2 row_stats(const T* __restrict__ x, int v, float* red) {
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < v; i += blockDim.x) m = fmaxf(m, (float)x[i]);
-  m = block_max(m, red);
-  float s = 0.0f;
-  for (int i = threadIdx.x; i < v; i += blockDim.x) s += expf((float)x[i] - m);
-  s = block_sum(s, red);
-  return make_float2(m, logf(s));
-}
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
 template <typename T>
 __device__ __forceinline__ float token_lp(const T* __restrict__ x, int64_t token, int v, float2 st) {
-  if (token < 0 || token >= v) return NAN;  // no such class: the loss says so
+  if (token < 0 || token >= v) return __uint_as_float(0x7fc00000u);  // no such class: the loss says so
   return ((float)x[token] - st.x) - st.y;
 }
 
-template <typename T>
-__device__ __forceinline__ void write_grad(const T* __restrict__ x, T* __restrict__ g, int64_t token,
-                                           int v, float2 st, float c) {
-  for (int i = threadIdx.x; i < v; i += blockDim.x) {
-    float q = 0.0f;
-    if (c != 0.0f) q = c * ((i == token ? 1.0f : 0.0f) - expf(((float)x[i] - st.x) - st.y));
-    g[i] = (T)q;
+// The terms of one token; returns the gradient's coefficient.
+__device__ __forceinline__ float policy_terms(const PolArgs& p, const PolTerms& q, int row, float lp,
+                                              bool writer) {
+  const int b = row / p.t, t = row % p.t;
+  const float w = q.weight ? q.weight[b] : q.every, adv = q.adv[b * q.ab + t * q.at];
+  const float rho = expf(lp - q.old[row]);
+  const float border = adv >= 0.0f ? 1.0f + q.high : 1.0f - q.low;
+  const bool clipped = adv >= 0.0f ? rho > border : rho < border;
+  float loss = -(clipped ? border : rho) * adv, c = clipped ? 0.0f : -adv * rho, kl = 0.0f;
+  if (q.ref) {
+    const float delta = q.ref[row] - lp, grow = expm1f(delta);
+    kl = grow - delta;
+    loss += q.beta * kl;
+    c -= q.beta * grow;
   }
+  if (writer) {
+    q.terms[row] = loss * w;
+    q.terms[q.padded + row] = kl * w;
+    q.terms[2 * (int64_t)q.padded + row] = clipped ? w : 0.0f;
+  }
+  return c * w;
+}
+__device__ __forceinline__ void no_terms(const PolTerms& q, int row) {
+  q.terms[row] = q.terms[q.padded + row] = q.terms[2 * (int64_t)q.padded + row] = 0.0f;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void pp_token_lp_kernel(const T* __restrict__ logits, PolArgs p,
-                                                          float* __restrict__ lp,
-                                                          float2* __restrict__ stats) {
+template <typename T, int THREADS>
+__device__ __forceinline__ void zero_row(T* __restrict__ g, int v, int tid) {
+  typedef PPElems<T, Span<T>::kVec> E;
+  const Span<T> s(g, v);
+  typename E::raw zero = {};
+  for (int i = tid; i < s.vecs; i += THREADS) E::stream(g + s.head + (int64_t)i * s.kVec, zero);
+  if (tid < s.edge) g[s.edge_at(tid)] = (T)0.0f;
+}
+
+// The statistics of a row by one pass over it: every lane keeps a running max and the sum relative to
+// it, kAhead vectors in flight.
+template <typename T, int THREADS>
+__device__ __forceinline__ float2 stream_stats(const T* __restrict__ x, int v, int tid, float* red) {
+  constexpr int kVec = Span<T>::kVec, kAhead = 4;
+  typedef PPElems<T, kVec> E;
+  const Span<T> s(x, v);
+  const T* body = x + s.head;
+  float m = -3.40282347e38f, sum = 0.0f;  // (finite, so that -inf - m is -inf and not NaN)
+  auto add = [&](const float (&e)[kVec]) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) top = fmaxf(top, e[j]);
+    sum *= exp_of(m - top);
+    m = top;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) sum += exp_of(e[j] - m);
+  };
+  int i = tid;
+  for (; i + (kAhead - 1) * THREADS < s.vecs; i += kAhead * THREADS) {
+    typename E::raw r[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) r[k] = E::take(body + (int64_t)(i + k * THREADS) * kVec);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      float e[kVec];
+      E::get(r[k], e);
+      add(e);
+    }
+  }
+  for (; i < s.vecs; i += THREADS) {
+    float e[kVec];
+    E::get(E::take(body + (int64_t)i * kVec), e);
+    add(e);
+  }
+  if (tid < s.edge) {
+    const float e = (float)x[s.edge_at(tid)], top = fmaxf(m, e);
+    sum = sum * exp_of(m - top) + exp_of(e - top);
+    m = top;
+  }
+  const float top = row_max<THREADS>(m, red);
+  sum = row_sum<THREADS>(sum * exp_of(m - top), red);
+  return make_float2(top, logf(sum));
+}
+
+// stats and lp, or stats, terms and coef, of each row.  THREADS lanes a row, 256 a workgroup.
+template <typename T, int THREADS, bool POLICY>
+__global__ __launch_bounds__(256) void pp_row_terms_kernel(const T* __restrict__ logits, PolArgs p,
+                                                           PolTerms q, float2* __restrict__ stats,
+                                                           float* __restrict__ out) {
   __shared__ float red[4];
-  const int row = blockIdx.x;
+  const int tid = threadIdx.x % THREADS;
+  const int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  if (row >= p.rows) return;
   if (p.mask && !p.mask[row]) {
-    if (threadIdx.x == 0) {
-      lp[row] = 0.0f;
+    if (tid == 0) {
       if (stats) stats[row] = make_float2(0.0f, 0.0f);
+      if (out) out[row] = 0.0f;
+      if (POLICY) no_terms(q, row);
     }
     return;
   }
   const T* x = logits + (row / p.t) * p.lb + (row % p.t) * p.lt;
-  const float2 st = row_stats(x, p.v, red);
-  if (threadIdx.x == 0) {
-    lp[row] = token_lp(x, p.tokens[row], p.v, st);
+  const float2 st = stream_stats<T, THREADS>(x, p.v, tid, red);
+  if (tid == 0) {
+    const float lp = token_lp(x, p.tokens[row], p.v, st);
     if (stats) stats[row] = st;
+    if (POLICY) {
+      const float c = policy_terms(p, q, row, lp, true);
+      if (out) out[row] = c;
+    } else {
+      out[row] = lp;
+    }
   }
+}
+
+// One vector of the gradient: k exp(x - max), and c more at the token.
+template <typename T>
+__device__ __forceinline__ typename PPElems<T, Span<T>::kVec>::raw grad_vec(
+    const typename PPElems<T, Span<T>::kVec>::raw& r, float m, float k, float c, int token_in) {
+  constexpr int kVec = Span<T>::kVec;
+  typedef PPElems<T, kVec> E;
+  float e[kVec];
+  E::get(r, e);
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) e[j] = k * exp_of(e[j] - m);
+  if ((unsigned)token_in < (unsigned)kVec) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) e[j] += j == token_in ? c : 0.0f;
+  }
+  return E::put(e);
 }
 
 // grad = gout * coef * (onehot - softmax).  done_if_one: the gradient for gout = 1 is in `grad`
 // already (the forward of the loss wrote it), so that only another gout needs the work; it starts
 // from the logits again, since scaling the stored 16-bit values would round twice and would not
 // bring back what underflowed at gout = 1 (a loss scaled for fp16).
-template <typename T>
-__global__ __launch_bounds__(256) void pp_token_lp_bwd_kernel(
-    const T* __restrict__ logits, PolArgs p, const float2* __restrict__ stats,
-    const float* __restrict__ coef, const float* __restrict__ gout, int done_if_one,
-    T* __restrict__ grad) {
+template <typename T, int THREADS>
+__global__ __launch_bounds__(256) void pp_row_grad_kernel(const T* __restrict__ logits, PolArgs p,
+                                                          const float2* __restrict__ stats,
+                                                          const float* __restrict__ coef,
+                                                          const float* __restrict__ gout,
+                                                          int done_if_one, T* __restrict__ grad) {
+  constexpr int kVec = Span<T>::kVec;
+  typedef PPElems<T, kVec> E;
   const float go = gout ? *gout : 1.0f;
   if (done_if_one && go == 1.0f) return;
-  for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  const int tid = threadIdx.x % THREADS;
+  for (int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS; row < p.rows;
+       row += gridDim.x * (256 / THREADS)) {
     const int64_t at = (row / p.t) * p.lb + (row % p.t) * p.lt;
-    const float c = p.mask && !p.mask[row] ? 0.0f : coef[row] * go;
-    write_grad(logits + at, grad + at, p.tokens[row], p.v, stats[row], c);
+    const T* x = logits + at;
+    T* g = grad + at;
+    if (p.mask && !p.mask[row]) {
+      zero_row<T, THREADS>(g, p.v, tid);
+      continue;
+    }
+    const float c = coef[row] * go;
+    const float2 st = stats[row];
+    const float k = -c * exp_of(-st.y);
+    const int64_t tok = p.tokens[row];
+    const int token = tok >= 0 && tok < p.v ? (int)tok : -1 - kVec;
+    const Span<T> s(x, p.v);
+    for (int i = tid; i < s.vecs; i += THREADS) {
+      const int64_t e = s.head + (int64_t)i * kVec;
+      E::stream(g + e, grad_vec<T>(E::take(x + e), st.x, k, c, token - (int)e));
+    }
+    if (tid < s.edge) {
+      const int e = s.edge_at(tid);
+      g[e] = (T)(k * exp_of((float)x[e] - st.x) + (e == token ? c : 0.0f));
+    }
   }
 }
 
-// the weight of a token of each sequence; one workgroup
+template <typename T>
+__device__ __forceinline__ typename PPElems<T, Span<T>::kVec>::raw minus_infinity() {
+  float e[Span<T>::kVec];
+#pragma unroll
+  for (int j = 0; j < Span<T>::kVec; ++j) e[j] = -INFINITY;
+  return PPElems<T, Span<T>::kVec>::put(e);
+}
+
+// Holds the row as it came: without this the compiler keeps its fp32 values, and then their
+// exponentials, from one walk to the next, in two to four times the registers.
+template <typename R, int NV>
+__device__ __forceinline__ void keep_raw(R (&r)[NV]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(r[i]));
+}
+
+// Statistics, terms and gradient of a row that NV vectors a thread hold.
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pp_policy_fused_kernel(
+    const T* __restrict__ logits, PolArgs p, PolTerms q, float2* __restrict__ stats,
+    float* __restrict__ coef, T* __restrict__ grad) {
+  constexpr int kVec = Span<T>::kVec, kRows = THREADS < 256 ? 256 / THREADS : 1;
+  typedef PPElems<T, kVec> E;
+  __shared__ float red[THREADS / 64 > 4 ? THREADS / 64 : 4];
+  const int tid = threadIdx.x % THREADS;
+  const int row = blockIdx.x * kRows + threadIdx.x / THREADS;
+  if (row >= p.rows) return;
+  const int64_t at = (row / p.t) * p.lb + (row % p.t) * p.lt;
+  const T* x = logits + at;
+  T* g = grad + at;
+  if (p.mask && !p.mask[row]) {
+    if (tid == 0) {
+      stats[row] = make_float2(0.0f, 0.0f);
+      coef[row] = 0.0f;
+      no_terms(q, row);
+    }
+    zero_row<T, THREADS>(g, p.v, tid);
+    return;
+  }
+  const Span<T> s(x, p.v);
+  typename E::raw r[NV];  // (-inf where the row has ended: no share in the sum)
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int n = i * THREADS + tid;
+    r[i] = minus_infinity<T>();
+    if (n < s.vecs) r[i] = E::take(x + s.head + (int64_t)n * kVec);
+  }
+  float edge = -INFINITY;
+  if (tid < s.edge) edge = (float)x[s.edge_at(tid)];
+  const int64_t tok = p.tokens[row];
+  const float xt = tok >= 0 && tok < p.v ? (float)x[tok] : __uint_as_float(0x7fc00000u);
+  float m = edge;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * THREADS < s.vecs) {  // (the same for all lanes)
+      float e[kVec];
+      E::get(r[i], e);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) m = fmaxf(m, e[j]);
+    }
+  }
+  keep_raw(r);
+  m = row_max<THREADS>(m, red);
+  float sum = tid < s.edge ? exp_of(edge - m) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * THREADS < s.vecs) {
+      float e[kVec];
+      E::get(r[i], e);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) sum += exp_of(e[j] - m);
+    }
+  }
+  keep_raw(r);
+  sum = row_sum<THREADS>(sum, red);
+  const float2 st = make_float2(m, logf(sum));
+  const float c = policy_terms(p, q, row, (xt - st.x) - st.y, tid == 0);
+  if (tid == 0) {
+    stats[row] = st;
+    coef[row] = c;
+  }
+  const float k = -c / sum;
+  const int token = tok >= 0 && tok < p.v ? (int)tok : -1 - kVec;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int n = i * THREADS + tid;
+    if (n < s.vecs) {
+      const int e = s.head + n * kVec;
+      E::stream(g + e, grad_vec<T>(r[i], m, k, c, token - e));
+    }
+  }
+  if (tid < s.edge) {
+    const int e = s.edge_at(tid);
+    g[e] = (T)(k * exp_of(edge - m) + (e == token ? c : 0.0f));
+  }
+}
+
+// The weight of a token of each sequence; one workgroup.
 __global__ __launch_bounds__(1024) void pp_policy_weight_kernel(const uint8_t* __restrict__ mask,
                                                                 int b, int t, int by_sequence,
                                                                 float* __restrict__ w) {
@@ -123,75 +370,43 @@ __global__ __launch_bounds__(1024) void pp_policy_weight_kernel(const uint8_t* _
   if (threadIdx.x == 0) total = filled = 0;
   __syncthreads();
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int s = wave; s < b; s += 16) {
-    int n = 0;
-    for (int i = lane; i < t; i += 64) n += mask ? mask[(int64_t)s * t + i] != 0 : 1;
-    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
-    if (lane == 0) {
-      atomicAdd(&total, n);
-      if (n) atomicAdd(&filled, 1);
-      w[s] = (float)n;
+  if (by_sequence) {
+    for (int s = wave; s < b; s += 16) {
+      int n = 0;
+#pragma unroll 4
+      for (int i = lane; i < t; i += 64) n += mask[(int64_t)s * t + i] != 0;
+      for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
+      if (lane == 0) {
+        if (n) atomicAdd(&filled, 1);
+        w[s] = (float)n;
+      }
     }
+  } else {
+    int n = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < b * t; i += 1024) n += mask[i] != 0;
+    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o);
+    if (lane == 0) atomicAdd(&total, n);
   }
   __syncthreads();
   for (int s = threadIdx.x; s < b; s += 1024) {
-    const float n = w[s];
-    w[s] = n == 0.0f ? 0.0f : by_sequence ? 1.0f / n / (float)filled : 1.0f / (float)total;
+    if (by_sequence) {
+      const float n = w[s];
+      w[s] = n == 0.0f ? 0.0f : 1.0f / n / (float)filled;
+    } else {
+      w[s] = total ? 1.0f / (float)total : 0.0f;
+    }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void pp_policy_kernel(const T* __restrict__ logits, PolArgs p,
-                                                        PolTerms q, const float* __restrict__ weight,
-                                                        float2* __restrict__ stats,
-                                                        float* __restrict__ coef,
-                                                        float* __restrict__ terms,
-                                                        T* __restrict__ grad) {
-  __shared__ float red[4];
-  const int row = blockIdx.x, b = row / p.t, t = row % p.t;
-  const int64_t at = b * p.lb + t * p.lt;
-  float c = 0.0f, loss = 0.0f, kl = 0.0f, cut = 0.0f;
-  float2 st = make_float2(0.0f, 0.0f);
-  int64_t token = 0;
-  if (!p.mask || p.mask[row]) {
-    const T* x = logits + at;
-    token = p.tokens[row];
-    st = row_stats(x, p.v, red);
-    const float lp = token_lp(x, token, p.v, st);
-    const float w = weight[b], adv = q.adv[b * q.ab + t * q.at];
-    const float rho = expf(lp - q.old[row]);
-    const float border = adv >= 0.0f ? 1.0f + q.high : 1.0f - q.low;
-    const bool clipped = adv >= 0.0f ? rho > border : rho < border;
-    loss = -(clipped ? border : rho) * adv;
-    c = clipped ? 0.0f : -adv * rho;
-    if (q.ref) {
-      const float delta = q.ref[row] - lp, grow = expm1f(delta);
-      kl = grow - delta;
-      loss += q.beta * kl;
-      c -= q.beta * grow;
-    }
-    c *= w;
-    loss *= w;
-    kl *= w;
-    cut = clipped ? w : 0.0f;
-  }
-  if (threadIdx.x == 0) {
-    terms[row] = loss;
-    terms[p.rows + row] = kl;
-    terms[2 * (int64_t)p.rows + row] = cut;
-    if (stats) {
-      stats[row] = st;
-      coef[row] = c;
-    }
-  }
-  if (grad) write_grad(logits + at, grad + at, token, p.v, st, c);
-}
-
+// Sum of each of the three lists, in 64 bits and in a fixed order.
 __global__ __launch_bounds__(1024) void pp_policy_finish_kernel(const float* __restrict__ terms,
-                                                                int rows, float* __restrict__ out) {
+                                                                int rows, int padded,
+                                                                float* __restrict__ out) {
   __shared__ double red[16];
-  const float* x = terms + (int64_t)blockIdx.x * rows;
+  const float* x = terms + (int64_t)blockIdx.x * padded;
   double s = 0.0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < rows; i += 1024) s += (double)x[i];
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -200,6 +415,58 @@ __global__ __launch_bounds__(1024) void pp_policy_finish_kernel(const float* __r
     for (int i = 1; i < 16; ++i) s += red[i];
     out[blockIdx.x] = (float)s;
   }
+}
+
+constexpr int kWaveRow = 4096;  // bytes up to which a row is one wave's
+
+template <typename T, bool POLICY>
+void run_terms(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* out,
+               hipStream_t st) {
+  if ((int64_t)p.v * (int64_t)sizeof(T) <= kWaveRow)
+    hipLaunchKernelGGL((pp_row_terms_kernel<T, 64, POLICY>), dim3((p.rows + 3) / 4), dim3(256), 0, st,
+                       logits, p, q, stats, out);
+  else
+    hipLaunchKernelGGL((pp_row_terms_kernel<T, 256, POLICY>), dim3(p.rows), dim3(256), 0, st, logits, p,
+                       q, stats, out);
+}
+
+template <typename T>
+void run_grad(const T* logits, const PolArgs& p, const float2* stats, const float* coef,
+              const float* gout, int done_if_one, T* grad, hipStream_t st) {
+  if ((int64_t)p.v * (int64_t)sizeof(T) <= kWaveRow)
+    hipLaunchKernelGGL((pp_row_grad_kernel<T, 64>), dim3(std::min((p.rows + 3) / 4, 8192)), dim3(256), 0,
+                       st, logits, p, stats, coef, gout, done_if_one, grad);
+  else
+    hipLaunchKernelGGL((pp_row_grad_kernel<T, 256>), dim3(std::min(p.rows, 8192)), dim3(256), 0, st,
+                       logits, p, stats, coef, gout, done_if_one, grad);
+}
+
+template <typename T, int THREADS, int NV>
+bool try_fused(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* coef, T* grad,
+               hipStream_t st) {
+  if (p.v > THREADS * NV * Span<T>::kVec) return false;
+  constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
+  hipLaunchKernelGGL((pp_policy_fused_kernel<T, THREADS, NV>), dim3((p.rows + kRows - 1) / kRows),
+                     dim3(THREADS < 256 ? 256 : THREADS), 0, st, logits, p, q, stats, coef, grad);
+  return true;
+}
+
+template <typename T>
+void run_policy(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* coef, T* grad,
+                hipStream_t st) {
+  if (grad && stats &&
+      (try_fused<T, 64, 1>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 64, 2>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 64, 4>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 256, 2>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 256, 4>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 256, 8>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 1024, 4>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 1024, 8>(logits, p, q, stats, coef, grad, st) ||
+       try_fused<T, 1024, 16>(logits, p, q, stats, coef, grad, st)))
+    return;
+  run_terms<T, true>(logits, p, q, stats, coef, st);
+  if (grad) run_grad<T>(logits, p, stats, coef, nullptr, 0, grad, st);
 }
 
 }  // namespace
@@ -215,9 +482,9 @@ hipError_t pp_launch_token_lp(const void* logits, int64_t lb, int64_t lt, int dt
                               const int64_t* tokens, const uint8_t* mask, float* lp, float* stats,
                               int b, int t, int v, hipStream_t st) {
   const PolArgs p = {tokens, mask, lb, lt, b * t, t, v};
-#define PP_CALL(T)                                                                               \
-  hipLaunchKernelGGL((pp_token_lp_kernel<T>), dim3(p.rows), dim3(256), 0, st,                    \
-                     static_cast<const T*>(logits), p, lp, reinterpret_cast<float2*>(stats))
+  const PolTerms q = {};
+#define PP_CALL(T) \
+  run_terms<T, false>(static_cast<const T*>(logits), p, q, reinterpret_cast<float2*>(stats), lp, st)
   PP_POL_TYPES(PP_CALL);
 #undef PP_CALL
   return hipGetLastError();
@@ -228,18 +495,18 @@ hipError_t pp_launch_token_lp_bwd(const void* logits, int64_t lb, int64_t lt, in
                                   const float* coef, const float* gout, int done_if_one, void* grad,
                                   int b, int t, int v, hipStream_t st) {
   const PolArgs p = {tokens, mask, lb, lt, b * t, t, v};
-  const int grid = std::min(p.rows, 4096);
-#define PP_CALL(T)                                                                               \
-  hipLaunchKernelGGL((pp_token_lp_bwd_kernel<T>), dim3(grid), dim3(256), 0, st,                  \
-                     static_cast<const T*>(logits), p, reinterpret_cast<const float2*>(stats),   \
-                     coef, gout, done_if_one, static_cast<T*>(grad))
+#define PP_CALL(T)                                                                                     \
+  run_grad<T>(static_cast<const T*>(logits), p, reinterpret_cast<const float2*>(stats), coef, gout,    \
+              done_if_one, static_cast<T*>(grad), st)
   PP_POL_TYPES(PP_CALL);
 #undef PP_CALL
   return hipGetLastError();
 }
 
+static int padded_rows(int b, int t) { return (b * t + 3) & ~3; }
+
 size_t pp_policy_workspace_bytes(int b, int t) {
-  return ((size_t)b + 3 * (size_t)b * t) * sizeof(float);
+  return ((((size_t)b + 3) & ~(size_t)3) + 3 * (size_t)padded_rows(b, t)) * sizeof(float);
 }
 
 hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtype,
@@ -248,17 +515,18 @@ hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtyp
                             float high, float beta, int by_sequence, float* out, float* stats,
                             float* coef, void* grad, void* ws, int b, int t, int v, hipStream_t st) {
   const PolArgs p = {tokens, mask, lb, lt, b * t, t, v};
-  const PolTerms q = {old, adv, ref, ab, at, low, high, beta};
   float* weight = static_cast<float*>(ws);
-  float* terms = weight + b;
-  hipLaunchKernelGGL(pp_policy_weight_kernel, dim3(1), dim3(1024), 0, st, mask, b, t, by_sequence,
-                     weight);
-#define PP_CALL(T)                                                                                \
-  hipLaunchKernelGGL((pp_policy_kernel<T>), dim3(p.rows), dim3(256), 0, st,                       \
-                     static_cast<const T*>(logits), p, q, weight, reinterpret_cast<float2*>(stats), \
-                     coef, terms, static_cast<T*>(grad))
+  // (without a mask both means are the mean over all tokens)
+  const PolTerms q = {old, adv, ref, ab, at, low, high, beta, mask ? weight : nullptr,
+                      1.0f / ((float)b * (float)t), weight + ((b + 3) & ~3), padded_rows(b, t)};
+  if (mask)
+    hipLaunchKernelGGL(pp_policy_weight_kernel, dim3(1), dim3(1024), 0, st, mask, b, t, by_sequence,
+                       weight);
+#define PP_CALL(T)                                                                                      \
+  run_policy<T>(static_cast<const T*>(logits), p, q, reinterpret_cast<float2*>(stats), coef,            \
+                static_cast<T*>(grad), st)
   PP_POL_TYPES(PP_CALL);
 #undef PP_CALL
-  hipLaunchKernelGGL(pp_policy_finish_kernel, dim3(3), dim3(1024), 0, st, terms, p.rows, out);
+  hipLaunchKernelGGL(pp_policy_finish_kernel, dim3(3), dim3(1024), 0, st, q.terms, p.rows, q.padded, out);
   return hipGetLastError();
 }
