@@ -1400,29 +1400,30 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     dtype, device = params[0].dtype, params[0].device
     if (masters is not None) != (dtype != torch.float32):
         raise ValueError("adamw_step: masters belong to bfloat16 and float16 params, and these need them")
-    sizes, at = [], {"params": []}
+    index, at = device.index, {"params": [p.data_ptr() for p in params]}
+    sizes, shapes = [p.numel() for p in params], [p.shape for p in params]
+    # the strides that all tensors of a param share; None: contiguous
+    strides = [None if p.is_contiguous() else p.stride() for p in params]
     for i, p in enumerate(params):
-        if p.dtype != dtype or p.device != device:
+        if p.dtype is not dtype or p.get_device() != index:
             raise TypeError(f"adamw_step: params[{i}] is {p.dtype} on {p.device}, params[0] {dtype} on {device}")
-        if not dense_storage(p):
+        if strides[i] is not None and not dense_storage(p):
             raise ValueError(f"adamw_step: params[{i}] has gaps or overlaps (strides {p.stride()})")
-        sizes.append(p.numel())
-        at["params"].append(p.data_ptr())
-    shapes, strides = [p.shape for p in params], [p.stride() for p in params]
     moment = torch.uint8 if eight else torch.float32
     wanted = {"grads": dtype, "exp_avgs": moment, "exp_avg_sqs": moment, "masters": torch.float32}
     for name, x in lists.items():
-        if name in wanted:
-            kind = wanted[name]
-            bad = [i for i, t in enumerate(x) if t.dtype != kind or t.shape != shapes[i] or
-                   t.stride() != strides[i] or t.device != device]
-        else:
-            bad = [i for i, t in enumerate(x) if t.dtype != torch.uint8 or t.numel() != -(-sizes[i] // 256) or
-                   not t.is_contiguous() or t.device != device]
-        if bad:
-            i, t = bad[0], x[bad[0]]
-            raise ValueError(f"adamw_step: {name}[{i}] ({t.dtype}, {tuple(t.shape)}, strides {t.stride()}, {t.device}) "
-                             f"does not fit params[{i}] ({dtype}, {tuple(shapes[i])}, strides {strides[i]}, {device})")
+        kind = wanted.get(name)
+        for i, t in enumerate(x):
+            if t.get_device() == index:
+                if kind is None:
+                    if t.dtype is torch.uint8 and t.numel() == -(-sizes[i] // 256) and t.is_contiguous():
+                        continue
+                elif t.dtype is kind and t.shape == shapes[i] and (
+                        t.is_contiguous() if strides[i] is None else t.stride() == strides[i]):
+                    continue
+            raise ValueError(
+                f"adamw_step: {name}[{i}] ({t.dtype}, {tuple(t.shape)}, strides {t.stride()}, {t.device}) does not "
+                f"fit params[{i}] ({dtype}, {tuple(shapes[i])}, strides {params[i].stride()}, {device})")
         at[name] = [t.data_ptr() for t in x]
     live = range(n) if min(sizes) else [i for i in range(n) if sizes[i]]
     for name, x in at.items():  # two updates of the same memory would race
