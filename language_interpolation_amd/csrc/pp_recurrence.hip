@@ -212,13 +212,169 @@ __device__ __forceinline__ void draw_tile(const RecArgs& p, int* shared, int& c,
   g = id % p.ngroup;
 }
 
+// The walks over the steps of a stretch.  FAST: all steps exist and none drops the state, which is
+// nearly always so; the general form costs twice the scalar and vector instructions, and either
+// kernel issues for half of its time.  fr, zr, gr: rows as they came; addresses advance by a row.
+template <bool FAST, typename T, int V>
+__device__ __forceinline__ void load_rows(typename PPElems<T, V>::raw (&fr)[kSteps], const T* fp, int64_t fl,
+                                          typename PPElems<T, V>::raw (&zr)[kSteps], const T* zp, int64_t zl,
+                                          uint32_t ch, int n) {
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    fr[j] = PPElems<T, V>::load(fp + ch);
+    zr[j] = PPElems<T, V>::load(zp + ch);
+    if (FAST || j + 1 < n) {  // behind the last: the last again
+      fp += fl;
+      zp += zl;
+    }
+  }
+}
+
+// hl, pl of each step: the state from 0 at the start of the stretch, the product of its a until then.
+template <bool FAST, typename T, int V>
+__device__ __forceinline__ void first_walk(const T* zp, int64_t zl, const T* fp, int64_t fl, uint32_t ch, int n,
+                                           uint32_t cut, float (&hl)[kSteps][V], float (&pl)[kSteps][V],
+                                           float (&P)[V], float (&H)[V]) {
+  typedef PPElems<T, V> E;
+  typename E::raw fr[kSteps], zr[kSteps];
+  load_rows<FAST, T, V>(fr, fp, fl, zr, zp, zl, ch, n);
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    float fv[V], zv[V];
+    E::get(fr[j], fv);
+    E::get(zr[j], zv);
+    if (FAST || j < n) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float a = gate<sizeof(T) == 4>(fv[v]);
+        if (!FAST && (cut >> j & 1)) {
+          P[v] = -0.0f;
+          H[v] = 0.0f;
+        }
+        H[v] = fmaf(a, H[v] - zv[v], zv[v]);
+        P[v] *= a;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      hl[j][v] = H[v];
+      pl[j][v] = P[v];
+    }
+  }
+}
+
+// y of each step from the state h that enters the stretch.
+template <bool FAST, typename T, int V>
+__device__ __forceinline__ void second_walk(T* yp, int d, uint32_t ch, int n, int rows,
+                                            const float (&hl)[kSteps][V], const float (&pl)[kSteps][V],
+                                            const float (&h)[V]) {
+  typedef PPElems<T, V> E;
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    float out[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      out[v] = FAST ? fmaf(pl[j][v], h[v], hl[j][v]) : j < n ? through(pl[j][v], hl[j][v], h[v]) : 0.0f;
+    if (FAST || j < rows) E::stream(yp + ch, E::put(out));
+    yp += d;
+  }
+}
+
+// q, gap of each step: its gates and h_{t-1} - z_t; gr: gy; (P, G) of the stretch, backwards.
+template <bool FAST, typename T, int V>
+__device__ __forceinline__ void first_walk_back(const T* zp, int64_t zl, const T* fp, int64_t fl, const T* gp,
+                                                int64_t gl, uint32_t ch, int n, uint32_t cut, float (&h)[V],
+                                                float (&q)[kSteps][V], float (&gap)[kSteps][V],
+                                                typename PPElems<T, V>::raw (&gr)[kSteps], float (&P)[V],
+                                                float (&G)[V]) {
+  typedef PPElems<T, V> E;
+  typename E::raw fr[kSteps], zr[kSteps];
+  load_rows<FAST, T, V>(fr, fp, fl, zr, zp, zl, ch, n);
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    gr[j] = E::load(gp + ch);
+    if (FAST || j + 1 < n) gp += gl;
+  }
+#pragma unroll
+  for (int j = 0; j < kSteps; ++j) {
+    float fv[V], zv[V];
+    E::get(fr[j], fv);
+    E::get(zr[j], zv);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      q[j][v] = gate_code<sizeof(T) == 4>(fv[v]);
+      float a, r;
+      gates(q[j][v], a, r);
+      if (!FAST && (cut >> j & 1)) h[v] = 0.0f;
+      gap[j][v] = h[v] - zv[v];
+      h[v] = fmaf(a, gap[j][v], zv[v]);
+      keep(q[j][v]);
+      keep(gap[j][v]);
+    }
+  }
+#pragma unroll
+  for (int j = kSteps - 1; j >= 0; --j) {
+    if (!FAST && j >= n) continue;
+    float gv[V];
+    E::get(gr[j], gv);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float a, r;
+      gates(q[j][v], a, r);
+      G[v] = a * (gv[v] + G[v]);
+      P[v] *= a;
+      if (!FAST && (cut >> j & 1)) {
+        P[v] = -0.0f;
+        G[v] = 0.0f;
+      }
+    }
+  }
+}
+
+// gz, gf of each step from the gradient u that arrives behind the stretch; u then leaves in front of it.
+template <bool FAST, typename T, int V>
+__device__ __forceinline__ void second_walk_back(T* gzp, T* gfp, int d, uint32_t ch, int n, int rows,
+                                                 uint32_t cut, const float (&q)[kSteps][V],
+                                                 const float (&gap)[kSteps][V],
+                                                 const typename PPElems<T, V>::raw (&gr)[kSteps],
+                                                 float (&u)[V]) {
+  typedef PPElems<T, V> E;
+  gzp += (int64_t)(kSteps - 1) * d;
+  gfp += (int64_t)(kSteps - 1) * d;
+#pragma unroll
+  for (int j = kSteps - 1; j >= 0; --j) {
+    float oz[V], of[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) oz[v] = of[v] = 0.0f;
+    if (FAST || j < n) {
+      float gv[V];
+      E::get(gr[j], gv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        float a, r;
+        gates(q[j][v], a, r);
+        const float e = gv[v] + u[v];
+        u[v] = a * e;
+        oz[v] = e * r;
+        of[v] = (u[v] * r) * gap[j][v];
+        if (!FAST && (cut >> j & 1)) u[v] = 0.0f;
+      }
+    }
+    if (FAST || j < rows) {
+      E::stream(gzp + ch, E::put(oz));
+      E::stream(gfp + ch, E::put(of));
+    }
+    gzp -= d;
+    gfp -= d;
+  }
+}
+
 template <typename T, int V>
 __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T* __restrict__ z,
                                                                  const T* __restrict__ f,
                                                                  T* __restrict__ y,
                                                                  float* __restrict__ h_last,
                                                                  float* __restrict__ starts, RecArgs p) {
-  typedef PPElems<T, V> E;
   __shared__ float2 part[kMostWaves][V][64];
   __shared__ float carry[V][64];
   __shared__ int drawn;
@@ -236,7 +392,6 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
   const int64_t chain = (int64_t)b * p.ngroup + g;
   const int64_t row0 = (int64_t)b * p.l + t0;
 
-  // of each step: the state from 0 at the start of the stretch, and the product of its a until then
   float hl[kSteps][V] = {}, pl[kSteps][V] = {};
   float P[V], H[V];
 #pragma unroll
@@ -245,40 +400,16 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
     H[v] = 0.0f;
   }
   uint32_t cut = 0;
+  bool fast = false;
   if (n > 0) {
     cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
     const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
     const T* fp = f + b * p.fb + t0 * p.fl;
-    typename E::raw fr[kSteps], zr[kSteps];
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      const int64_t t = min(j, n - 1);
-      fr[j] = E::load(fp + t * p.fl + chl);
-      zr[j] = E::load(zp + t * p.zl + chl);
-    }
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      float fv[V], zv[V];
-      E::get(fr[j], fv);
-      E::get(zr[j], zv);
-      if (j < n) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float a = gate<sizeof(T) == 4>(fv[v]);
-          if (cut >> j & 1) {
-            P[v] = -0.0f;
-            H[v] = 0.0f;
-          }
-          H[v] = fmaf(a, H[v] - zv[v], zv[v]);
-          P[v] *= a;
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        hl[j][v] = H[v];
-        pl[j][v] = P[v];
-      }
-    }
+    fast = n == kSteps && cut == 0;
+    if (fast)
+      first_walk<true, T, V>(zp, p.zl, fp, p.fl, chl, n, cut, hl, pl, P, H);
+    else
+      first_walk<false, T, V>(zp, p.zl, fp, p.fl, chl, n, cut, hl, pl, P, H);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) part[wave][v][lane] = make_float2(P[v], H[v]);
@@ -331,13 +462,10 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
     for (int v = 0; v < V; ++v) at[chl + v] = h[v];
   }
   T* yp = y + row0 * p.d;
-#pragma unroll
-  for (int j = 0; j < kSteps; ++j) {
-    float out[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = j < n ? through(pl[j][v], hl[j][v], h[v]) : 0.0f;
-    if (j < rows) E::stream(yp + (int64_t)j * p.d + chl, E::put(out));
-  }
+  if (fast)
+    second_walk<true, T, V>(yp, p.d, chl, n, rows, hl, pl, h);
+  else
+    second_walk<false, T, V>(yp, p.d, chl, n, rows, hl, pl, h);
   if ((n > 0 && t0 + n == len) || (len == 0 && c == 0 && wave == 0)) {
 #pragma unroll
     for (int v = 0; v < V; ++v) h_last[(int64_t)b * p.d + ch + v] = through(P[v], H[v], h[v]);
@@ -379,58 +507,21 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
     G[v] = 0.0f;
   }
   uint32_t cut = 0;
+  bool fast = false;
   if (n > 0) {
     cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
     const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
     const T* fp = f + b * p.fb + t0 * p.fl;
     const T* gp = gy + b * p.gb + t0 * p.gl;
     const float* sp = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d;
-    typename E::raw fr[kSteps], zr[kSteps];
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = sp[chl + v];
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      const int64_t t = min(j, n - 1);
-      fr[j] = E::load(fp + t * p.fl + chl);
-      zr[j] = E::load(zp + t * p.zl + chl);
-    }
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) gr[j] = E::load(gp + (int64_t)min(j, n - 1) * p.gl + chl);
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      float fv[V], zv[V];
-      E::get(fr[j], fv);
-      E::get(zr[j], zv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        q[j][v] = gate_code<sizeof(T) == 4>(fv[v]);
-        float a, r;
-        gates(q[j][v], a, r);
-        if (cut >> j & 1) h[v] = 0.0f;
-        gap[j][v] = h[v] - zv[v];
-        h[v] = fmaf(a, gap[j][v], zv[v]);
-        keep(q[j][v]);
-        keep(gap[j][v]);
-      }
-    }
-#pragma unroll
-    for (int j = kSteps - 1; j >= 0; --j) {
-      if (j >= n) continue;
-      float gv[V];
-      E::get(gr[j], gv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a, r;
-        gates(q[j][v], a, r);
-        G[v] = a * (gv[v] + G[v]);
-        P[v] *= a;
-        if (cut >> j & 1) {
-          P[v] = -0.0f;
-          G[v] = 0.0f;
-        }
-      }
-    }
+    fast = n == kSteps && cut == 0;
+    if (fast)
+      first_walk_back<true, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, chl, n, cut, h, q, gap, gr, P, G);
+    else
+      first_walk_back<false, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, chl, n, cut, h, q, gap, gr, P, G);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) part[wave][v][lane] = make_float2(P[v], G[v]);
@@ -480,29 +571,10 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
   keep_all<V>(q);
   T* gzp = gz + row0 * p.d;
   T* gfp = gf + row0 * p.d;
-#pragma unroll
-  for (int j = kSteps - 1; j >= 0; --j) {
-    float oz[V], of[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) oz[v] = of[v] = 0.0f;
-    if (j < n) {
-      float gv[V];
-      E::get(gr[j], gv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a, r;
-        gates(q[j][v], a, r);
-        const float e = gv[v] + u[v];
-        oz[v] = e * r;
-        of[v] = (e * gap[j][v]) * (a * r);
-        u[v] = cut >> j & 1 ? 0.0f : a * e;
-      }
-    }
-    if (j < rows) {
-      E::stream(gzp + (int64_t)j * p.d + chl, E::put(oz));
-      E::stream(gfp + (int64_t)j * p.d + chl, E::put(of));
-    }
-  }
+  if (fast)
+    second_walk_back<true, T, V>(gzp, gfp, p.d, chl, n, rows, cut, q, gap, gr, u);
+  else
+    second_walk_back<false, T, V>(gzp, gfp, p.d, chl, n, rows, cut, q, gap, gr, u);
   if (gh0 && chunk0 == 0 && wave == 0) {
 #pragma unroll
     for (int v = 0; v < V; ++v) gh0[(int64_t)b * p.d + ch + v] = u[v];
@@ -543,9 +615,12 @@ bool fits(int v, size_t size, std::initializer_list<const void*> at, std::initia
   return true;
 }
 
+// A short row is one chunk, others are cut into chunks of kMostWaves stretches: with half of that the
+// long chains wait twice as often (bf16 [1, 100003, 640] forward + backward 292 against 248 us, fp32
+// [4, 1024, 2048] 75 against 64), and where nothing waits little is gained ([2, 8192, 2048] 129, 131).
 void plan(RecArgs& p, int v, void* ws) {
   p.ngroup = (p.d + 64 * v - 1) / (64 * v);
-  p.chunk = kSteps * std::min(kMostWaves, (p.l + kSteps - 1) / kSteps);  // a short row is one chunk
+  p.chunk = kSteps * std::min(kMostWaves, (p.l + kSteps - 1) / kSteps);
   p.nchunk = (p.l + p.chunk - 1) / p.chunk;
   p.ticket = static_cast<uint32_t*>(ws);
   const int64_t n = (int64_t)p.b * p.nchunk * p.ngroup * 64 * v;
@@ -560,14 +635,12 @@ void fill(const RecArgs& p, int v, hipStream_t st) {
                      p.ticket, words);
 }
 
-// One channel a lane in the forward, whatever the type: 60 registers, twice the waves of two channels a
-// lane (114).  bf16 [8, 2048, 2048]: 55 against 59 us, [1, 100003, 640]: 112 against 120 us.
-template <typename T>
+template <typename T, int V>
 void run_fwd(const void* z, const void* f, void* y, float* h_last, float* starts, RecArgs p, void* ws,
              hipStream_t st) {
-  plan(p, 1, ws);
-  fill(p, 1, st);
-  hipLaunchKernelGGL((pp_rec_fwd_kernel<T, 1>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
+  plan(p, V, ws);
+  fill(p, V, st);
+  hipLaunchKernelGGL((pp_rec_fwd_kernel<T, V>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
                      dim3(4 * p.chunk), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
                      static_cast<T*>(y), h_last, starts, p);
 }
@@ -611,7 +684,15 @@ hipError_t pp_launch_rec_fwd(const void* z, int64_t zb, int64_t zl, const void* 
                              const uint8_t* reset, void* y, float* h_last, float* starts, void* ws,
                              int b, int l, int d, hipStream_t st) {
   const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, 0, 0, 0, h0, lengths, reset, nullptr, nullptr, nullptr};
-#define PP_CALL(T) run_fwd<T>(z, f, y, h_last, starts, p, ws, st)
+  // Two channels a lane in 16-bit types, one in fp32: 4 bytes an access either way.
+  const bool two = dtype != PP_F32 && fits(2, 2, {z, f, y}, {zb, zl, fb, fl, (int64_t)d});
+#define PP_CALL(T)                                                                      \
+  do {                                                                                  \
+    if (sizeof(T) == 2 && two)                                                          \
+      run_fwd<T, sizeof(T) == 2 ? 2 : 1>(z, f, y, h_last, starts, p, ws, st);           \
+    else                                                                                \
+      run_fwd<T, 1>(z, f, y, h_last, starts, p, ws, st);                                \
+  } while (0)
   PP_REC_TYPES(PP_CALL);
 #undef PP_CALL
 }
@@ -623,8 +704,8 @@ hipError_t pp_launch_rec_bwd(const void* z, int64_t zb, int64_t zl, const void* 
                              int l, int d, hipStream_t st) {
   const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, 0, 0, 0, nullptr, lengths, reset, nullptr, nullptr, nullptr};
   const size_t s = dtype == PP_F32 ? 4 : 2;
-  // Two channels a lane in 16-bit types: with one, the 2-byte accesses of five tensors are the limit
-  // (bf16 [1, 100003, 640]: 154 against 201 us).  In fp32 two would need more registers than there are.
+  // (as in the forward; one channel a lane costs [1, 100003, 640] in bf16 201 instead of 144 us, two in
+  // fp32 more registers than there are)
   const bool two = s == 2 && fits(2, s, {z, f, gy, gz, gf}, {zb, zl, fb, fl, gb, gl, (int64_t)d});
 #define PP_CALL(T)                                                           \
   do {                                                                       \
