@@ -490,30 +490,31 @@ int pp_gated_recurrence_step(const void* z, int64_t zb, const void* f, int64_t f
  *   lp = logits[token] - logsumexp(logits)                                     (0 where masked)
  * stats: NULL, or [b][t][2] floats for the backward, which writes
  *   grad = gout[0] * coef[b][t] * (onehot(token) - softmax)     (zeros where masked; gout NULL: 1)
- * with the logits' strides; where those leave gaps, the gaps are not written.  done_if_one: grad
- * holds the result for gout = 1 already.
+ * with strides (gb, gt): rows do not overlap and start at the same offset within 16 bytes as the
+ * logits' (gb - lb, gt - lt and the difference of the addresses are multiples of 16 bytes); what lies
+ * between rows is not written.  done_if_one: grad holds the result for gout = 1 already.
  *   rho = exp(lp - old);  k = exp(ref - lp) - (ref - lp) - 1
  *   loss = mean(-min(rho adv, clip(rho, 1 - clip_low, 1 + clip_high) adv) + kl_coef k)
  * out[0] = loss, out[1] = mean k (ref NULL: 0, and no such term), out[2] = share of the tokens whose
  * ratio was clipped.  The mean is over the tokens that count, or (by_sequence) over the means of
  * the sequences that have any; nothing counts: 0.  old, ref: [b][t] fp32; adv: fp32 with strides
- * (ab, at), 0 where it is shared.  stats, coef ([b][t] floats: dloss/dlp) and grad (dloss/dlogits,
- * the logits' strides and alignment to 16 bytes) are written unless stats / grad are NULL.
+ * (ab, at), 0 where it is shared.  stats and coef ([b][t] floats: dloss/dlp) are written unless NULL,
+ * grad (dloss/dlogits, strides as above) unless NULL; a grad needs stats and coef.
  * Bitwise reproducible. */
 int pp_token_log_probs_fwd(const void* logits, int64_t lb, int64_t lt, int dtype,
                            const int64_t* tokens, const uint8_t* mask, float* lp, float* stats,
                            int b, int t, int v, void* stream);
 int pp_token_log_probs_bwd(const void* logits, int64_t lb, int64_t lt, int dtype,
                            const int64_t* tokens, const uint8_t* mask, const float* stats,
-                           const float* coef, const float* gout, int done_if_one, void* grad, int b,
-                           int t, int v, void* stream);
+                           const float* coef, const float* gout, int done_if_one, void* grad,
+                           int64_t gb, int64_t gt, int b, int t, int v, void* stream);
 size_t pp_clipped_policy_loss_workspace_bytes(int b, int t);
 int pp_clipped_policy_loss_fwd(const void* logits, int64_t lb, int64_t lt, int dtype,
                                const int64_t* tokens, const uint8_t* mask, const float* old_lp,
                                const float* adv, int64_t ab, int64_t at, const float* ref_lp,
                                float clip_low, float clip_high, float kl_coef, int by_sequence,
-                               float* out, float* stats, float* coef, void* grad, void* workspace,
-                               size_t workspace_bytes, int b, int t, int v, void* stream);
+                               float* out, float* stats, float* coef, void* grad, int64_t gb, int64_t gt,
+                               void* workspace, size_t workspace_bytes, int b, int t, int v, void* stream);
 
 /* AdamW beside Lion (csrc/pp_adamw.hip), `count` <= PP_OPT_MAX_TENSORS tensors in one launch:
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2

@@ -132,12 +132,12 @@ SIGNATURES = {
     "pp_gated_recurrence_step": (c_int, [_P, c_int64, _P, c_int64, c_int, _P, c_int64, _P, c_int,
                                          c_int, _P]),
     "pp_token_log_probs_fwd": (c_int, [_P, c_int64, c_int64, c_int] + [_P] * 4 + [c_int] * 3 + [_P]),
-    "pp_token_log_probs_bwd": (c_int, [_P, c_int64, c_int64, c_int] + [_P] * 5 + [c_int, _P] +
-                               [c_int] * 3 + [_P]),
+    "pp_token_log_probs_bwd": (c_int, [_P, c_int64, c_int64, c_int] + [_P] * 5 +
+                               [c_int, _P, c_int64, c_int64] + [c_int] * 3 + [_P]),
     "pp_clipped_policy_loss_workspace_bytes": (c_size_t, [c_int, c_int]),
     "pp_clipped_policy_loss_fwd": (c_int, [_P, c_int64, c_int64, c_int] + [_P] * 4 +
-                                   [c_int64, c_int64, _P] + [c_float] * 3 + [c_int] + [_P] * 5 +
-                                   [c_size_t] + [c_int] * 3 + [_P]),
+                                   [c_int64, c_int64, _P] + [c_float] * 3 + [c_int] + [_P] * 4 +
+                                   [c_int64, c_int64, _P, c_size_t] + [c_int] * 3 + [_P]),
     "pp_moment_blocks": (c_int64, [c_int64]),
     "pp_count_step": (c_int, [c_int, _P, _P]),
     "pp_adamw_step": (c_int, [c_int] * 3 + [_P] * 10 + [c_double] * 5 + [_P, c_uint32, c_uint32, _P]),

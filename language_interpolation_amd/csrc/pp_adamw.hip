@@ -306,7 +306,7 @@ hipError_t pp_launch_adamw(int count, int dtype, int bits, void* const* p, const
     blocks += (numel[t] + per_block - 1) / per_block;
   }
   d.first[count] = (int)blocks;
-  if (blocks >= (1LL << 31)) return hipErrorInvalidValue;
+  if (blocks >= (1LL << 24)) return hipErrorInvalidValue;  // 2^32 threads
   const dim3 grid((unsigned)blocks), block(256);
 #define PP_ADAMW(T)                                                                             \
   do {                                                                                          \
@@ -324,7 +324,7 @@ hipError_t pp_launch_adamw(int count, int dtype, int bits, void* const* p, const
 hipError_t pp_launch_decode_moment(const uint8_t* code, const uint8_t* exps, void* out, int dtype,
                                    int is_signed, int64_t n, hipStream_t st) {
   const int64_t blocks = (n + 2047) / 2048;
-  if (blocks >= (1LL << 31)) return hipErrorInvalidValue;
+  if (blocks >= (1LL << 24)) return hipErrorInvalidValue;
   const int wide = (size_t)code % 8 == 0 && (size_t)out % 16 == 0;
   const dim3 grid((unsigned)blocks), block(256);
 #define PP_DECODE(T)                                                                             \

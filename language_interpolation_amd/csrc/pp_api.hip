@@ -875,9 +875,11 @@ static size_t elem_size(int dtype) { return dtype == PP_F32 ? 4 : 2; }
 static int rec_args_ok(int dtype, int b, int l, int d) {
   if (!elem_ok(dtype)) return PP_ERR_METHOD;
   if (b < 1 || l < 1 || d < 1 || b > 65535) return PP_ERR_SHAPE;
-  if ((int64_t)b * l >= (1LL << 31) || (int64_t)l + 4096 >= (1LL << 31) || d > (1 << 24) ||
-      (int64_t)b * ((l + 127) / 128) * ((d + 63) / 64) >= (1LL << 31))  // workgroups
+  if ((int64_t)b * l >= (1LL << 31) || (int64_t)l + 4096 >= (1LL << 31) || d > (1 << 24))
     return PP_ERR_RANGE;
+  // a launch has fewer than 2^32 threads: 64 for up to 16 steps of 64 channels, 1024 for 256 steps
+  const int64_t threads = l <= 256 ? 64 * ((l + 15) / 16) : 1024 * (((int64_t)l + 255) / 256);
+  if ((int64_t)b * ((d + 63) / 64) >= (1LL << 32) / threads) return PP_ERR_RANGE;
   return PP_OK;
 }
 
@@ -934,6 +936,7 @@ int pp_gated_recurrence_step(const void* z, int64_t zb, const void* f, int64_t f
   int rc = rec_args_ok(dtype, b, 1, d);
   if (rc != PP_OK) return rc;
   if (hb < d && b > 1) return PP_ERR_SHAPE;  // two sequences would share a state
+  if ((int64_t)b * d >= (1LL << 32)) return PP_ERR_RANGE;
   const size_t s = elem_size(dtype);
   if (!aligned_to(z, s) || !aligned_to(f, s) || !aligned_to(y, s) || !aligned_to(h, 4))
     return PP_ERR_ALIGN;
@@ -944,6 +947,16 @@ static int pol_args_ok(int dtype, int b, int t, int v) {
   if (!elem_ok(dtype)) return PP_ERR_METHOD;
   if (b < 1 || t < 1 || v < 1) return PP_ERR_SHAPE;
   if ((int64_t)b * t >= (1LL << 30) || v > (1 << 30)) return PP_ERR_RANGE;
+  return PP_OK;
+}
+
+// A gradient's rows do not overlap and begin at the logits' offsets within 16 bytes.
+static int grad_rows_ok(const void* logits, int64_t lb, int64_t lt, const void* grad, int64_t gb, int64_t gt,
+                        int dtype, int b, int t, int v) {
+  const int64_t vec = 16 / (int64_t)elem_size(dtype);
+  if ((t > 1 && gt < v) || (b > 1 && gb < (t - 1) * gt + v)) return PP_ERR_SHAPE;
+  if ((((size_t)logits ^ (size_t)grad) & 15) || (t > 1 && (gt - lt) % vec) || (b > 1 && (gb - lb) % vec))
+    return PP_ERR_ALIGN;
   return PP_OK;
 }
 
@@ -962,16 +975,18 @@ int pp_token_log_probs_fwd(const void* logits, int64_t lb, int64_t lt, int dtype
 
 int pp_token_log_probs_bwd(const void* logits, int64_t lb, int64_t lt, int dtype,
                            const int64_t* tokens, const uint8_t* mask, const float* stats,
-                           const float* coef, const float* gout, int done_if_one, void* grad, int b,
-                           int t, int v, void* stream) {
+                           const float* coef, const float* gout, int done_if_one, void* grad,
+                           int64_t gb, int64_t gt, int b, int t, int v, void* stream) {
   if (!logits || !tokens || !stats || !coef || !grad) return PP_ERR_NULL;
   int rc = pol_args_ok(dtype, b, t, v);
   if (rc != PP_OK) return rc;
   if (!aligned_to(logits, elem_size(dtype)) || !aligned_to(tokens, 8) || !aligned_to(coef, 4) ||
-      !aligned_to(stats, 8) || (((size_t)logits ^ (size_t)grad) & 15))
+      !aligned_to(stats, 8) || !aligned_to(gout, 4))
     return PP_ERR_ALIGN;
+  rc = grad_rows_ok(logits, lb, lt, grad, gb, gt, dtype, b, t, v);
+  if (rc != PP_OK) return rc;
   return hip_rc(pp_launch_token_lp_bwd(logits, lb, lt, dtype, tokens, mask, stats, coef, gout,
-                                       done_if_one, grad, b, t, v, (hipStream_t)stream));
+                                       done_if_one, grad, gb, gt, b, t, v, (hipStream_t)stream));
 }
 
 size_t pp_clipped_policy_loss_workspace_bytes(int b, int t) {
@@ -982,21 +997,25 @@ int pp_clipped_policy_loss_fwd(const void* logits, int64_t lb, int64_t lt, int d
                                const int64_t* tokens, const uint8_t* mask, const float* old_lp,
                                const float* adv, int64_t ab, int64_t at, const float* ref_lp,
                                float clip_low, float clip_high, float kl_coef, int by_sequence,
-                               float* out, float* stats, float* coef, void* grad, void* workspace,
-                               size_t workspace_bytes, int b, int t, int v, void* stream) {
-  if (!logits || !tokens || !old_lp || !adv || !out || (stats && !coef)) return PP_ERR_NULL;
+                               float* out, float* stats, float* coef, void* grad, int64_t gb, int64_t gt,
+                               void* workspace, size_t workspace_bytes, int b, int t, int v, void* stream) {
+  if (!logits || !tokens || !old_lp || !adv || !out || (grad && (!stats || !coef))) return PP_ERR_NULL;
   int rc = pol_args_ok(dtype, b, t, v);
   if (rc != PP_OK) return rc;
   if (!(clip_low >= 0.0f) || !(clip_high >= 0.0f)) return PP_ERR_SHAPE;
   if (!aligned_to(logits, elem_size(dtype)) || !aligned_to(tokens, 8) || !aligned_to(old_lp, 4) ||
       !aligned_to(adv, 4) || !aligned_to(ref_lp, 4) || !aligned_to(out, 4) || !aligned_to(coef, 4) ||
-      !aligned_to(stats, 8) || (grad && (((size_t)logits ^ (size_t)grad) & 15)))
+      !aligned_to(stats, 8))
     return PP_ERR_ALIGN;
+  if (grad) {
+    rc = grad_rows_ok(logits, lb, lt, grad, gb, gt, dtype, b, t, v);
+    if (rc != PP_OK) return rc;
+  }
   if (!workspace || workspace_bytes < pp_policy_workspace_bytes(b, t)) return PP_ERR_WORKSPACE;
   if (!aligned16(workspace)) return PP_ERR_ALIGN;
   return hip_rc(pp_launch_policy(logits, lb, lt, dtype, tokens, mask, old_lp, adv, ab, at, ref_lp,
-                                 clip_low, clip_high, kl_coef, by_sequence, out, stats, coef, grad,
-                                 workspace, b, t, v, (hipStream_t)stream));
+                                 clip_low, clip_high, kl_coef, by_sequence, out, stats, coef, grad, gb,
+                                 gt, workspace, b, t, v, (hipStream_t)stream));
 }
 
 int64_t pp_moment_blocks(int64_t numel) { return numel > 0 ? (numel + 255) / 256 : 0; }
@@ -1025,13 +1044,15 @@ int pp_adamw_step(int count, int dtype, int moment_bits, void* const* p, const v
   if ((dtype != PP_F32 && !master) || (moment_bits == 8 && (!m_exp || !v_exp))) return PP_ERR_NULL;
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return PP_ERR_SHAPE;
   const size_t s = elem_size(dtype), ms = moment_bits / 8;
+  int64_t blocks = 0;
   if (!aligned_to(grad_scale, 4)) return PP_ERR_ALIGN;
   for (int t = 0; t < count; ++t) {
     if (!p[t] || !g[t] || !m[t] || !v[t] || (dtype != PP_F32 && !master[t]) ||
         (moment_bits == 8 && (!m_exp[t] || !v_exp[t])) || (step_dev && !step_dev[t]))
       return PP_ERR_NULL;
     if (numel[t] < 1 || (!step_dev && step[t] < 1)) return PP_ERR_SHAPE;
-    if (numel[t] > (1LL << 36)) return PP_ERR_RANGE;
+    blocks += numel[t] / (moment_bits == 8 ? 2048 : 1024) + 1;
+    if (numel[t] > (1LL << 36) || blocks >= (1LL << 24)) return PP_ERR_RANGE;  // of a launch: 2^32 threads
     if (!aligned_to(p[t], s) || !aligned_to(g[t], s) || !aligned_to(m[t], ms) ||
         !aligned_to(v[t], ms) || (dtype != PP_F32 && !aligned_to(master[t], 4)) ||
         (step_dev && !aligned_to(step_dev[t], 8)))
@@ -1047,7 +1068,7 @@ int pp_decode_moment(const uint8_t* codes, const uint8_t* exponents, void* out, 
   if (!codes || !exponents || !out) return PP_ERR_NULL;
   if (!elem_ok(dtype)) return PP_ERR_METHOD;
   if (numel < 1) return PP_ERR_SHAPE;
-  if (numel > (1LL << 36)) return PP_ERR_RANGE;
+  if (numel >= (1LL << 35)) return PP_ERR_RANGE;
   if (!aligned_to(out, elem_size(dtype))) return PP_ERR_ALIGN;
   return hip_rc(pp_launch_decode_moment(codes, exponents, out, dtype, is_signed, numel,
                                         (hipStream_t)stream));

@@ -199,13 +199,14 @@ hipError_t pp_launch_token_lp(const void* logits, int64_t lb, int64_t lt, int dt
 hipError_t pp_launch_token_lp_bwd(const void* logits, int64_t lb, int64_t lt, int dtype,
                                   const int64_t* tokens, const uint8_t* mask, const float* stats,
                                   const float* coef, const float* gout, int done_if_one, void* grad,
-                                  int b, int t, int v, hipStream_t st);
+                                  int64_t gb, int64_t gt, int b, int t, int v, hipStream_t st);
 size_t pp_policy_workspace_bytes(int b, int t);
 hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtype,
                             const int64_t* tokens, const uint8_t* mask, const float* old,
                             const float* adv, int64_t ab, int64_t at, const float* ref, float low,
                             float high, float beta, int by_sequence, float* out, float* stats,
-                            float* coef, void* grad, void* ws, int b, int t, int v, hipStream_t st);
+                            float* coef, void* grad, int64_t gb, int64_t gt, void* ws, int b, int t, int v,
+                            hipStream_t st);
 
 // ---- AdamW over many tensors (pp_adamw.hip) ----
 hipError_t pp_launch_count_step(int count, int64_t* const* step, hipStream_t st);

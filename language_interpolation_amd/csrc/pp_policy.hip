@@ -27,8 +27,10 @@ constexpr float kLog2e = 1.44269504f;
 struct PolArgs {
   const int64_t* tokens;
   const uint8_t* mask;
-  int64_t lb, lt;  // strides of the logits (and of their gradient) over batch and time
-  int rows, t, v;
+  int64_t lb, lt, gb, gt;  // strides of the logits and of their gradient over batch and time
+  int first, rows, t, v;   // of this launch: rows first .. rows - 1
+  __device__ __forceinline__ int64_t logits_at(int row) const { return (row / t) * lb + (row % t) * lt; }
+  __device__ __forceinline__ int64_t grad_at(int row) const { return (row / t) * gb + (row % t) * gt; }
 };
 struct PolTerms {
   const float* old;
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(256) void pp_row_terms_kernel(const T* __restrict__
                                                            float* __restrict__ out) {
   __shared__ float red[4];
   const int tid = threadIdx.x % THREADS;
-  const int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  const int row = p.first + blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
   if (row >= p.rows) return;
   if (p.mask && !p.mask[row]) {
     if (tid == 0) {
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(256) void pp_row_terms_kernel(const T* __restrict__
     }
     return;
   }
-  const T* x = logits + (row / p.t) * p.lb + (row % p.t) * p.lt;
+  const T* x = logits + p.logits_at(row);
   const float2 st = stream_stats<T, THREADS>(x, p.v, tid, red);
   if (tid == 0) {
     const float lp = token_lp(x, p.tokens[row], p.v, st);
@@ -241,9 +243,8 @@ __global__ __launch_bounds__(256) void pp_row_grad_kernel(const T* __restrict__ 
   const int tid = threadIdx.x % THREADS;
   for (int row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS; row < p.rows;
        row += gridDim.x * (256 / THREADS)) {
-    const int64_t at = (row / p.t) * p.lb + (row % p.t) * p.lt;
-    const T* x = logits + at;
-    T* g = grad + at;
+    const T* x = logits + p.logits_at(row);
+    T* g = grad + p.grad_at(row);
     if (p.mask && !p.mask[row]) {
       zero_row<T, THREADS>(g, p.v, tid);
       continue;
@@ -290,11 +291,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pp_policy_fused
   typedef PPElems<T, kVec> E;
   __shared__ float red[THREADS / 64 > 4 ? THREADS / 64 : 4];
   const int tid = threadIdx.x % THREADS;
-  const int row = blockIdx.x * kRows + threadIdx.x / THREADS;
+  const int row = p.first + blockIdx.x * kRows + threadIdx.x / THREADS;
   if (row >= p.rows) return;
-  const int64_t at = (row / p.t) * p.lb + (row % p.t) * p.lt;
-  const T* x = logits + at;
-  T* g = grad + at;
+  const T* x = logits + p.logits_at(row);
+  T* g = grad + p.grad_at(row);
   if (p.mask && !p.mask[row]) {
     if (tid == 0) {
       stats[row] = make_float2(0.0f, 0.0f);
@@ -419,15 +419,28 @@ __global__ __launch_bounds__(1024) void pp_policy_finish_kernel(const float* __r
 
 constexpr int kWaveRow = 4096;  // bytes up to which a row is one wave's
 
+// A launch takes fewer than 2^32 threads: the rows in slices, `kernel(p, rows)` for each.
+constexpr int kSlice = 1 << 20;
+template <typename F>
+void in_slices(PolArgs p, F kernel) {
+  const int rows = p.rows;
+  for (p.first = 0; p.first < rows; p.first += kSlice) {
+    p.rows = std::min(rows - p.first, kSlice) + p.first;
+    kernel(p, p.rows - p.first);
+  }
+}
+
 template <typename T, bool POLICY>
-void run_terms(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* out,
+void run_terms(const T* logits, const PolArgs& all, const PolTerms& q, float2* stats, float* out,
                hipStream_t st) {
-  if ((int64_t)p.v * (int64_t)sizeof(T) <= kWaveRow)
-    hipLaunchKernelGGL((pp_row_terms_kernel<T, 64, POLICY>), dim3((p.rows + 3) / 4), dim3(256), 0, st,
-                       logits, p, q, stats, out);
-  else
-    hipLaunchKernelGGL((pp_row_terms_kernel<T, 256, POLICY>), dim3(p.rows), dim3(256), 0, st, logits, p,
-                       q, stats, out);
+  in_slices(all, [&](const PolArgs& p, int rows) {
+    if ((int64_t)p.v * (int64_t)sizeof(T) <= kWaveRow)
+      hipLaunchKernelGGL((pp_row_terms_kernel<T, 64, POLICY>), dim3((rows + 3) / 4), dim3(256), 0, st,
+                         logits, p, q, stats, out);
+    else
+      hipLaunchKernelGGL((pp_row_terms_kernel<T, 256, POLICY>), dim3(rows), dim3(256), 0, st, logits, p,
+                         q, stats, out);
+  });
 }
 
 template <typename T>
@@ -442,28 +455,29 @@ void run_grad(const T* logits, const PolArgs& p, const float2* stats, const floa
 }
 
 template <typename T, int THREADS, int NV>
-bool try_fused(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* coef, T* grad,
+bool try_fused(const T* logits, const PolArgs& all, const PolTerms& q, float2* stats, float* coef, T* grad,
                hipStream_t st) {
-  if (p.v > THREADS * NV * Span<T>::kVec) return false;
+  if (all.v > THREADS * NV * Span<T>::kVec) return false;
   constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;
-  hipLaunchKernelGGL((pp_policy_fused_kernel<T, THREADS, NV>), dim3((p.rows + kRows - 1) / kRows),
-                     dim3(THREADS < 256 ? 256 : THREADS), 0, st, logits, p, q, stats, coef, grad);
+  in_slices(all, [&](const PolArgs& p, int rows) {
+    hipLaunchKernelGGL((pp_policy_fused_kernel<T, THREADS, NV>), dim3((rows + kRows - 1) / kRows),
+                       dim3(THREADS < 256 ? 256 : THREADS), 0, st, logits, p, q, stats, coef, grad);
+  });
   return true;
 }
 
 template <typename T>
 void run_policy(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* coef, T* grad,
                 hipStream_t st) {
-  if (grad && stats &&
-      (try_fused<T, 64, 1>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 64, 2>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 64, 4>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 256, 2>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 256, 4>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 256, 8>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 1024, 4>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 1024, 8>(logits, p, q, stats, coef, grad, st) ||
-       try_fused<T, 1024, 16>(logits, p, q, stats, coef, grad, st)))
+  if (grad && (try_fused<T, 64, 1>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 64, 2>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 64, 4>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 256, 2>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 256, 4>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 256, 8>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 1024, 4>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 1024, 8>(logits, p, q, stats, coef, grad, st) ||
+               try_fused<T, 1024, 16>(logits, p, q, stats, coef, grad, st)))
     return;
   run_terms<T, true>(logits, p, q, stats, coef, st);
   if (grad) run_grad<T>(logits, p, stats, coef, nullptr, 0, grad, st);
@@ -481,7 +495,7 @@ void run_policy(const T* logits, const PolArgs& p, const PolTerms& q, float2* st
 hipError_t pp_launch_token_lp(const void* logits, int64_t lb, int64_t lt, int dtype,
                               const int64_t* tokens, const uint8_t* mask, float* lp, float* stats,
                               int b, int t, int v, hipStream_t st) {
-  const PolArgs p = {tokens, mask, lb, lt, b * t, t, v};
+  const PolArgs p = {tokens, mask, lb, lt, 0, 0, 0, b * t, t, v};
   const PolTerms q = {};
 #define PP_CALL(T) \
   run_terms<T, false>(static_cast<const T*>(logits), p, q, reinterpret_cast<float2*>(stats), lp, st)
@@ -493,8 +507,8 @@ hipError_t pp_launch_token_lp(const void* logits, int64_t lb, int64_t lt, int dt
 hipError_t pp_launch_token_lp_bwd(const void* logits, int64_t lb, int64_t lt, int dtype,
                                   const int64_t* tokens, const uint8_t* mask, const float* stats,
                                   const float* coef, const float* gout, int done_if_one, void* grad,
-                                  int b, int t, int v, hipStream_t st) {
-  const PolArgs p = {tokens, mask, lb, lt, b * t, t, v};
+                                  int64_t gb, int64_t gt, int b, int t, int v, hipStream_t st) {
+  const PolArgs p = {tokens, mask, lb, lt, gb, gt, 0, b * t, t, v};
 #define PP_CALL(T)                                                                                     \
   run_grad<T>(static_cast<const T*>(logits), p, reinterpret_cast<const float2*>(stats), coef, gout,    \
               done_if_one, static_cast<T*>(grad), st)
@@ -513,8 +527,9 @@ hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtyp
                             const int64_t* tokens, const uint8_t* mask, const float* old,
                             const float* adv, int64_t ab, int64_t at, const float* ref, float low,
                             float high, float beta, int by_sequence, float* out, float* stats,
-                            float* coef, void* grad, void* ws, int b, int t, int v, hipStream_t st) {
-  const PolArgs p = {tokens, mask, lb, lt, b * t, t, v};
+                            float* coef, void* grad, int64_t gb, int64_t gt, void* ws, int b, int t, int v,
+                            hipStream_t st) {
+  const PolArgs p = {tokens, mask, lb, lt, gb, gt, 0, b * t, t, v};
   float* weight = static_cast<float*>(ws);
   // (without a mask both means are the mean over all tokens)
   const PolTerms q = {old, adv, ref, ab, at, low, high, beta, mask ? weight : nullptr,

@@ -1190,14 +1190,15 @@ def _class_rows(logits):
 
 
 def _class_grad(logits, lb, lt):
-    """An empty gradient with the strides of the logits and their offset within 16 bytes."""
+    """(empty gradient of [b, t, v], its strides): rows at the logits' offsets within 16 bytes, else
+    as close together as that allows (contiguous where the logits are)."""
     b, t, v = logits.shape
+    vec = 16 // logits.element_size()
+    gt = v + (lt - v) % vec
+    gb = t * gt + (lb - t * gt) % vec
     off = logits.data_ptr() % 16 // logits.element_size()
-    if off == 0 and logits.is_contiguous():
-        return torch.empty_like(logits)
-    span = (b - 1) * lb + (t - 1) * lt + v
-    buf = torch.empty(off + span, device=logits.device, dtype=logits.dtype)
-    return buf.as_strided((b, t, v), (lb, lt, 1), off)
+    buf = torch.empty(off + b * gb, device=logits.device, dtype=logits.dtype)
+    return buf.as_strided((b, t, v), (gb, gt, 1), off), gb, gt
 
 
 def _check_classes(logits, tokens, mask):
@@ -1231,7 +1232,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
         logits, tokens, mask, stats = ctx.saved_tensors
         grad = _class_grad(logits, *ctx.strides)
         _class_backward(logits, tokens, mask, stats, glp.float().contiguous(), None, 0, grad, ctx.strides)
-        return grad, None, None
+        return grad[0], None, None
 
 
 def _class_backward(logits, tokens, mask, stats, coef, gout, done_if_one, grad, strides):
@@ -1239,9 +1240,10 @@ def _class_backward(logits, tokens, mask, stats, coef, gout, done_if_one, grad, 
     b, t, v = logits.shape
     if b * t == 0:
         return
+    g, gb, gt = grad
     _launch("pp_token_log_probs_bwd", logits.device, _at(logits), strides[0], strides[1],
             _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(stats), _at(coef), _at(gout),
-            done_if_one, _at(grad), b, t, v)
+            done_if_one, _at(g), gb, gt, b, t, v)
 
 
 def token_log_probs(logits, tokens, mask=None):
@@ -1268,22 +1270,23 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         logits, lb, lt = _class_rows(logits)
         out = torch.empty(3, device=logits.device, dtype=torch.float32)
         stats = coef = grad = None
+        gb = gt = 0
         if ctx.needs_input_grad[0]:
             stats = torch.empty(b, t, 2, device=logits.device)
             coef = torch.empty(b, t, device=logits.device)
-            grad = _class_grad(logits, lb, lt)
+            grad, gb, gt = _class_grad(logits, lb, lt)
         if b * t:
             nbytes = lib.pp_clipped_policy_loss_workspace_bytes(b, t)
             ws = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
             _launch("pp_clipped_policy_loss_fwd", logits.device, _at(logits), lb, lt,
                     _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(old), _at(adv), adv.stride(0),
                     adv.stride(1), _at(ref), low, high, beta, by_sequence, _at(out), _at(stats),
-                    _at(coef), _at(grad), _at(ws), nbytes, b, t, v)
+                    _at(coef), _at(grad), gb, gt, _at(ws), nbytes, b, t, v)
         else:
             out.zero_()
         if grad is not None:
             ctx.save_for_backward(logits, tokens, mask, stats, coef)
-            ctx.grad, ctx.strides = grad, (lb, lt)
+            ctx.grad, ctx.strides = (grad, gb, gt), (lb, lt)
         loss, kl, clipped = out[0], out[1], out[2]
         ctx.mark_non_differentiable(kl, clipped)
         return loss, kl, clipped
@@ -1298,7 +1301,7 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
             grad = _class_grad(logits, *ctx.strides)
         gout = gloss.reshape(1).to(torch.float32).contiguous()
         _class_backward(logits, tokens, mask, stats, coef, gout, done, grad, ctx.strides)
-        return (grad,) + (None,) * 9
+        return (grad[0],) + (None,) * 9
 
 
 def clipped_policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, mask=None,

@@ -168,7 +168,11 @@ def test_slices_and_padded_vocabularies(v, dtype):
     wide[:, 1:7, 3:v + 3] = logits.cuda()
     got = _loss(wide[:, 1:7, 3:v + 3], *rest)
     _compare(got, want)
-    assert got["grad"].stride() == wide[:, 1:7, 3:v + 3].stride()
+    # rows at the offsets of the logits' rows within 16 bytes, and no more memory than that takes
+    vec = 16 // logits.element_size()
+    assert got["grad"].data_ptr() % 16 == wide[:, 1:7, 3:].data_ptr() % 16
+    assert (got["grad"].stride(1) - wide.stride(1)) % vec == 0
+    assert got["grad"].untyped_storage().nbytes() <= (3 * (6 * (v + vec) + vec) + vec) * logits.element_size()
     turned = logits.cuda().transpose(0, 1).contiguous().transpose(0, 1)
     _compare(_loss(turned, *rest), want)
     classes_first = logits.cuda().permute(2, 0, 1).contiguous().permute(1, 2, 0)
@@ -182,6 +186,10 @@ def test_slices_and_padded_vocabularies(v, dtype):
     loss.backward()
     so.check(whole.grad[:, :6], want["grad"], "whole")
     assert bool((whole.grad[:, 6] == 0).all())
+    # the last position of every sequence only
+    last = _loss(wide[:, 6:7, 3:v + 3], *(x[:, 5:] for x in rest))
+    _compare(last, _want(logits[:, 5:], *(x[:, 5:] for x in rest)))
+    assert last["grad"].untyped_storage().nbytes() <= (3 * (v + 2 * vec) + vec) * logits.element_size()
     # one row of logits for all tokens
     one = logits[:1, :1].cuda().expand(3, 6, v)
     shared = logits[:1, :1].expand(3, 6, v)

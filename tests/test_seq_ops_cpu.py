@@ -30,6 +30,8 @@ def test_recurrence_entry_refuses():
     assert _rec(z=BAD) == E_ALIGN and _rec(f=ODD, dtype=1) == E_ALIGN
     assert _rec(h0=BAD) == E_ALIGN and _rec(starts=BAD) == E_ALIGN
     assert _rec(l=2 ** 31 - 1) == E_RANGE
+    assert _rec(b=65535, l=32767, d=1) == E_RANGE  # more than 2^32 threads
+    assert lib.pp_gated_recurrence_step(OK, 8, OK, 8, 0, OK, 1 << 20, OK, 65535, 1 << 20, NULL) == E_RANGE
     assert lib.pp_gated_recurrence_step(OK, 8, OK, 8, 0, OK, 7, OK, 2, 8, NULL) == E_SHAPE
     assert lib.pp_gated_recurrence_step(OK, 8, OK, 8, 0, NULL, 8, OK, 2, 8, NULL) == E_NULL
     assert lib.pp_gated_recurrence_bwd(OK, 8, 8, OK, 8, 8, 0, NULL, NULL, NULL, OK, 8, 8, NULL, OK, OK, NULL, NULL, 0,
@@ -42,25 +44,31 @@ def test_recurrence_entry_refuses():
                                            100000, 64, NULL) == E_WS
 
 
-def _pol(logits=OK, tokens=OK, old=OK, adv=OK, out=OK, stats=NULL, coef=NULL, grad=NULL, ws=OK, nbytes=1 << 20,
-         dtype=0, low=0.2, high=0.2, b=2, t=3, v=8):
+def _pol(logits=OK, tokens=OK, old=OK, adv=OK, out=OK, stats=NULL, coef=NULL, grad=NULL, gb=None, gt=None, ws=OK,
+         nbytes=1 << 20, dtype=0, low=0.2, high=0.2, b=2, t=3, v=8):
     return _lib.load().pp_clipped_policy_loss_fwd(logits, t * v, v, dtype, tokens, NULL, old, adv, t, 1, NULL, low, high,
-                                                  0.0, 0, out, stats, coef, grad, ws, nbytes, b, t, v, NULL)
+                                                  0.0, 0, out, stats, coef, grad, t * v if gb is None else gb,
+                                                  v if gt is None else gt, ws, nbytes, b, t, v, NULL)
 
 
 def test_policy_entry_refuses():
     lib = _lib.load()
-    for kw in (dict(logits=NULL), dict(tokens=NULL), dict(old=NULL), dict(adv=NULL), dict(out=NULL), dict(stats=OK)):
+    for kw in (dict(logits=NULL), dict(tokens=NULL), dict(old=NULL), dict(adv=NULL), dict(out=NULL), dict(grad=OK),
+               dict(grad=OK, stats=OK), dict(grad=OK, coef=OK)):
         assert _pol(**kw) == E_NULL
     for kw in (dict(b=0), dict(t=0), dict(v=0), dict(low=-0.1), dict(high=float("nan"))):
         assert _pol(**kw) == E_SHAPE
     assert _pol(dtype=7) == E_METHOD
-    assert _pol(logits=BAD) == E_ALIGN and _pol(grad=ctypes.c_void_p(4104)) == E_ALIGN  # another offset in 16 bytes
+    assert _pol(logits=BAD) == E_ALIGN
+    full = dict(grad=OK, stats=OK, coef=OK)
+    assert _pol(**dict(full, grad=ctypes.c_void_p(4104))) == E_ALIGN  # another offset in 16 bytes
+    assert _pol(**full, gt=9, gb=28) == E_ALIGN and _pol(**full, gb=26) == E_ALIGN
+    assert _pol(**full, gt=4) == E_SHAPE and _pol(**full, gb=20) == E_SHAPE  # rows that overlap
     assert _pol(ws=NULL) == E_WS and _pol(nbytes=8) == E_WS
     assert _pol(b=1 << 20, t=1 << 20) == E_RANGE
     assert lib.pp_token_log_probs_fwd(OK, 8, 8, 0, OK, NULL, NULL, NULL, 1, 1, 8, NULL) == E_NULL
     assert lib.pp_token_log_probs_fwd(OK, 8, 8, 0, ctypes.c_void_p(4100), NULL, OK, NULL, 1, 1, 8, NULL) == E_ALIGN
-    assert lib.pp_token_log_probs_bwd(OK, 8, 8, 0, OK, NULL, NULL, OK, NULL, 0, OK, 1, 1, 8, NULL) == E_NULL
+    assert lib.pp_token_log_probs_bwd(OK, 8, 8, 0, OK, NULL, NULL, OK, NULL, 0, OK, 8, 8, 1, 1, 8, NULL) == E_NULL
 
 
 def _adam(count=1, dtype=0, bits=32, p=4096, g=4096, m=4096, v=4096, w=None, e=None, n=8, step=1, b1=0.9, b2=0.99):
@@ -79,6 +87,7 @@ def test_adamw_entry_refuses():
     assert _adam(p=0) == E_NULL and _adam(dtype=1) == E_NULL and _adam(bits=8) == E_NULL
     assert _adam(n=0) == E_SHAPE and _adam(step=0) == E_SHAPE and _adam(b1=1.0) == E_SHAPE and _adam(b2=-0.1) == E_SHAPE
     assert _adam(b1=float("nan")) == E_SHAPE
+    assert _adam(n=1 << 40) == E_RANGE and _adam(n=1 << 34) == E_RANGE
     assert _adam(g=4098) == E_ALIGN and _adam(dtype=2, w=4096, p=4097) == E_ALIGN
     two = (ctypes.c_void_p * 2)(4096, 4096)
     assert lib.pp_count_step(2, two, None) == E_SHAPE  # the same counter twice
