@@ -5,8 +5,10 @@
 //   loss = sum_t w_t term_t,  w = mask / #tokens  or  mask / (#tokens of the sequence * #sequences)
 //   dloss/dlogits = c (onehot(token) - softmax),  c = w (-A rho [not clipped] + beta (1 - exp(ref - lp)))
 //
-// Row statistics are kept as (max, log of the sum of exp(x - max)) in fp32: lp = (x - max) - log sum
-// is a difference of small numbers, where x - logsumexp would lose the digits of a large max.
+// The sum of exp(x - max) is taken in fp32 a lane and in 64 bits over the lanes; lp = (x - max) - log sum
+// and its differences to old and ref are formed in 64 bits (a few operations a row: the log is that of the
+// mantissa in fp32, and the exponent times log 2), since a ratio is the exponential of a small difference of
+// numbers around -10, whose fp32 spacing alone would be 1e-6 of it.  The backward keeps (max, log sum) in fp32.
 // A masked token's logits, token, old, ref and advantage are not read; its gradient row is zeros.
 //
 // Bound: the logits are read once and the gradient written once.  A row that fits is therefore held
@@ -77,38 +79,61 @@ __device__ __forceinline__ float row_max(float v, float* red) {
   return v;
 }
 template <int THREADS>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-  v = pp_wave_sum(v);
+__device__ __forceinline__ double row_sum(float v, double* red) {
+  v = pp_dpp_add<0x128>(v);
+  v = pp_dpp_add<0x124>(v);
+  v = pp_dpp_add<0x122>(v);
+  v = pp_dpp_add<0x121>(v);
+  double s = ((double)pp_readlane_f(v, 0) + (double)pp_readlane_f(v, 16)) +
+             ((double)pp_readlane_f(v, 32) + (double)pp_readlane_f(v, 48));
   if (THREADS > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int i = 1; i < THREADS / 64; ++i) v += red[i];
+    s = 0.0;
+    // (not all at once: that takes 32 registers beside the row)
+#pragma unroll 4
+    for (int i = 0; i < THREADS / 64; ++i) s += red[i];
     __syncthreads();
   }
-  return v;
+  return s;
 }
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
+// log of a sum: exponent and mantissa apart
+__device__ __forceinline__ double log_of(double sum) {
+  const float f = (float)sum;
+  const float low = (float)((sum - (double)f) / sum);  // what fp32 rounds off (NaN for 0 and infinity)
+  const double l = (double)__builtin_amdgcn_frexp_expf(f) * 0.69314718055994531 +
+                   (double)logf(__builtin_amdgcn_frexp_mantf(f));
+  return low == low ? l + (double)low : l;
+}
+
+// A row's max and the log of the sum of exp(x - max).
+struct RowStats {
+  float max;
+  double log_sum;
+  __device__ __forceinline__ float2 kept() const { return make_float2(max, (float)log_sum); }
+  __device__ __forceinline__ double lp(float x) const { return ((double)x - (double)max) - log_sum; }
+};
+
+// The token's logit; NaN where there is no such class: the loss says so.
 template <typename T>
-__device__ __forceinline__ float token_lp(const T* __restrict__ x, int64_t token, int v, float2 st) {
-  if (token < 0 || token >= v) return __uint_as_float(0x7fc00000u);  // no such class: the loss says so
-  return ((float)x[token] - st.x) - st.y;
+__device__ __forceinline__ float token_logit(const T* __restrict__ x, int64_t token, int v) {
+  return token >= 0 && token < v ? (float)x[token] : __uint_as_float(0x7fc00000u);
 }
 
 // The terms of one token; returns the gradient's coefficient.
-__device__ __forceinline__ float policy_terms(const PolArgs& p, const PolTerms& q, int row, float lp,
+__device__ __forceinline__ float policy_terms(const PolArgs& p, const PolTerms& q, int row, double lp,
                                               bool writer) {
   const int b = row / p.t, t = row % p.t;
   const float w = q.weight ? q.weight[b] : q.every, adv = q.adv[b * q.ab + t * q.at];
-  const float rho = expf(lp - q.old[row]);
+  const float rho = expf((float)(lp - (double)q.old[row]));
   const float border = adv >= 0.0f ? 1.0f + q.high : 1.0f - q.low;
   const bool clipped = adv >= 0.0f ? rho > border : rho < border;
   float loss = -(clipped ? border : rho) * adv, c = clipped ? 0.0f : -adv * rho, kl = 0.0f;
   if (q.ref) {
-    const float delta = q.ref[row] - lp, grow = expm1f(delta);
+    const float delta = (float)((double)q.ref[row] - lp), grow = expm1f(delta);
     kl = grow - delta;
     loss += q.beta * kl;
     c -= q.beta * grow;
@@ -136,7 +161,7 @@ __device__ __forceinline__ void zero_row(T* __restrict__ g, int v, int tid) {
 // The statistics of a row by one pass over it: every lane keeps a running max and the sum relative to
 // it, kAhead vectors in flight.
 template <typename T, int THREADS>
-__device__ __forceinline__ float2 stream_stats(const T* __restrict__ x, int v, int tid, float* red) {
+__device__ __forceinline__ RowStats stream_stats(const T* __restrict__ x, int v, int tid, double* red) {
   constexpr int kVec = Span<T>::kVec, kAhead = 4;
   typedef PPElems<T, kVec> E;
   const Span<T> s(x, v);
@@ -173,9 +198,8 @@ __device__ __forceinline__ float2 stream_stats(const T* __restrict__ x, int v, i
     sum = sum * exp_of(m - top) + exp_of(e - top);
     m = top;
   }
-  const float top = row_max<THREADS>(m, red);
-  sum = row_sum<THREADS>(sum * exp_of(m - top), red);
-  return make_float2(top, logf(sum));
+  const float top = row_max<THREADS>(m, reinterpret_cast<float*>(red));
+  return {top, log_of(row_sum<THREADS>(sum * exp_of(m - top), red))};
 }
 
 // stats and lp, or stats, terms and coef, of each row.  THREADS lanes a row, 256 a workgroup.
@@ -183,7 +207,7 @@ template <typename T, int THREADS, bool POLICY>
 __global__ __launch_bounds__(256) void pp_row_terms_kernel(const T* __restrict__ logits, PolArgs p,
                                                            PolTerms q, float2* __restrict__ stats,
                                                            float* __restrict__ out) {
-  __shared__ float red[4];
+  __shared__ double red[4];
   const int tid = threadIdx.x % THREADS;
   const int row = p.first + blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
   if (row >= p.rows) return;
@@ -196,15 +220,15 @@ __global__ __launch_bounds__(256) void pp_row_terms_kernel(const T* __restrict__
     return;
   }
   const T* x = logits + p.logits_at(row);
-  const float2 st = stream_stats<T, THREADS>(x, p.v, tid, red);
+  const RowStats st = stream_stats<T, THREADS>(x, p.v, tid, red);
   if (tid == 0) {
-    const float lp = token_lp(x, p.tokens[row], p.v, st);
-    if (stats) stats[row] = st;
+    const double lp = st.lp(token_logit(x, p.tokens[row], p.v));
+    if (stats) stats[row] = st.kept();
     if (POLICY) {
       const float c = policy_terms(p, q, row, lp, true);
       if (out) out[row] = c;
     } else {
-      out[row] = lp;
+      out[row] = (float)lp;
     }
   }
 }
@@ -284,12 +308,12 @@ __device__ __forceinline__ void keep_raw(R (&r)[NV]) {
 
 // Statistics, terms and gradient of a row that NV vectors a thread hold.
 template <typename T, int THREADS, int NV>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pp_policy_fused_kernel(
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, NV <= 8 ? 8 : 4) void pp_policy_fused_kernel(
     const T* __restrict__ logits, PolArgs p, PolTerms q, float2* __restrict__ stats,
     float* __restrict__ coef, T* __restrict__ grad) {
   constexpr int kVec = Span<T>::kVec, kRows = THREADS < 256 ? 256 / THREADS : 1;
   typedef PPElems<T, kVec> E;
-  __shared__ float red[THREADS / 64 > 4 ? THREADS / 64 : 4];
+  __shared__ double red[THREADS / 64 > 4 ? THREADS / 64 : 4];
   const int tid = threadIdx.x % THREADS;
   const int row = p.first + blockIdx.x * kRows + threadIdx.x / THREADS;
   if (row >= p.rows) return;
@@ -315,7 +339,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pp_policy_fused
   float edge = -INFINITY;
   if (tid < s.edge) edge = (float)x[s.edge_at(tid)];
   const int64_t tok = p.tokens[row];
-  const float xt = tok >= 0 && tok < p.v ? (float)x[tok] : __uint_as_float(0x7fc00000u);
+  const float xt = token_logit(x, tok, p.v);
   float m = edge;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -327,7 +351,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pp_policy_fused
     }
   }
   keep_raw(r);
-  m = row_max<THREADS>(m, red);
+  m = row_max<THREADS>(m, reinterpret_cast<float*>(red));
   float sum = tid < s.edge ? exp_of(edge - m) : 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -339,14 +363,14 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void pp_policy_fused
     }
   }
   keep_raw(r);
-  sum = row_sum<THREADS>(sum, red);
-  const float2 st = make_float2(m, logf(sum));
-  const float c = policy_terms(p, q, row, (xt - st.x) - st.y, tid == 0);
+  const double total = row_sum<THREADS>(sum, red);
+  const RowStats st = {m, log_of(total)};
+  const float c = policy_terms(p, q, row, st.lp(xt), tid == 0);
   if (tid == 0) {
-    stats[row] = st;
+    stats[row] = st.kept();
     coef[row] = c;
   }
-  const float k = -c / sum;
+  const float k = -c / (float)total;
   const int token = tok >= 0 && tok < p.v ? (int)tok : -1 - kVec;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
