@@ -17,6 +17,12 @@
 // remainder stands for keeps the expected value exact.  The bits come from a hash of (seed, step,
 // tensor, entry), so a step can be repeated.  A positive v never becomes zero: the step m / eps that
 // would follow is unbounded.
+//
+// Bound: HBM.  Everything is read and written once, in 16-byte accesses (4 bytes of codes) that pass the caches
+// by: nothing is used again before the next step, and 92 M fp32 weights take 432 us (6.0 TB/s) that way, 478
+// through the caches.  Codes stay in the caches (8-bit step of 226 M bf16 weights and a decode 930 us, 994 past
+// them).  A thread takes four entries at a time, a workgroup 1024 or, with the longer 8-bit arithmetic, 2048
+// (bf16 / 8 bits 624 us, 5.8 TB/s, 674 with 1024; fp32 / 32 bits 432 with 1024, 460 with 2048).
 #include <algorithm>
 #include <cmath>
 

@@ -28,6 +28,12 @@
 //   A reset makes P = -0.0, which no product of gates is: it cuts even a state that is NaN.
 // The forward of a training step keeps h at the start of every kSteps steps in fp32 (the states in
 // between are recomputed from it; y, rounded to 16 bits, would not do for the differences).
+//
+// Bound: forward 3 and backward 5 values an entry through HBM, each once.  Measured (MI355X, bf16):
+// [8, 2048, 2048] forward 53 us (4.0 TB/s with the kept states), backward 75 us (4.6); [1, 100003, 640] 106
+// and 148 us.  The rest is the shape of a workgroup: 16 waves of 112 registers are all that a CU holds, so
+// its loads, its walks (half of the time is instruction issue) and its waits follow one another; counter and
+// look-back are 5 to 15 % (measured without them).
 #include <algorithm>
 
 #include "pp_device.h"

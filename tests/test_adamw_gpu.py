@@ -172,6 +172,8 @@ def test_decoded_moments():
         want = so.decode(codes.numpy(), exps.numpy(), top, signed)
         got = PF.decode_moment(codes.cuda(), exps.cuda(), signed)
         assert _same(got, want)
+        odd = torch.empty(10009, dtype=torch.uint8, device="cuda")[3:10004].copy_(codes)  # no multiple of 8
+        assert _same(PF.decode_moment(odd, exps.cuda(), signed), want)
         for dt in (BF16, F16):
             assert torch.equal(PF.decode_moment(codes.cuda(), exps.cuda(), signed, dt).cpu().nan_to_num(7.0),
                                torch.from_numpy(want).to(dt).nan_to_num(7.0))

@@ -1,6 +1,9 @@
 """Sequence-model operators without a GPU: refusals of the C entries and of the Python ones, and the
 restatements the GPU tests compare with."""
 import ctypes
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -202,3 +205,16 @@ def test_codes_are_unbiased_and_ordered():
     counts = np.bincount(bits, minlength=256)
     # 2^19 draws in 256 bins: mean 2048, deviation 45
     assert counts.min() > 2048 - 6 * 45 and counts.max() < 2048 + 6 * 45
+
+
+def test_no_packed_fp32_instruction_in_the_sequence_operators(tmp_path):
+    """Some packed-fp32 forms have given wrong results on this chip; the units are compiled without."""
+    csrc = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc")
+    subprocess.run(["make", "-C", csrc, "asm-seq", f"ASMDIR={tmp_path}", "-j", "3"], check=True,
+                   stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
+    for unit in ("pp_recurrence", "pp_policy", "pp_adamw"):
+        text = (tmp_path / f"{unit}.s").read_text()
+        assert text.count(".amdhsa_kernel") >= 4
+        assert not re.findall(r"v_pk_(?:mul|add|fma)_f32", text), unit
+        # nothing spills: a row, or a stretch, is held in registers by design
+        assert not re.findall(r"\.vgpr_spill_count:\s+[1-9]", text), unit
