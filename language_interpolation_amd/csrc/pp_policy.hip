@@ -323,14 +323,14 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, NV <= 8 ? 8 : 4) voi
   const int row = p.first + blockIdx.x * kRows + threadIdx.x / THREADS;
   if (row >= p.rows) return;
   const T* x = logits + p.logits_at(row);
-  T* g = grad + p.grad_at(row);
+  T* g = grad ? grad + p.grad_at(row) : nullptr;
   if (p.mask && !p.mask[row]) {
     if (tid == 0) {
-      stats[row] = make_float2(0.0f, 0.0f);
-      coef[row] = 0.0f;
+      if (stats) stats[row] = make_float2(0.0f, 0.0f);
+      if (coef) coef[row] = 0.0f;
       no_terms(q, row);
     }
-    zero_row<T, THREADS>(g, p.v, tid);
+    if (g) zero_row<T, THREADS>(g, p.v, tid);
     return;
   }
   const Span<T> s(x, p.v);
@@ -372,9 +372,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, NV <= 8 ? 8 : 4) voi
   const RowStats st = {m, log_of(total)};
   const float c = policy_terms(p, q, row, st.lp(xt), tid == 0);
   if (tid == 0) {
-    stats[row] = st.kept();
-    coef[row] = c;
+    if (stats) stats[row] = st.kept();
+    if (coef) coef[row] = c;
   }
+  if (!g) return;
   const float k = -c / (float)total;
   const int token = tok >= 0 && tok < p.v ? (int)tok : -1 - kVec;
 #pragma unroll
@@ -498,15 +499,16 @@ bool try_fused(const T* logits, const PolArgs& all, const PolTerms& q, float2* s
 template <typename T>
 void run_policy(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* coef, T* grad,
                 hipStream_t st) {
-  if (grad && (try_fused<T, 64, 1>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 64, 2>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 64, 4>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 256, 2>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 256, 4>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 256, 8>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 1024, 4>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 1024, 8>(logits, p, q, stats, coef, grad, st) ||
-               try_fused<T, 1024, 16>(logits, p, q, stats, coef, grad, st)))
+  // (without a gradient too: the loss has the same bits whether one follows or not)
+  if (try_fused<T, 64, 1>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 64, 2>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 64, 4>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 256, 2>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 256, 4>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 256, 8>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 1024, 4>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 1024, 8>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 1024, 16>(logits, p, q, stats, coef, grad, st))
     return;
   run_terms<T, true>(logits, p, q, stats, coef, st);
   if (grad) run_grad<T>(logits, p, stats, coef, nullptr, 0, grad, st);

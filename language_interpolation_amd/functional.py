@@ -1072,6 +1072,11 @@ def _bytes_of(mask: Optional[torch.Tensor]):
     return None if mask is None else mask.contiguous().view(torch.uint8)
 
 
+def _graded(*tensors) -> bool:
+    """A backward may follow.  (A Function's needs_input_grad is also set under no_grad.)"""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
@@ -1081,7 +1086,7 @@ class GatedRecurrenceFunction(torch.autograd.Function):
     PP_RECURRENCE_STEPS steps, the backward recomputes the states in between."""
 
     @staticmethod
-    def forward(ctx, z, f, h0, lengths, reset):
+    def forward(ctx, z, f, h0, lengths, reset, graded):
         lib = _lib.load()
         ctx.set_materialize_grads(False)
         z, f = _last_contiguous(z), _last_contiguous(f)
@@ -1093,14 +1098,14 @@ class GatedRecurrenceFunction(torch.autograd.Function):
             h = torch.zeros(b, d, device=z.device) if h0 is None else h0.clone()
         else:
             h = torch.empty(b, d, device=z.device, dtype=torch.float32)
-            if any(ctx.needs_input_grad):
+            if graded:
                 starts = torch.empty(b, lib.pp_gated_recurrence_starts(l), d, device=z.device)
             nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
             ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
             _launch("pp_gated_recurrence_fwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
                     f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(h0), _at(lengths), _at(reset),
                     _at(y), _at(h), _at(starts), _at(ws), nbytes, b, l, d)
-        if any(ctx.needs_input_grad):
+        if graded:
             ctx.save_for_backward(z, f, starts, lengths, reset)
         return y, h
 
@@ -1114,7 +1119,7 @@ class GatedRecurrenceFunction(torch.autograd.Function):
         gf = torch.empty_like(gz)
         gh = None if gh is None else gh.contiguous()
         if z.numel() == 0:
-            return gz, gf, gh if ctx.needs_input_grad[2] else None, None, None
+            return gz, gf, gh if ctx.needs_input_grad[2] else None, None, None, None
         gy = torch.zeros_like(gz) if gy is None else _last_contiguous(gy)
         gh0 = torch.empty(b, d, device=z.device) if ctx.needs_input_grad[2] else None
         nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
@@ -1123,7 +1128,7 @@ class GatedRecurrenceFunction(torch.autograd.Function):
                 f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(lengths), _at(reset), _at(starts),
                 _at(gy), gy.stride(0), gy.stride(1), _at(gh), _at(gz), _at(gf), _at(gh0), _at(ws),
                 nbytes, b, l, d)
-        return gz, gf, gh0, None, None
+        return gz, gf, gh0, None, None, None
 
 
 def gated_recurrence(z, f, h0=None, lengths=None, reset=None):
@@ -1150,7 +1155,7 @@ def gated_recurrence(z, f, h0=None, lengths=None, reset=None):
     if reset is not None:
         _require_aux(reset, "reset", (b, l), (torch.bool, torch.uint8), z.device)
         reset = _bytes_of(reset)
-    return GatedRecurrenceFunction.apply(z, f, h0, lengths, reset)
+    return GatedRecurrenceFunction.apply(z, f, h0, lengths, reset, _graded(z, f, h0))
 
 
 def gated_recurrence_step(z, f, h):
@@ -1213,11 +1218,11 @@ def _check_classes(logits, tokens, mask):
 
 class TokenLogProbsFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, mask):
+    def forward(ctx, logits, tokens, mask, graded):
         b, t, v = logits.shape
         logits, lb, lt = _class_rows(logits)
         lp = torch.empty(b, t, device=logits.device, dtype=torch.float32)
-        stats = torch.empty(b, t, 2, device=logits.device) if ctx.needs_input_grad[0] else None
+        stats = torch.empty(b, t, 2, device=logits.device) if graded else None
         if lp.numel():
             _launch("pp_token_log_probs_fwd", logits.device, _at(logits), lb, lt,
                     _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(lp), _at(stats), b, t, v)
@@ -1232,7 +1237,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
         logits, tokens, mask, stats = ctx.saved_tensors
         grad = _class_grad(logits, *ctx.strides)
         _class_backward(logits, tokens, mask, stats, glp.float().contiguous(), None, 0, grad, ctx.strides)
-        return grad[0], None, None
+        return grad[0], None, None, None
 
 
 def _class_backward(logits, tokens, mask, stats, coef, gout, done_if_one, grad, strides):
@@ -1254,7 +1259,7 @@ def token_log_probs(logits, tokens, mask=None):
     if isinstance(logits, torch.Tensor) and logits.dim() == 2:
         return token_log_probs(logits[None], tokens[None], None if mask is None else mask[None])[0]
     tokens, mask = _check_classes(logits, tokens, mask)
-    return TokenLogProbsFunction.apply(logits, tokens, mask)
+    return TokenLogProbsFunction.apply(logits, tokens, mask, _graded(logits))
 
 
 class ClippedPolicyLossFunction(torch.autograd.Function):
@@ -1264,14 +1269,14 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     handed out before, computes it again from the logits."""
 
     @staticmethod
-    def forward(ctx, logits, tokens, mask, old, adv, ref, low, high, beta, by_sequence):
+    def forward(ctx, logits, tokens, mask, old, adv, ref, low, high, beta, by_sequence, graded):
         lib = _lib.load()
         b, t, v = logits.shape
         logits, lb, lt = _class_rows(logits)
         out = torch.empty(3, device=logits.device, dtype=torch.float32)
         stats = coef = grad = None
         gb = gt = 0
-        if ctx.needs_input_grad[0]:
+        if graded:
             stats = torch.empty(b, t, 2, device=logits.device)
             coef = torch.empty(b, t, device=logits.device)
             grad, gb, gt = _class_grad(logits, lb, lt)
@@ -1301,7 +1306,7 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
             grad = _class_grad(logits, *ctx.strides)
         gout = gloss.reshape(1).to(torch.float32).contiguous()
         _class_backward(logits, tokens, mask, stats, coef, gout, done, grad, ctx.strides)
-        return (grad[0],) + (None,) * 9
+        return (grad[0],) + (None,) * 10
 
 
 def clipped_policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, mask=None,
@@ -1337,7 +1342,7 @@ def clipped_policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, mas
         ref_logp = ref_logp.detach().contiguous()
     return ClippedPolicyLossFunction.apply(
         logits, tokens, mask, old_logp.detach().contiguous(), advantages.detach(), ref_logp,
-        float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"))
+        float(clip_low), float(clip_high), float(kl_coef), int(reduction == "sequence"), _graded(logits))
 
 
 def dense_storage(t: torch.Tensor) -> bool:
@@ -1456,8 +1461,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
             for name in ("params", "grads", "masters", "exp_avgs", "exp_avg_sqs", "avg_exponents", "sq_exponents"))
         _launch("pp_adamw_step", device, k, _ELEMENT[dtype], 8 if eight else 32, p, g, w, m, v, me, ve,
                 numbers(*[sizes[i] for i in part]), None if counted else numbers(*[steps[i] for i in part]),
-                pointers(*[steps[i].data_ptr() for i in part]) if counted else None, lr, b1, b2, eps,
-                weight_decay, _at(grad_scale), seed & 0xFFFFFFFF, lo)
+                pointers(*[steps[i].data_ptr() for i in part]) if counted else None, float(lr), b1, b2, float(eps),
+                float(weight_decay), _at(grad_scale), seed & 0xFFFFFFFF, lo)
     # written through raw pointers: tell autograd and the pre-split weight cache
     for name, x in lists.items():
         if name != "grads":

@@ -283,7 +283,9 @@ class AdamW(torch.optim.Optimizer):
     moment_bits=8 keeps both moments in one byte an entry (tensors under MIN_8BIT entries stay in 32
     bits: they are most of the tensors and none of the memory); `seed` is that of their rounding.
     capturable: the step numbers are device counters, so that a captured step counts its replays.
-    step(grad_scale=t): gradients are multiplied by the device scalar t first."""
+    step(grad_scale=t): gradients are multiplied by the device scalar t first.
+    16-bit weights follow their masters: who sets them from outside after the first step sets
+    state[p]["master"] too.  State dicts of torch.optim.Adam and AdamW can be loaded."""
 
     MIN_8BIT = 4096
 
@@ -331,11 +333,16 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if g.is_sparse:
                     raise RuntimeError("AdamW: sparse gradients are not supported")
-                st = self.state[p] or self._init_state(p, group)
+                st = self.state[p]
+                if not st:
+                    if group["capturable"] and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: take a step before the capture (the graph would set the "
+                                           "state to zero with every replay)")
+                    st = self._init_state(p, group)
                 if not group["capturable"]:
                     st["step"] += 1
-                if g.stride() != p.stride():  # one order for all that belongs to a parameter
-                    g = torch.empty_like(p).copy_(g)
+                if g.stride() != p.stride() and not (g.is_contiguous() and p.is_contiguous()):
+                    g = torch.empty_like(p).copy_(g)  # one order for all that belongs to a parameter
                 kinds.setdefault((p.device, p.dtype, "exp_avg_exponent" in st), []).append((p, g, st))
             for k, ((_, dtype, eight), todo) in enumerate(kinds.items()):
                 PF.adamw_step(
@@ -354,22 +361,26 @@ class AdamW(torch.optim.Optimizer):
         moments and masters to the parameter's) and its own order of the entries."""
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        mine = [(p, g) for g in self.param_groups for p in g["params"]]
+        mine = []
+        for group in self.param_groups:
+            for name, value in self.defaults.items():  # a torch.optim group has no moment_bits and seed
+                group.setdefault(name, value)
+            mine += [(p, group) for p in group["params"]]
         for i, (p, group) in zip(saved, mine):
             old = state_dict["state"].get(i)
             if not old:
                 continue
-            st = {}
-            for name, x in old.items():
-                if name == "step":
-                    x = int(x)
-                    st[name] = torch.tensor(x, device=p.device) if group["capturable"] else x
-                elif x.shape == p.shape and not name.endswith("_exponent"):
-                    if x.dtype == torch.uint8 and x.stride() != p.stride():
+            step = int(old["step"])
+            st = {"step": torch.tensor(step, device=p.device) if group["capturable"] else step}
+            for name in ("exp_avg", "exp_avg_sq"):
+                x = old[name]
+                if x.dtype == torch.uint8:
+                    if x.stride() != p.stride():
                         raise ValueError("AdamW: 8-bit moments belong to another order of the entries")
-                    st[name] = torch.empty_like(p, dtype=x.dtype).copy_(x)
-                else:
-                    st[name] = x.to(p.device, copy=True)
+                    st[name + "_exponent"] = old[name + "_exponent"].to(p.device, copy=True)
+                st[name] = torch.empty_like(p, dtype=torch.uint8 if x.dtype == torch.uint8 else torch.float32).copy_(x)
+            if p.dtype != torch.float32:
+                st["master"] = torch.empty_like(p, dtype=torch.float32).copy_(old.get("master", p))
             self.state[p] = st
 
 

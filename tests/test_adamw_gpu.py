@@ -268,6 +268,30 @@ def test_optimizer_keeps_its_types_through_a_checkpoint(dtype, tmp_path):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_checkpoint_of_torch_goes_on(dtype):
+    """Moments of torch.optim.AdamW (there in the weights' type), then a step here and there in 64 bits."""
+    from language_interpolation_amd.train import AdamW
+    gen = torch.Generator().manual_seed(7)
+    base = torch.randn(60, 30, generator=gen).to(dtype)
+    grads = [torch.randn(60, 30, generator=gen).to(dtype) for _ in range(3)]
+    p = base.clone().cuda().requires_grad_()
+    opt = torch.optim.AdamW([p], lr=1e-2)
+    for g in grads[:2]:
+        p.grad = g.cuda()
+        opt.step()
+    state = opt.state_dict()
+    mine = AdamW([p], lr=1.0)
+    mine.load_state_dict(state)
+    st = mine.state[p]
+    w, m, v = (x.detach().float().cpu().numpy().ravel() for x in (p, st["exp_avg"], st["exp_avg_sq"]))
+    assert st["step"] == 2 and st["exp_avg"].dtype == F32 and ("master" in st) == (dtype != F32)
+    p.grad = grads[2].cuda()
+    mine.step()
+    want = so.adamw(w, grads[2].float().numpy().ravel(), m, v, 3, 1e-2, (0.9, 0.999), 1e-8, 1e-2)[0]
+    assert _same(p.detach().float().view(-1), torch.from_numpy(want).to(dtype).float().numpy())
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_captured_step(dtype, bits):
@@ -299,6 +323,10 @@ def test_captured_step(dtype, bits):
     with pytest.raises(RuntimeError, match="capturable"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             eager.step()
+    fresh = AdamW(ps[1], lr=1e-2, moment_bits=bits, capturable=True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fresh.step()
 
 
 def test_side_stream():

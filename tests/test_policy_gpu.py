@@ -214,6 +214,19 @@ def test_repeated_backward_and_loss_scale():
         assert all(torch.equal(p, first[k]) for p, k in zip(plain, ("loss", "kl", "clipped")))
 
 
+def test_no_gradient_is_made_where_none_can_follow():
+    from language_interpolation_amd import functional as PF
+    s = _inputs(4, 64, 20000, BF16, seed=36)
+    x = s[0].cuda().requires_grad_()
+    rest = [t.cuda() for t in s[1:5]]
+    with torch.no_grad():
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        PF.clipped_policy_loss(x, *rest, mask=s[5].cuda(), kl_coef=BETA)
+        assert torch.cuda.max_memory_allocated() - before < x.numel()  # bytes: half of a gradient
+
+
 def test_changed_logits_are_noticed():
     """The backward may need the logits again: changed in place, it refuses."""
     from language_interpolation_amd import functional as PF
