@@ -442,12 +442,14 @@ __global__ __launch_bounds__(1024) void pp_policy_finish_kernel(const float* __r
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
+#pragma unroll
     for (int i = 1; i < 16; ++i) s += red[i];
     out[blockIdx.x] = (float)s;
   }
 }
 
-constexpr int kWaveRow = 4096;  // bytes up to which a row is one wave's
+constexpr int kWaveRow = 4096;     // bytes up to which a row is one wave's
+constexpr int kWorkgroups = 8192;  // of the gradient kernel, which strides over the rows
 
 // A launch takes fewer than 2^32 threads: the rows in slices, `kernel(p, rows)` for each.
 constexpr int kSlice = 1 << 20;
@@ -477,10 +479,10 @@ template <typename T>
 void run_grad(const T* logits, const PolArgs& p, const float2* stats, const float* coef,
               const float* gout, int done_if_one, T* grad, hipStream_t st) {
   if ((int64_t)p.v * (int64_t)sizeof(T) <= kWaveRow)
-    hipLaunchKernelGGL((pp_row_grad_kernel<T, 64>), dim3(std::min((p.rows + 3) / 4, 8192)), dim3(256), 0,
+    hipLaunchKernelGGL((pp_row_grad_kernel<T, 64>), dim3(std::min((p.rows + 3) / 4, kWorkgroups)), dim3(256), 0,
                        st, logits, p, stats, coef, gout, done_if_one, grad);
   else
-    hipLaunchKernelGGL((pp_row_grad_kernel<T, 256>), dim3(std::min(p.rows, 8192)), dim3(256), 0, st,
+    hipLaunchKernelGGL((pp_row_grad_kernel<T, 256>), dim3(std::min(p.rows, kWorkgroups)), dim3(256), 0, st,
                        logits, p, stats, coef, gout, done_if_one, grad);
 }
 

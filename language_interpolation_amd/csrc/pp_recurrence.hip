@@ -30,10 +30,10 @@
 // between are recomputed from it; y, rounded to 16 bits, would not do for the differences).
 //
 // Bound: forward 3 and backward 5 values an entry through HBM, each once.  Measured (MI355X, bf16):
-// [8, 2048, 2048] forward 53 us (4.0 TB/s with the kept states), backward 75 us (4.6); [1, 100003, 640] 106
-// and 148 us.  The rest is the shape of a workgroup: 16 waves of 112 registers are all that a CU holds, so
-// its loads, its walks (half of the time is instruction issue) and its waits follow one another; counter and
-// look-back are 5 to 15 % (measured without them).
+// [8, 2048, 2048] forward 50 us (4.2 TB/s with the kept states), backward 73 us (4.7); [1, 100003, 640] 101
+// and 144 us.  The rest is the shape of a workgroup: 16 waves of 113 registers are all that a CU holds, so
+// its loads, its walks and its waits follow one another.  Counter and look-back are 5 to 10 %, the gates
+// nothing (measured without them).
 #include <algorithm>
 
 #include "pp_device.h"
@@ -635,7 +635,7 @@ bool fits(int v, size_t size, std::initializer_list<const void*> at, std::initia
 }
 
 // A short row is one chunk, others are cut into chunks of kMostWaves stretches: with half of that the
-// long chains wait twice as often (bf16 [1, 100003, 640] forward + backward 292 against 248 us, fp32
+// long chains wait twice as often (bf16 [1, 100003, 640] forward + backward 289 against 241 us, fp32
 // [4, 1024, 2048] 75 against 64), and where nothing waits little is gained ([2, 8192, 2048] 129, 131).
 void plan(RecArgs& p, int v, void* ws) {
   p.ngroup = (p.d + 64 * v - 1) / (64 * v);

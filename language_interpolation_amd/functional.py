@@ -1039,6 +1039,12 @@ def _launch(name: str, device: torch.device, *args) -> None:
         _lib.check(rc, name)
 
 
+def _written(tensors) -> None:
+    """Tell autograd and the pre-split weight cache what was written through raw pointers (tensors of
+    inference mode have no version)."""
+    torch._C._increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _at(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -1178,7 +1184,7 @@ def gated_recurrence_step(z, f, h):
     z, f = _last_contiguous(z), _last_contiguous(f)
     _launch("pp_gated_recurrence_step", z.device, _at(z), z.stride(0), _at(f), f.stride(0),
             _ELEMENT[z.dtype], _at(h), max(h.stride(0), d), _at(y), b, d)
-    torch._C._increment_version([h])
+    _written([h])
     return y
 
 
@@ -1449,7 +1455,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
         for lo in range(0, len(unique), most):
             part = unique[lo:lo + most]
             _launch("pp_count_step", device, len(part), (c_void_p * len(part))(*[s.data_ptr() for s in part]))
-        torch._C._increment_version(unique)
+        _written(unique)
     elif min(steps) < 1:
         raise ValueError("adamw_step: steps are counted from 1")
     for lo in range(0, len(live), most):
@@ -1463,11 +1469,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
                 numbers(*[sizes[i] for i in part]), None if counted else numbers(*[steps[i] for i in part]),
                 pointers(*[steps[i].data_ptr() for i in part]) if counted else None, float(lr), b1, b2, float(eps),
                 float(weight_decay), _at(grad_scale), seed & 0xFFFFFFFF, lo)
-    # written through raw pointers: tell autograd and the pre-split weight cache
     for name, x in lists.items():
         if name != "grads":
             params = params + x
-    torch._C._increment_version(params)
+    _written(params)
 
 
 def decode_moment(codes, exponents, signed: bool, dtype=torch.float32):

@@ -163,6 +163,22 @@ def test_single_token(b, d, dtype):
     so.check(pool[:, :d], so.recurrence(z[:, :1], f[:, :1], h0)["h"], "state in a pool")
 
 
+def test_inference_mode():
+    """As a server calls it: states made inside and outside of inference mode."""
+    from language_interpolation_amd import functional as PF
+    z, f, _, h0, _ = _inputs(3, 20, 40, BF16, seed=14)
+    want = so.recurrence(z, f, h0)
+    outside = h0.cuda()
+    with torch.inference_mode():
+        inside = h0.cuda()
+        for h in (inside, outside):
+            for t in range(20):
+                PF.gated_recurrence_step(z.cuda()[:, t], f.cuda()[:, t], h)
+            so.check(h, want["h"], "state")
+        y, h = PF.gated_recurrence(z.cuda(), f.cuda(), h0.cuda())
+    so.check(y, want["y"], "y")
+
+
 def test_pieces_make_the_whole():
     """A long row in pieces with the state handed on, then token by token, is the row at once."""
     from language_interpolation_amd import functional as PF
