@@ -1146,7 +1146,8 @@ def gated_recurrence(z, f, h0=None, lengths=None, reset=None):
     one projection are).  h0: the state before the first step, fp32 [b, d] (default zeros).
     lengths: int [b], the steps of each row that exist (y is 0 behind them, h_last is the state
     before them); reset: bool [b, l], steps before which the state is dropped (a new document in a
-    packed row).  y has z's dtype, h_last is fp32.  Differentiable in z, f and h0."""
+    packed row).  y has z's dtype, h_last is fp32.  Differentiable in z, f and h0.  Formed as
+    z + a (h - z), which keeps the digits of a gate near 1: an infinite z gives NaN."""
     _require_element(z, "z")
     _require_element(f, "f", like=z)
     if z.dim() != 3 or f.shape != z.shape:
@@ -1298,7 +1299,8 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         if grad is not None:
             ctx.save_for_backward(logits, tokens, mask, stats, coef)
             ctx.grad, ctx.strides = (grad, gb, gt), (lb, lt)
-        loss, kl, clipped = out[0], out[1], out[2]
+        # (no views of each other for autograd: `loss /= n` is allowed, and `kl += x` leaves the loss alone)
+        loss, kl, clipped = (x.data for x in out.unbind())
         ctx.mark_non_differentiable(kl, clipped)
         return loss, kl, clipped
 
@@ -1327,8 +1329,8 @@ def clipped_policy_loss(logits, tokens, old_logp, advantages, ref_logp=None, mas
     mask: bool [b, t], False where a token does not count (nothing of it is read).  The mean is over
     the tokens that count (reduction "token"), or over the means of the sequences that have any
     ("sequence"); if none counts, all three are 0.  kl: mean k (0 without ref_logp); clipped: share
-    of the tokens whose ratio was clipped.  Differentiable in the logits; old_logp, advantages and
-    ref_logp are constants."""
+    of the tokens whose ratio was clipped.  The loss is differentiable in the logits (kl and clipped are
+    figures without a gradient); old_logp, advantages and ref_logp are constants."""
     tokens, mask = _check_classes(logits, tokens, mask)
     b, t, _ = logits.shape
     if reduction not in ("token", "sequence"):

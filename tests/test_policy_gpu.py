@@ -214,6 +214,24 @@ def test_repeated_backward_and_loss_scale():
         assert all(torch.equal(p, first[k]) for p, k in zip(plain, ("loss", "kl", "clipped")))
 
 
+def test_results_changed_in_place():
+    """Each of the three is a tensor of its own: the loss is divided (accumulated steps), figures are summed."""
+    from language_interpolation_amd import functional as PF
+    inputs = _inputs(2, 6, 40, F32, 77)
+    logits, tokens, old, adv, ref, m = (_cuda(x) for x in inputs)
+    whole = _loss(*inputs)
+    x = logits.requires_grad_()
+    loss, kl, cut = PF.clipped_policy_loss(x, tokens, old, adv, ref, m, LOW, HIGH, BETA)
+    assert not any(r._is_view() for r in (loss, kl, cut))
+    kl += 1.0
+    cut.zero_()
+    loss /= 4
+    loss.backward()
+    assert torch.equal(loss, whole["loss"] / 4)
+    assert torch.equal(kl, whole["kl"] + 1.0)
+    so.check(x.grad, _want(*inputs, gout=0.25)["grad"], "grad")
+
+
 def test_no_gradient_is_made_where_none_can_follow():
     from language_interpolation_amd import functional as PF
     s = _inputs(4, 64, 20000, BF16, seed=36)
