@@ -12,13 +12,13 @@
 // A masked token's logits, token, old, ref and advantage are not read; its gradient row is zeros.
 //
 // Bound: the logits are read once and the gradient written once.  A row that fits is therefore held
-// in registers, as it came, between the statistics and the gradient (pp_policy_fused_kernel: a wave,
-// 256 or 1024 threads a row, up to 16 vectors of 16 bytes a thread); a longer one is read twice
+// in registers, as it came, between the statistics and the gradient (pp_policy_fused_kernel: a wave or
+// 256 to 1024 threads a row, up to 16 vectors of 16 bytes a thread); a longer one is read twice
 // (pp_row_terms_kernel, then pp_row_grad_kernel, which are also the score and the backward alone).
 // Rows start anywhere: up to 7 elements before the first 16-byte boundary and behind the last are
 // taken one by one ("edge"), all others as aligned vectors.
-// Measured (MI355X, bf16): training [16, 384, 50021], 58 % of the tokens counting, 197 us (4.9 TB/s), [4, 1500,
-// 131072] 475 us (5.1), in registers against 303 and 594 read twice; score [8, 511, 32000] 27 us (5.5).  Between
+// Measured (MI355X, bf16): training [16, 384, 50021], 58 % of the tokens counting, 199 us (4.9 TB/s), [4, 1500,
+// 131072] 454 us (5.1), in registers against 303 and 594 read twice; score [8, 511, 32000] 27 us (5.5).  Between
 // load and store a row needs two exponentials an entry, which is 40 % of the time and hides only behind
 // the other rows of the CU: two at up to 65536 entries, one above.
 #include <algorithm>
@@ -65,44 +65,63 @@ struct Span {
   __device__ __forceinline__ int edge_at(int i) const { return i < head ? i : i + vecs * kVec; }
 };
 
-// max / sum over the THREADS lanes that share a row; red: one float a wave of the workgroup
-template <int THREADS>
-__device__ __forceinline__ float row_max(float v, float* red) {
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// What a lane has seen: the max, and the sum of exp(x - max), brought to a new max by one factor a vector.
+struct Running {
+  float max = -3.40282347e38f, sum = 0.0f;  // (finite, so that -inf - max is -inf and not NaN)
+  template <int N>
+  __device__ __forceinline__ void add(const float (&e)[N]) {
+    float top = max;
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = fmaxf(top, e[j]);
+    sum *= exp_of(max - top);
+    max = top;
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum += exp_of(e[j] - top);
+  }
+  __device__ __forceinline__ void add(float e) {
+    const float one[1] = {e};
+    add(one);
+  }
+};
+
+// The same of the THREADS lanes that share a row, the sum in 64 bits over the lanes.  One exchange through
+// LDS: each wave its pair, then as many neighbouring lanes as there are waves join those.
+struct MaxSum {
+  float max;
+  double sum;
+};
+__device__ __forceinline__ float wave_max(float v) {
   v = pp_dpp_max<0x128>(v);
   v = pp_dpp_max<0x124>(v);
   v = pp_dpp_max<0x122>(v);
   v = pp_dpp_max<0x121>(v);
-  v = fmaxf(fmaxf(pp_readlane_f(v, 0), pp_readlane_f(v, 16)), fmaxf(pp_readlane_f(v, 32), pp_readlane_f(v, 48)));
-  if (THREADS > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) v = fmaxf(v, red[i]);
-    __syncthreads();
-  }
-  return v;
+  return fmaxf(fmaxf(pp_readlane_f(v, 0), pp_readlane_f(v, 16)), fmaxf(pp_readlane_f(v, 32), pp_readlane_f(v, 48)));
 }
 template <int THREADS>
-__device__ __forceinline__ double row_sum(float v, double* red) {
+__device__ __forceinline__ MaxSum join_lanes(const Running& run, MaxSum* red) {
+  MaxSum r;
+  r.max = wave_max(run.max);
+  float v = run.sum * exp_of(run.max - r.max);
   v = pp_dpp_add<0x128>(v);
   v = pp_dpp_add<0x124>(v);
   v = pp_dpp_add<0x122>(v);
   v = pp_dpp_add<0x121>(v);
-  double s = ((double)pp_readlane_f(v, 0) + (double)pp_readlane_f(v, 16)) +
-             ((double)pp_readlane_f(v, 32) + (double)pp_readlane_f(v, 48));
+  r.sum = ((double)pp_readlane_f(v, 0) + (double)pp_readlane_f(v, 16)) +
+          ((double)pp_readlane_f(v, 32) + (double)pp_readlane_f(v, 48));
   if (THREADS > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    constexpr int kWaves = THREADS / 64;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = r;
     __syncthreads();
-    s = 0.0;
-    // (not all at once: that takes 32 registers beside the row)
-#pragma unroll 4
-    for (int i = 0; i < THREADS / 64; ++i) s += red[i];
-    __syncthreads();
+    const MaxSum mine = red[threadIdx.x % kWaves];
+    r.max = wave_max(mine.max);
+    r.sum = mine.sum * (double)exp_of(mine.max - r.max);
+#pragma unroll
+    for (int o = kWaves / 2; o; o >>= 1) r.sum += __shfl_xor(r.sum, o);
   }
-  return s;
+  return r;
 }
-
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
 // log of a sum: exponent and mantissa apart
 __device__ __forceinline__ double log_of(double sum) {
@@ -162,24 +181,14 @@ __device__ __forceinline__ void zero_row(T* __restrict__ g, int v, int tid) {
   if (tid < s.edge) g[s.edge_at(tid)] = (T)0.0f;
 }
 
-// The statistics of a row by one pass over it: every lane keeps a running max and the sum relative to
-// it, kAhead vectors in flight.
+// The statistics of a row by one pass over it, kAhead vectors in flight.
 template <typename T, int THREADS>
-__device__ __forceinline__ RowStats stream_stats(const T* __restrict__ x, int v, int tid, double* red) {
+__device__ __forceinline__ RowStats stream_stats(const T* __restrict__ x, int v, int tid, MaxSum* red) {
   constexpr int kVec = Span<T>::kVec, kAhead = 4;
   typedef PPElems<T, kVec> E;
   const Span<T> s(x, v);
   const T* body = x + s.head;
-  float m = -3.40282347e38f, sum = 0.0f;  // (finite, so that -inf - m is -inf and not NaN)
-  auto add = [&](const float (&e)[kVec]) {
-    float top = m;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) top = fmaxf(top, e[j]);
-    sum *= exp_of(m - top);
-    m = top;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) sum += exp_of(e[j] - m);
-  };
+  Running run;
   int i = tid;
   for (; i + (kAhead - 1) * THREADS < s.vecs; i += kAhead * THREADS) {
     typename E::raw r[kAhead];
@@ -189,21 +198,17 @@ __device__ __forceinline__ RowStats stream_stats(const T* __restrict__ x, int v,
     for (int k = 0; k < kAhead; ++k) {
       float e[kVec];
       E::get(r[k], e);
-      add(e);
+      run.add(e);
     }
   }
   for (; i < s.vecs; i += THREADS) {
     float e[kVec];
     E::get(E::take(body + (int64_t)i * kVec), e);
-    add(e);
+    run.add(e);
   }
-  if (tid < s.edge) {
-    const float e = (float)x[s.edge_at(tid)], top = fmaxf(m, e);
-    sum = sum * exp_of(m - top) + exp_of(e - top);
-    m = top;
-  }
-  const float top = row_max<THREADS>(m, reinterpret_cast<float*>(red));
-  return {top, log_of(row_sum<THREADS>(sum * exp_of(m - top), red))};
+  if (tid < s.edge) run.add((float)x[s.edge_at(tid)]);
+  const MaxSum all = join_lanes<THREADS>(run, red);
+  return {all.max, log_of(all.sum)};
 }
 
 // stats and lp, or stats, terms and coef, of each row.  THREADS lanes a row, 256 a workgroup.
@@ -211,7 +216,7 @@ template <typename T, int THREADS, bool POLICY>
 __global__ __launch_bounds__(256) void pp_row_terms_kernel(const T* __restrict__ logits, PolArgs p,
                                                            PolTerms q, float2* __restrict__ stats,
                                                            float* __restrict__ out) {
-  __shared__ double red[4];
+  __shared__ MaxSum red[4];
   const int tid = threadIdx.x % THREADS;
   const int row = p.first + blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
   if (row >= p.rows) return;
@@ -311,14 +316,14 @@ __device__ __forceinline__ void keep_raw(R (&r)[NV]) {
 }
 
 // Statistics, terms and gradient of a row that NV vectors a thread hold.  Up to 8 of them leave room for
-// 8 waves a SIMD (64 registers): without that bound [16, 384, 50021] takes 242 instead of 209 us.
+// 8 waves a SIMD (64 registers): without that bound [16, 384, 50021] takes 242 instead of 211 us.
 template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, NV <= 8 ? 8 : 4) void pp_policy_fused_kernel(
     const T* __restrict__ logits, PolArgs p, PolTerms q, float2* __restrict__ stats,
     float* __restrict__ coef, T* __restrict__ grad) {
   constexpr int kVec = Span<T>::kVec, kRows = THREADS < 256 ? 256 / THREADS : 1;
   typedef PPElems<T, kVec> E;
-  __shared__ double red[THREADS / 64 > 4 ? THREADS / 64 : 4];
+  __shared__ MaxSum red[THREADS / 64];
   const int tid = threadIdx.x % THREADS;
   const int row = p.first + blockIdx.x * kRows + threadIdx.x / THREADS;
   if (row >= p.rows) return;
@@ -345,50 +350,40 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, NV <= 8 ? 8 : 4) voi
   if (tid < s.edge) edge = (float)x[s.edge_at(tid)];
   const int64_t tok = p.tokens[row];
   const float xt = token_logit(x, tok, p.v);
-  float m = edge;
+  // (no max of the whole row first: with that exchange before the sums' own [4, 1500, 131072] takes 474, not 452
+  // us, [16, 384, 50021] 209, not 211)
+  Running run;
+  if (tid < s.edge) run.add(edge);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if (i * THREADS < s.vecs) {  // (the same for all lanes)
       float e[kVec];
       E::get(r[i], e);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) m = fmaxf(m, e[j]);
+      run.add(e);
     }
   }
   keep_raw(r);
-  m = row_max<THREADS>(m, reinterpret_cast<float*>(red));
-  float sum = tid < s.edge ? exp_of(edge - m) : 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (i * THREADS < s.vecs) {
-      float e[kVec];
-      E::get(r[i], e);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) sum += exp_of(e[j] - m);
-    }
-  }
-  keep_raw(r);
-  const double total = row_sum<THREADS>(sum, red);
-  const RowStats st = {m, log_of(total)};
+  const MaxSum all = join_lanes<THREADS>(run, red);
+  const RowStats st = {all.max, log_of(all.sum)};
   const float c = policy_terms(p, q, row, st.lp(xt), tid == 0);
   if (tid == 0) {
     if (stats) stats[row] = st.kept();
     if (coef) coef[row] = c;
   }
   if (!g) return;
-  const float k = -c / (float)total;
+  const float k = -c / (float)all.sum;
   const int token = tok >= 0 && tok < p.v ? (int)tok : -1 - kVec;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int n = i * THREADS + tid;
     if (n < s.vecs) {
       const int e = s.head + n * kVec;
-      E::stream(g + e, grad_vec<T>(r[i], m, k, c, token - e));
+      E::stream(g + e, grad_vec<T>(r[i], all.max, k, c, token - e));
     }
   }
   if (tid < s.edge) {
     const int e = s.edge_at(tid);
-    g[e] = (T)(k * exp_of(edge - m) + (e == token ? c : 0.0f));
+    g[e] = (T)(k * exp_of(edge - all.max) + (e == token ? c : 0.0f));
   }
 }
 
@@ -501,14 +496,16 @@ bool try_fused(const T* logits, const PolArgs& all, const PolTerms& q, float2* s
 template <typename T>
 void run_policy(const T* logits, const PolArgs& p, const PolTerms& q, float2* stats, float* coef, T* grad,
                 hipStream_t st) {
-  // (without a gradient too: the loss has the same bits whether one follows or not)
+  // The least threads that hold the row in 8 vectors, so that many rows share a CU (bf16 [8, 512, 20001] with 8 of
+  // 512 threads 75 us, with 4 of 1024 87; [8, 512, 12000] with 8 of 256 50, with 4 of 512 55); 16 vectors where
+  // 1024 threads are not enough.  Without a gradient too: the loss has the same bits whether one follows or not.
   if (try_fused<T, 64, 1>(logits, p, q, stats, coef, grad, st) ||
       try_fused<T, 64, 2>(logits, p, q, stats, coef, grad, st) ||
       try_fused<T, 64, 4>(logits, p, q, stats, coef, grad, st) ||
       try_fused<T, 256, 2>(logits, p, q, stats, coef, grad, st) ||
       try_fused<T, 256, 4>(logits, p, q, stats, coef, grad, st) ||
       try_fused<T, 256, 8>(logits, p, q, stats, coef, grad, st) ||
-      try_fused<T, 1024, 4>(logits, p, q, stats, coef, grad, st) ||
+      try_fused<T, 512, 8>(logits, p, q, stats, coef, grad, st) ||
       try_fused<T, 1024, 8>(logits, p, q, stats, coef, grad, st) ||
       try_fused<T, 1024, 16>(logits, p, q, stats, coef, grad, st))
     return;
