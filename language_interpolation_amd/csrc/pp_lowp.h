@@ -42,7 +42,7 @@ struct PPPair<pp_f16> {
 };
 
 // N consecutive elements as raw 32-bit words, loaded and stored in one access (N * sizeof(T) = 2
-// to 16 bytes, the address a multiple of that), and their fp32 values.
+// to 16 bytes, the address a multiple of that unless said otherwise), and their fp32 values.
 template <int BYTES>
 struct PPRaw;
 template <>
@@ -59,6 +59,12 @@ struct PPElems {
   typedef typename PPRaw<N * sizeof(T)>::type raw;
   static __device__ __forceinline__ raw load(const T* p) { return *reinterpret_cast<const raw*>(p); }
   static __device__ __forceinline__ void store(T* p, raw r) { *reinterpret_cast<raw*>(p) = r; }
+  // at any element: one access all the same
+  typedef raw loose __attribute__((aligned(sizeof(T))));
+  static __device__ __forceinline__ raw load_any(const T* p) { return *reinterpret_cast<const loose*>(p); }
+  static __device__ __forceinline__ void stream_any(T* p, raw r) {
+    __builtin_nontemporal_store(r, reinterpret_cast<loose*>(p));
+  }
   // what is read or written once: no place in the caches for it
   static __device__ __forceinline__ raw take(const T* p) {
     return __builtin_nontemporal_load(reinterpret_cast<const raw*>(p));

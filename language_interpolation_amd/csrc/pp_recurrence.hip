@@ -258,8 +258,8 @@ __device__ __forceinline__ void load_rows(typename PPElems<T, V>::raw (&fr)[kSte
                                           uint32_t ch, int n) {
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
-    fr[j] = PPElems<T, V>::load(fp + ch);
-    zr[j] = PPElems<T, V>::load(zp + ch);
+    fr[j] = PPElems<T, V>::load_any(fp + ch);
+    zr[j] = PPElems<T, V>::load_any(zp + ch);
     if (FAST || j + 1 < n) {  // behind the last: the last again
       fp += fl;
       zp += zl;
@@ -312,7 +312,7 @@ __device__ __forceinline__ void second_walk(T* yp, int d, uint32_t ch, int n, in
 #pragma unroll
     for (int v = 0; v < V; ++v)
       out[v] = FAST ? fmaf(pl[j][v], h[v], hl[j][v]) : j < n ? through(pl[j][v], hl[j][v], h[v]) : 0.0f;
-    if (FAST || j < rows) E::stream(yp + ch, E::put(out));
+    if (FAST || j < rows) E::stream_any(yp + ch, E::put(out));
     yp += d;
   }
 }
@@ -329,7 +329,7 @@ __device__ __forceinline__ void first_walk_back(const T* zp, int64_t zl, const T
   load_rows<FAST, T, V>(fr, fp, fl, zr, zp, zl, ch, n);
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
-    gr[j] = E::load(gp + ch);
+    gr[j] = E::load_any(gp + ch);
     if (FAST || j + 1 < n) gp += gl;
   }
 #pragma unroll
@@ -398,8 +398,8 @@ __device__ __forceinline__ void second_walk_back(T* gzp, T* gfp, int d, uint32_t
       }
     }
     if (FAST || j < rows) {
-      E::stream(gzp + ch, E::put(oz));
-      E::stream(gfp + ch, E::put(of));
+      E::stream_any(gzp + ch, E::put(oz));
+      E::stream_any(gfp + ch, E::put(of));
     }
     gzp -= d;
     gfp -= d;
@@ -419,9 +419,9 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
   draw_tile(p, &drawn, c, g, b);
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ch = (g * 64 + lane) * V;
-  const bool live = ch < p.d;
-  const uint32_t chl = live ? ch : 0;  // a lane without channels reads some and writes nothing
+  const int want = (g * 64 + lane) * V;
+  const bool live = want < p.d;            // a lane without channels reads the last ones and writes nothing
+  const uint32_t ch = min(want, p.d - V);  // (an odd last channel is taken with the one before, by two lanes alike)
   const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
   const int t0 = c * p.chunk + wave * kSteps;
   const int n = max(0, min(kSteps, len - t0));        // steps of this wave that exist
@@ -444,9 +444,9 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
     const T* fp = f + b * p.fb + t0 * p.fl;
     fast = n == kSteps && cut == 0;
     if (fast)
-      first_walk<true, T, V>(zp, p.zl, fp, p.fl, chl, n, cut, hl, pl, P, H);
+      first_walk<true, T, V>(zp, p.zl, fp, p.fl, ch, n, cut, hl, pl, P, H);
     else
-      first_walk<false, T, V>(zp, p.zl, fp, p.fl, chl, n, cut, hl, pl, P, H);
+      first_walk<false, T, V>(zp, p.zl, fp, p.fl, ch, n, cut, hl, pl, P, H);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) part[wave][v][lane] = make_float2(P[v], H[v]);
@@ -487,13 +487,13 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
   if (starts && n > 0) {
     float* at = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d;
 #pragma unroll
-    for (int v = 0; v < V; ++v) at[chl + v] = h[v];
+    for (int v = 0; v < V; ++v) at[ch + v] = h[v];
   }
   T* yp = y + row0 * p.d;
   if (fast)
-    second_walk<true, T, V>(yp, p.d, chl, n, rows, hl, pl, h);
+    second_walk<true, T, V>(yp, p.d, ch, n, rows, hl, pl, h);
   else
-    second_walk<false, T, V>(yp, p.d, chl, n, rows, hl, pl, h);
+    second_walk<false, T, V>(yp, p.d, ch, n, rows, hl, pl, h);
   if ((n > 0 && t0 + n == len) || (len == 0 && c == 0 && wave == 0)) {
 #pragma unroll
     for (int v = 0; v < V; ++v) h_last[(int64_t)b * p.d + ch + v] = through(P[v], H[v], h[v]);
@@ -515,9 +515,9 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
   draw_tile(p, &drawn, c, g, b);
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ch = (g * 64 + lane) * V;
-  const bool live = ch < p.d;
-  const uint32_t chl = live ? ch : 0;
+  const int want = (g * 64 + lane) * V;
+  const bool live = want < p.d;
+  const uint32_t ch = min(want, p.d - V);
   const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
   const int chunk0 = (p.nchunk - 1 - c) * p.chunk;  // first step of the chunk
   const int t0 = chunk0 + wave * kSteps;
@@ -544,12 +544,12 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
     const float* sp = starts + ((int64_t)b * ((p.l + kSteps - 1) / kSteps) + t0 / kSteps) * p.d;
     float h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = sp[chl + v];
+    for (int v = 0; v < V; ++v) h[v] = sp[ch + v];
     fast = n == kSteps && cut == 0;
     if (fast)
-      first_walk_back<true, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, chl, n, cut, h, q, gap, gr, P, G);
+      first_walk_back<true, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, ch, n, cut, h, q, gap, gr, P, G);
     else
-      first_walk_back<false, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, chl, n, cut, h, q, gap, gr, P, G);
+      first_walk_back<false, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, ch, n, cut, h, q, gap, gr, P, G);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) part[wave][v][lane] = make_float2(P[v], G[v]);
@@ -591,9 +591,9 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
   T* gzp = gz + row0 * p.d;
   T* gfp = gf + row0 * p.d;
   if (fast)
-    second_walk_back<true, T, V>(gzp, gfp, p.d, chl, n, rows, cut, q, gap, gr, u);
+    second_walk_back<true, T, V>(gzp, gfp, p.d, ch, n, rows, cut, q, gap, gr, u);
   else
-    second_walk_back<false, T, V>(gzp, gfp, p.d, chl, n, rows, cut, q, gap, gr, u);
+    second_walk_back<false, T, V>(gzp, gfp, p.d, ch, n, rows, cut, q, gap, gr, u);
   if (gh0 && chunk0 == 0 && wave == 0) {
 #pragma unroll
     for (int v = 0; v < V; ++v) gh0[(int64_t)b * p.d + ch + v] = u[v];
@@ -654,6 +654,16 @@ void fill(const RecArgs& p, int v, hipStream_t st) {
                      p.ticket, words);
 }
 
+// Two channels a lane, 4 bytes an access, in 16-bit types where that fills the lanes (fp32 has not the registers:
+// it spills), and where a wave for every 64 channels and 16 steps would be more than 16 for each of 256 CUs: more
+// and smaller waves win until then (bf16 forward + backward, one against two channels: [8, 2000, 256], 4000 waves,
+// 30 and 32 us, [10, 2000, 256], 5000 waves, 39 and 34, [1, 100003, 640] 302 and 241; [1, 100003, 64] 96 and 119).
+// Pairs start at any element: odd rows too ([8, 2048, 2047] 162 us, 198 by single elements).
+bool pairs(int dtype, int b, int l, int d) {
+  return dtype != PP_F32 && d > 64 &&
+         (int64_t)b * ((d + 63) / 64) * ((l + kSteps - 1) / kSteps) > 16 * 256;
+}
+
 template <typename T, int V>
 void run_fwd(const void* z, const void* f, void* y, float* h_last, float* starts, RecArgs p, void* ws,
              hipStream_t st) {
@@ -703,8 +713,7 @@ hipError_t pp_launch_rec_fwd(const void* z, int64_t zb, int64_t zl, const void* 
                              const uint8_t* reset, void* y, float* h_last, float* starts, void* ws,
                              int b, int l, int d, hipStream_t st) {
   const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, 0, 0, 0, h0, lengths, reset, nullptr, nullptr, nullptr};
-  // Two channels a lane in 16-bit types, one in fp32: 4 bytes an access either way.
-  const bool two = dtype != PP_F32 && fits(2, 2, {z, f, y}, {zb, zl, fb, fl, (int64_t)d});
+  const bool two = pairs(dtype, b, l, d);
 #define PP_CALL(T)                                                                      \
   do {                                                                                  \
     if (sizeof(T) == 2 && two)                                                          \
@@ -722,10 +731,7 @@ hipError_t pp_launch_rec_bwd(const void* z, int64_t zb, int64_t zl, const void* 
                              const float* gh_last, void* gz, void* gf, float* gh0, void* ws, int b,
                              int l, int d, hipStream_t st) {
   const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, 0, 0, 0, nullptr, lengths, reset, nullptr, nullptr, nullptr};
-  const size_t s = dtype == PP_F32 ? 4 : 2;
-  // (as in the forward; one channel a lane costs [1, 100003, 640] in bf16 201 instead of 144 us, two in
-  // fp32 more registers than there are)
-  const bool two = s == 2 && fits(2, s, {z, f, gy, gz, gf}, {zb, zl, fb, fl, gb, gl, (int64_t)d});
+  const bool two = pairs(dtype, b, l, d);
 #define PP_CALL(T)                                                           \
   do {                                                                       \
     if (sizeof(T) == 2 && two)                                               \

@@ -125,6 +125,32 @@ def test_strides_broadcasts_and_transposed_inputs():
     so.check(gf, ref["gf"], "gf of the state")
 
 
+# few and many (stretches of 16 steps) x (64 channels): one and two channels a lane in 16-bit types
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", [(3, 300, 1), (3, 300, 2), (3, 300, 127), (120, 300, 129), (70, 300, 255), (65, 1025, 66),
+                                   (260, 16, 1031), (33, 257, 512)])
+def test_rows_at_any_element(dtype, shape):
+    """16-bit rows of odd strides and addresses, cut and reset: pairs of channels start at any element."""
+    from language_interpolation_amd import functional as PF
+    b, l, d = shape
+    z, f, gy, h0, gh = _inputs(b, l, d, dtype, seed=d)
+    g = torch.Generator().manual_seed(d)
+    lengths = torch.randint(0, l + 1, (b,), generator=g, dtype=torch.int32)
+    lengths[0], lengths[-1] = l, 0
+    reset = torch.rand(b, l, generator=g) < 0.02
+    stride = d + 2 + (d + 1) % 2  # odd
+    rows = []
+    for x in (z, f, gy):
+        wide = torch.full((b, l, stride), float("nan"), dtype=dtype, device="cuda")
+        rows.append(wide[..., 1:1 + d].copy_(x.cuda()))
+    zd, fd, hd = rows[0].requires_grad_(), rows[1].requires_grad_(), h0.cuda().requires_grad_()
+    y, h = PF.gated_recurrence(zd, fd, h0=hd, lengths=lengths.cuda(), reset=reset.cuda())
+    grads = torch.autograd.grad((y, h), (zd, fd, hd), (rows[2], gh.cuda()))
+    _compare(dict(zip(("y", "h", "gz", "gf", "gh0"), (y, h) + grads)),
+             so.recurrence(z, f, h0, lengths, reset, gy, gh))
+    _compare(_run(z, f, gy, h0, gh), so.recurrence(z, f, h0, gy=gy, gh=gh))
+
+
 def test_gradient_against_differences():
     z, f, gy, h0, gh = (x.double() for x in _inputs(2, 37, 3, F32, seed=10))
     got = _run(z.float(), f.float(), gy.float(), h0.float(), gh.float())
