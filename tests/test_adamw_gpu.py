@@ -179,6 +179,52 @@ def test_decoded_moments():
                                torch.from_numpy(want).to(dt).nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_eight_bit_blocks_of_every_size(dtype):
+    """Blocks from the smallest to the largest exponent, codes of every value (no numbers among them), gradients
+    from none to large: v is 0, below 2^-96 or infinite in some waves and ordinary in others."""
+    n, rng = 4000 * 256 - 77, np.random.default_rng(12)
+    blocks = -(-n // 256)
+    host, dev = _tensors([n], dtype, 8, seed=12)
+    h = host[0]
+    g = rng.normal(size=n) * np.exp2(np.repeat(rng.integers(-70, 30, blocks), 256)[:n])
+    g[np.repeat(rng.random(blocks) < 0.3, 256)[:n]] = 0.0
+    h["g"] = torch.from_numpy(g.astype(np.float32)).to(dtype).float().numpy()
+    for k, none in (("m", 127), ("v", 255)):
+        h[k] = rng.integers(0, 256, n).astype(np.uint8)
+        every = np.repeat(rng.random(blocks) < 0.8, 256)[:n]  # the other blocks have codes that are no numbers
+        h[k][every & ((h[k] & none) == none)] = 5
+        h[k + "e"] = rng.integers(0, 255, blocks).astype(np.uint8)
+        dev[k][0].copy_(torch.from_numpy(h[k]))
+        dev[k + "e"][0].copy_(torch.from_numpy(h[k + "e"]))
+    dev["g"][0].copy_(torch.from_numpy(h["g"]))
+    for step in (3, 4):
+        _step(dev, dtype, 8, step, seed=8)
+        with np.errstate(all="ignore"):
+            _host_step(host, 8, step, seed=8)
+        assert _same(dev["w"][0], h["w"])
+        for k, none in (("m", 127), ("v", 255)):  # (the sign of what is no number is not specified)
+            got, want = dev[k][0].cpu().numpy(), h[k]
+            odd = (want & none) == none
+            assert np.array_equal((got & none) == none, odd) and np.array_equal(got[~odd], want[~odd]), k
+            assert _same(dev[k + "e"][0], h[k + "e"]), k
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_many_decoded_moments(dt):
+    """Enough of them for several turns a thread; the end inside a turn, aligned and not."""
+    from language_interpolation_amd import functional as PF
+    n = (1 << 23) + 5 * 512 + 13
+    g = torch.Generator().manual_seed(2)
+    codes = torch.randint(0, 256, (n,), generator=g).to(torch.uint8)
+    exps = torch.randint(100, 140, (-(-n // 256),), generator=g).to(torch.uint8)
+    odd = torch.empty(n + 3, dtype=torch.uint8, device="cuda")[3:].copy_(codes)
+    for signed, top in ((True, 14), (False, 30)):
+        want = torch.from_numpy(so.decode(codes.numpy(), exps.numpy(), top, signed)).to(dt).nan_to_num(7.0)
+        for c in (codes.cuda(), odd):
+            assert torch.equal(PF.decode_moment(c, exps.cuda(), signed, dt).cpu().nan_to_num(7.0), want)
+
+
 def test_eight_bits_follow_thirty_two():
     """200 steps with drifting gradients: a moment kept in 8 bits has the expected value of the exact
     one, where rounding to nearest would not let v move at all.  Mean over 50 000 entries; an entry's
