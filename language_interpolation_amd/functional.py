@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from ctypes import c_void_p
+from array import array
 from dataclasses import dataclass, field
 from typing import Optional, Tuple
 
@@ -1042,7 +1042,10 @@ def _launch(name: str, device: torch.device, *args) -> None:
 def _written(tensors) -> None:
     """Tell autograd and the pre-split weight cache what was written through raw pointers (tensors of
     inference mode have no version)."""
-    torch._C._increment_version([t for t in tensors if not t.is_inference()])
+    try:
+        torch._C._increment_version(tensors)
+    except RuntimeError:
+        torch._C._increment_version([t for t in tensors if not t.is_inference()])
 
 
 def _at(t: Optional[torch.Tensor]):
@@ -1416,34 +1419,40 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     dtype, device = params[0].dtype, params[0].device
     if (masters is not None) != (dtype != torch.float32):
         raise ValueError("adamw_step: masters belong to bfloat16 and float16 params, and these need them")
-    index, at = device.index, {"params": [p.data_ptr() for p in params]}
-    sizes, shapes = [p.numel() for p in params], [p.shape for p in params]
+    index, shapes = device.index, [p.shape for p in params]
+    at = {"params": [p.data_ptr() for p in params if p.dtype is dtype and p.get_device() == index]}
+    if len(at["params"]) < n:
+        i = [p.dtype is dtype and p.get_device() == index for p in params].index(False)
+        raise TypeError(f"adamw_step: params[{i}] is {params[i].dtype} on {params[i].device}, params[0] {dtype} on {device}")
     # the strides that all tensors of a param share; None: contiguous
     strides = [None if p.is_contiguous() else p.stride() for p in params]
-    for i, p in enumerate(params):
-        if p.dtype is not dtype or p.get_device() != index:
-            raise TypeError(f"adamw_step: params[{i}] is {p.dtype} on {p.device}, params[0] {dtype} on {device}")
-        if strides[i] is not None and not dense_storage(p):
-            raise ValueError(f"adamw_step: params[{i}] has gaps or overlaps (strides {p.stride()})")
+    for p, st in zip(params, strides):
+        if st is not None and not dense_storage(p):
+            raise ValueError(f"adamw_step: a param has gaps or overlaps (strides {st})")
+    sizes = [p.numel() for p in params]
     moment = torch.uint8 if eight else torch.float32
     wanted = {"grads": dtype, "exp_avgs": moment, "exp_avg_sqs": moment, "masters": torch.float32}
     for name, x in lists.items():
         kind = wanted.get(name)
-        for i, t in enumerate(x):
-            if t.get_device() == index:
-                if kind is None:
-                    if t.dtype is torch.uint8 and t.numel() == -(-sizes[i] // 256) and t.is_contiguous():
-                        continue
-                elif t.dtype is kind and t.shape == shapes[i] and (
-                        t.is_contiguous() if strides[i] is None else t.stride() == strides[i]):
-                    continue
-            raise ValueError(
-                f"adamw_step: {name}[{i}] ({t.dtype}, {tuple(t.shape)}, strides {t.stride()}, {t.device}) does not "
-                f"fit params[{i}] ({dtype}, {tuple(shapes[i])}, strides {params[i].stride()}, {device})")
-        at[name] = [t.data_ptr() for t in x]
-    live = range(n) if min(sizes) else [i for i in range(n) if sizes[i]]
+        if kind is None:  # (one comprehension a list: an attribute of a tensor costs the host 0.1 us)
+            at[name] = [t.data_ptr() for t, k in zip(x, sizes) if t.get_device() == index and t.dtype is torch.uint8 and
+                        t.numel() == -(-k // 256) and t.is_contiguous()]
+        else:
+            at[name] = [t.data_ptr() for t, s, st in zip(x, shapes, strides)
+                        if t.get_device() == index and t.dtype is kind and t.shape == s and
+                        (t.is_contiguous() if st is None else t.stride() == st)]
+        if len(at[name]) < n:
+            raise ValueError(f"adamw_step: {name} do not fit params ({dtype} on {device}; shape and strides of each, "
+                             f"{kind or 'uint8 [moment_blocks(numel)]'}): " + ", ".join(
+                                 f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}" for t in x[:8]))
+    numbers = steps
+    if not min(sizes):
+        live = [i for i in range(n) if sizes[i]]
+        at = {name: [x[i] for i in live] for name, x in at.items()}
+        sizes, numbers = [sizes[i] for i in live], [steps[i] for i in live]
+    count = len(sizes)
     for name, x in at.items():  # two updates of the same memory would race
-        if name != "grads" and len({x[i] for i in live}) < len(live):
+        if name != "grads" and len(set(x)) < count:
             raise ValueError(f"adamw_step: a tensor is twice in {name}")
     if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or
                                    grad_scale.device != device):
@@ -1456,20 +1465,22 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
                 raise ValueError("adamw_step: a step counter is one int64 on the device of the params")
         for lo in range(0, len(unique), most):
             part = unique[lo:lo + most]
-            _launch("pp_count_step", device, len(part), (c_void_p * len(part))(*[s.data_ptr() for s in part]))
+            counters = array("Q", [s.data_ptr() for s in part])
+            _launch("pp_count_step", device, len(part), counters.buffer_info()[0])
         _written(unique)
+        numbers = [s.data_ptr() for s in numbers]
     elif min(steps) < 1:
         raise ValueError("adamw_step: steps are counted from 1")
-    for lo in range(0, len(live), most):
-        part = live[lo:lo + most]
-        k = len(part)
-        pointers, numbers = c_void_p * k, ctypes.c_int64 * k
-        p, g, w, m, v, me, ve = (
-            pointers(*[at[name][i] for i in part]) if name in at else None
-            for name in ("params", "grads", "masters", "exp_avgs", "exp_avg_sqs", "avg_exponents", "sq_exponents"))
-        _launch("pp_adamw_step", device, k, _ELEMENT[dtype], 8 if eight else 32, p, g, w, m, v, me, ve,
-                numbers(*[sizes[i] for i in part]), None if counted else numbers(*[steps[i] for i in part]),
-                pointers(*[steps[i].data_ptr() for i in part]) if counted else None, float(lr), b1, b2, float(eps),
+    at = {name: array("Q", x) for name, x in at.items()}
+    at["sizes"], at["numbers"] = array("q", sizes), array("q", numbers)
+    base = {name: x.buffer_info()[0] for name, x in at.items()}
+    for lo in range(0, count, most):
+        p, g, w, m, v, me, ve, size, number = (
+            base[name] + 8 * lo if name in base else None
+            for name in ("params", "grads", "masters", "exp_avgs", "exp_avg_sqs", "avg_exponents", "sq_exponents",
+                         "sizes", "numbers"))
+        _launch("pp_adamw_step", device, min(most, count - lo), _ELEMENT[dtype], 8 if eight else 32, p, g, w, m, v, me,
+                ve, size, None if counted else number, number if counted else None, float(lr), b1, b2, float(eps),
                 float(weight_decay), _at(grad_scale), seed & 0xFFFFFFFF, lo)
     for name, x in lists.items():
         if name != "grads":
