@@ -1086,6 +1086,15 @@ def _graded(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _once_differentiable(backward):
+    """once_differentiable where a graph of the gradient is asked for; its guards cost 6 us a call."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
@@ -1119,7 +1128,7 @@ class GatedRecurrenceFunction(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, gy, gh):
         lib = _lib.load()
         z, f, starts, lengths, reset = ctx.saved_tensors
@@ -1242,7 +1251,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
         return lp
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, glp):
         logits, tokens, mask, stats = ctx.saved_tensors
         grad = _class_grad(logits, *ctx.strides)
@@ -1308,14 +1317,14 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         return loss, kl, clipped
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, gloss, _gkl, _gclipped):
         logits, tokens, mask, stats, coef = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
         done = int(grad is not None)
         if grad is None:
             grad = _class_grad(logits, *ctx.strides)
-        gout = gloss.reshape(1).to(torch.float32).contiguous()
+        gout = gloss if gloss.dtype is torch.float32 else gloss.float()
         _class_backward(logits, tokens, mask, stats, coef, gout, done, grad, ctx.strides)
         return (grad[0],) + (None,) * 10
 

@@ -130,3 +130,20 @@ def test_the_configured_optimizers_train(name):
         # float atomics in the small layers' weight gradients: the last bits differ, and an entry whose
         # gradient is nothing but those may step either way, 5 steps of lr
         assert float((p - q).detach().abs().max()) <= 5 * 2.2e-3
+
+
+def test_second_derivatives_are_refused():
+    """A graph of the gradient may be asked for (another term of the loss may need it); using it is an error."""
+    from language_interpolation_amd import functional as PF
+    z, f = (torch.randn(2, 20, 8, device="cuda", requires_grad=True) for _ in range(2))
+    x = torch.randn(2, 5, 30, device="cuda", requires_grad=True)
+    tok = torch.randint(0, 30, (2, 5), device="cuda")
+    old, adv = torch.full((2, 5), -3.0, device="cuda"), torch.ones(2, device="cuda")
+    calls = [(lambda: PF.gated_recurrence(z, f)[0].square().sum(), z), (lambda: PF.token_log_probs(x, tok).square().sum(), x),
+             (lambda: PF.clipped_policy_loss(x, tok, old, adv)[0].square(), x)]
+    for call, leaf in calls:
+        (plain,) = torch.autograd.grad(call(), leaf)
+        (g,) = torch.autograd.grad(call(), leaf, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="twice"):
+            g.sum().backward()
