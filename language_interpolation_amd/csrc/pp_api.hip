@@ -108,7 +108,7 @@ bool matrix_core_bwd_x(const PPShape& sh) { return dense_preferred(sh) && sh.B >
 
 extern "C" {
 
-int pp_version(void) { return 400; }  // 400: gated recurrence, token log-probabilities, clipped policy loss, AdamW; round 3: PP_FWD_TILE, PP_BWD_X_TILE, pp_forward_max_abs_ws_f32, regacc in parts, LayerNorm fold, grid tables
+int pp_version(void) { return 400; }  // 400: gated recurrence, token log-probabilities, clipped policy loss, AdamW; 302: PP_FWD_TILE, PP_BWD_X_TILE, pp_forward_max_abs_ws_f32, regacc in parts, LayerNorm fold, grid tables
 
 const char* pp_error_string(int code) {
   switch (code) {
