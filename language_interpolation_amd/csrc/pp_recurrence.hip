@@ -33,7 +33,7 @@
 // [8, 2048, 2048] forward 50 us (4.2 TB/s with the kept states), backward 73 us (4.7); [1, 100003, 640] 101
 // and 144 us.  The rest is the shape of a workgroup: 16 waves of 113 registers are all that a CU holds, so
 // its loads, its walks and its waits follow one another.  Counter and look-back are 5 to 10 %, the gates
-// nothing (measured without them).
+// nothing (measured without them).  Rows of few channels share waves (folds).
 #include <algorithm>
 
 #include "pp_device.h"
@@ -48,8 +48,9 @@ constexpr uint32_t kNotYet = 0xffffffffu;
 struct RecArgs {
   int64_t zb, zl, fb, fl, gb, gl;  // strides in elements of z, f and gy over batch and time
   int b, l, d;
-  int nchunk, ngroup;  // chunks of a row, groups of 64 V channels
+  int nchunk, ngroup;  // chunks of a row, groups of 64 V channels (of one row, or folded: of all)
   int chunk;           // steps of a chunk
+  int chains;
   const float* h0;
   const int32_t* lengths;
   const uint8_t* reset;
@@ -235,6 +236,14 @@ __device__ __forceinline__ uint32_t reset_bits(const uint8_t* reset, int64_t row
   return (uint32_t)__ballot(on);
 }
 
+// The same for one lane's row.
+__device__ __forceinline__ uint32_t own_reset_bits(const uint8_t* reset, int64_t at, int n) {
+  uint32_t bits = 0u;
+  if (reset)
+    for (int j = 0; j < n; ++j) bits |= (reset[at + j] != 0 ? 1u : 0u) << j;
+  return bits;
+}
+
 // this workgroup's chunk (counted along the chain), channel group and row
 __device__ __forceinline__ void draw_tile(const RecArgs& p, int* shared, int& c, int& g, int& b) {
   int id = blockIdx.x;
@@ -243,9 +252,8 @@ __device__ __forceinline__ void draw_tile(const RecArgs& p, int* shared, int& c,
     __syncthreads();
     id = __builtin_amdgcn_readfirstlane(*shared);
   }
-  const int chains = p.ngroup * p.b;
-  c = id / chains;
-  b = (id % chains) / p.ngroup;
+  c = id / p.chains;
+  b = (id % p.chains) / p.ngroup;
   g = id % p.ngroup;
 }
 
@@ -300,19 +308,27 @@ __device__ __forceinline__ void first_walk(const T* zp, int64_t zl, const T* fp,
   }
 }
 
+// (folded rows are a few bytes long: the cache joins a lane's to lines)
+template <bool FOLD, typename T, int V>
+__device__ __forceinline__ void put_row(T* at, const float (&x)[V]) {
+  if (FOLD)
+    PPElems<T, V>::store(at, PPElems<T, V>::put(x));
+  else
+    PPElems<T, V>::stream_any(at, PPElems<T, V>::put(x));
+}
+
 // y of each step from the state h that enters the stretch.
-template <bool FAST, typename T, int V>
+template <bool FAST, bool FOLD, typename T, int V>
 __device__ __forceinline__ void second_walk(T* yp, int d, uint32_t ch, int n, int rows,
                                             const float (&hl)[kSteps][V], const float (&pl)[kSteps][V],
                                             const float (&h)[V]) {
-  typedef PPElems<T, V> E;
 #pragma unroll
   for (int j = 0; j < kSteps; ++j) {
     float out[V];
 #pragma unroll
     for (int v = 0; v < V; ++v)
       out[v] = FAST ? fmaf(pl[j][v], h[v], hl[j][v]) : j < n ? through(pl[j][v], hl[j][v], h[v]) : 0.0f;
-    if (FAST || j < rows) E::stream_any(yp + ch, E::put(out));
+    if (FAST || j < rows) put_row<FOLD, T, V>(yp + ch, out);
     yp += d;
   }
 }
@@ -369,7 +385,7 @@ __device__ __forceinline__ void first_walk_back(const T* zp, int64_t zl, const T
 }
 
 // gz, gf of each step from the gradient u that arrives behind the stretch; u then leaves in front of it.
-template <bool FAST, typename T, int V>
+template <bool FAST, bool FOLD, typename T, int V>
 __device__ __forceinline__ void second_walk_back(T* gzp, T* gfp, int d, uint32_t ch, int n, int rows,
                                                  uint32_t cut, const float (&q)[kSteps][V],
                                                  const float (&gap)[kSteps][V],
@@ -398,8 +414,8 @@ __device__ __forceinline__ void second_walk_back(T* gzp, T* gfp, int d, uint32_t
       }
     }
     if (FAST || j < rows) {
-      E::stream_any(gzp + ch, E::put(oz));
-      E::stream_any(gfp + ch, E::put(of));
+      put_row<FOLD, T, V>(gzp + ch, oz);
+      put_row<FOLD, T, V>(gfp + ch, of);
     }
     gzp -= d;
     gfp -= d;
@@ -414,7 +430,29 @@ __device__ __forceinline__ void zero_rows(T* p, int d, uint32_t ch, int rows) {
   for (int j = 0; j < rows; ++j) PPElems<T, V>::stream_any(p + (int64_t)j * d + ch, zero);
 }
 
-template <typename T, int V>
+// What a lane works on.  FOLD: rows of fewer channels than half a wave share it, a lane's row is its own; a
+// sequence that has ended is then a stretch with P = 1, H = 0, and every chain is as long as the tensors.
+template <int V, bool FOLD>
+struct Place {
+  int b;        // row
+  uint32_t ch;  // first channel
+  bool live;    // (a lane without channels reads the last ones and writes nothing)
+  __device__ __forceinline__ Place(const RecArgs& p, int g, int row) {
+    const int want = (g * 64 + (int)(threadIdx.x & 63)) * V;
+    if (FOLD) {
+      live = want < p.b * p.d;
+      const int i = min(want, p.b * p.d - 1);
+      b = i / p.d;
+      ch = i % p.d;
+    } else {
+      live = want < p.d;
+      b = row;
+      ch = min(want, p.d - V);  // (an odd last channel is taken with the one before, by two lanes alike)
+    }
+  }
+};
+
+template <typename T, int V, bool FOLD>
 __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T* __restrict__ z,
                                                                  const T* __restrict__ f,
                                                                  T* __restrict__ y,
@@ -423,18 +461,20 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
   __shared__ float2 part[kMostWaves][V][64];
   __shared__ float carry[V][64];
   __shared__ int drawn;
-  int c, g, b;
-  draw_tile(p, &drawn, c, g, b);
+  int c, g, row;
+  draw_tile(p, &drawn, c, g, row);
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int want = (g * 64 + lane) * V;
-  const bool live = want < p.d;            // a lane without channels reads the last ones and writes nothing
-  const uint32_t ch = min(want, p.d - V);  // (an odd last channel is taken with the one before, by two lanes alike)
-  const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
+  const Place<V, FOLD> place(p, g, row);
+  const int b = place.b;
+  const uint32_t ch = place.ch;
+  const bool live = place.live;
+  const int own = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;  // steps of the row
+  const int len = FOLD ? p.l : own;                                   // steps of the chain
   const int t0 = c * p.chunk + wave * kSteps;
-  const int n = max(0, min(kSteps, len - t0));        // steps of this wave that exist
+  const int n = max(0, min(kSteps, own - t0));        // steps of this wave that exist
   const int rows = max(0, min(kSteps, p.l - t0));     // rows of y to write
-  const int64_t chain = (int64_t)b * p.ngroup + g;
+  const int64_t chain = FOLD ? g : (int64_t)b * p.ngroup + g;
   const int64_t row0 = (int64_t)b * p.l + t0;
   if (c > 0 && c * p.chunk >= len) {  // (all of the workgroup, and nobody waits for it)
     if (live) zero_rows<T, V>(y + row0 * p.d, p.d, ch, rows);
@@ -450,11 +490,12 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
   }
   uint32_t cut = 0;
   bool fast = false;
-  if (n > 0) {
-    cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
+  if (FOLD ? rows > 0 : n > 0) {
+    cut = FOLD ? own_reset_bits(p.reset, row0, n) : reset_bits(p.reset, (int64_t)b * p.l, t0, n);
     const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
     const T* fp = f + b * p.fb + t0 * p.fl;
     fast = n == kSteps && cut == 0;
+    if (FOLD) fast = __all(fast);
     if (fast)
       first_walk<true, T, V>(zp, p.zl, fp, p.fl, ch, n, cut, hl, pl, P, H);
     else
@@ -503,10 +544,10 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
   }
   T* yp = y + row0 * p.d;
   if (fast)
-    second_walk<true, T, V>(yp, p.d, ch, n, rows, hl, pl, h);
+    second_walk<true, FOLD, T, V>(yp, p.d, ch, n, rows, hl, pl, h);
   else
-    second_walk<false, T, V>(yp, p.d, ch, n, rows, hl, pl, h);
-  if ((n > 0 && t0 + n == len) || (len == 0 && c == 0 && wave == 0)) {
+    second_walk<false, FOLD, T, V>(yp, p.d, ch, n, rows, hl, pl, h);
+  if (FOLD ? rows > 0 && t0 + rows == p.l : (n > 0 && t0 + n == len) || (len == 0 && c == 0 && wave == 0)) {
 #pragma unroll
     for (int v = 0; v < V; ++v) h_last[(int64_t)b * p.d + ch + v] = through(P[v], H[v], h[v]);
   }
@@ -514,7 +555,7 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
 
 // Chunks are counted from the end of the (allocated) row: chunk c of the chain is row chunk
 // nchunk - 1 - c; those behind the end of a shorter row only write zeros.
-template <typename T, int V>
+template <typename T, int V, bool FOLD>
 __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
     const T* __restrict__ z, const T* __restrict__ f, const float* __restrict__ starts,
     const T* __restrict__ gy, const float* __restrict__ gh, T* __restrict__ gz, T* __restrict__ gf,
@@ -523,19 +564,21 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
   __shared__ float2 part[kMostWaves][V][64];
   __shared__ float carry[V][64];
   __shared__ int drawn;
-  int c, g, b;
-  draw_tile(p, &drawn, c, g, b);
+  int c, g, row;
+  draw_tile(p, &drawn, c, g, row);
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int want = (g * 64 + lane) * V;
-  const bool live = want < p.d;
-  const uint32_t ch = min(want, p.d - V);
-  const int len = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
+  const Place<V, FOLD> place(p, g, row);
+  const int b = place.b;
+  const uint32_t ch = place.ch;
+  const bool live = place.live;
+  const int own = p.lengths ? max(0, min(p.l, p.lengths[b])) : p.l;
+  const int len = FOLD ? p.l : own;
   const int chunk0 = (p.nchunk - 1 - c) * p.chunk;  // first step of the chunk
   const int t0 = chunk0 + wave * kSteps;
-  const int n = max(0, min(kSteps, len - t0));
+  const int n = max(0, min(kSteps, own - t0));
   const int rows = max(0, min(kSteps, p.l - t0));
-  const int64_t chain = (int64_t)b * p.ngroup + g;
+  const int64_t chain = FOLD ? g : (int64_t)b * p.ngroup + g;
   const int64_t row0 = (int64_t)b * p.l + t0;
   if (chunk0 > 0 && chunk0 >= len) {
     if (live) {
@@ -555,8 +598,8 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
   }
   uint32_t cut = 0;
   bool fast = false;
-  if (n > 0) {
-    cut = reset_bits(p.reset, (int64_t)b * p.l, t0, n);
+  if (FOLD ? rows > 0 : n > 0) {
+    cut = FOLD ? own_reset_bits(p.reset, row0, n) : reset_bits(p.reset, (int64_t)b * p.l, t0, n);
     const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
     const T* fp = f + b * p.fb + t0 * p.fl;
     const T* gp = gy + b * p.gb + t0 * p.gl;
@@ -565,6 +608,7 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = sp[ch + v];
     fast = n == kSteps && cut == 0;
+    if (FOLD) fast = __all(fast);
     if (fast)
       first_walk_back<true, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, ch, n, cut, h, q, gap, gr, P, G);
     else
@@ -610,9 +654,9 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
   T* gzp = gz + row0 * p.d;
   T* gfp = gf + row0 * p.d;
   if (fast)
-    second_walk_back<true, T, V>(gzp, gfp, p.d, ch, n, rows, cut, q, gap, gr, u);
+    second_walk_back<true, FOLD, T, V>(gzp, gfp, p.d, ch, n, rows, cut, q, gap, gr, u);
   else
-    second_walk_back<false, T, V>(gzp, gfp, p.d, ch, n, rows, cut, q, gap, gr, u);
+    second_walk_back<false, FOLD, T, V>(gzp, gfp, p.d, ch, n, rows, cut, q, gap, gr, u);
   if (gh0 && chunk0 == 0 && wave == 0) {
 #pragma unroll
     for (int v = 0; v < V; ++v) gh0[(int64_t)b * p.d + ch + v] = u[v];
@@ -656,19 +700,20 @@ bool fits(int v, size_t size, std::initializer_list<const void*> at, std::initia
 // A short row is one chunk, others are cut into chunks of kMostWaves stretches: with half of that the
 // long chains wait twice as often (bf16 [1, 100003, 640] forward + backward 289 against 241 us, fp32
 // [4, 1024, 2048] 75 against 64), and where nothing waits little is gained ([2, 8192, 2048] 129, 131).
-void plan(RecArgs& p, int v, void* ws) {
-  p.ngroup = (p.d + 64 * v - 1) / (64 * v);
+void plan(RecArgs& p, int v, bool fold, void* ws) {
+  p.ngroup = ((fold ? p.b * p.d : p.d) + 64 * v - 1) / (64 * v);
+  p.chains = fold ? p.ngroup : p.ngroup * p.b;
   p.chunk = kSteps * std::min(kMostWaves, (p.l + kSteps - 1) / kSteps);
   p.nchunk = (p.l + p.chunk - 1) / p.chunk;
   p.ticket = static_cast<uint32_t*>(ws);
-  const int64_t n = (int64_t)p.b * p.nchunk * p.ngroup * 64 * v;
+  const int64_t n = (int64_t)p.chains * p.nchunk * 64 * v;
   p.part = reinterpret_cast<unsigned long long*>(p.ticket + 4);
   p.done = reinterpret_cast<uint32_t*>(p.part + n);
 }
 
 void fill(const RecArgs& p, int v, hipStream_t st) {
   if (p.nchunk == 1) return;
-  const int64_t words = 4 + (int64_t)p.b * p.nchunk * p.ngroup * 64 * v * 3;
+  const int64_t words = 4 + (int64_t)p.chains * p.nchunk * 64 * v * 3;
   hipLaunchKernelGGL(pp_rec_fill_kernel, dim3((unsigned)((words + 1023) / 1024)), dim3(256), 0, st,
                      p.ticket, words);
 }
@@ -683,21 +728,30 @@ bool pairs(int dtype, int b, int l, int d) {
          (int64_t)b * ((d + 63) / 64) * ((l + kSteps - 1) / kSteps) > 16 * 256;
 }
 
-template <typename T, int V>
+// Rows of up to 32 channels share waves where a wave a row would be more than 16 for each of 256 CUs and shared waves
+// are still enough to hide the loads of single rows (us, bf16 forward + backward, shared and a wave a row: [457, 131072,
+// 1] 1377 and 11798, [256, 5000, 16] 103 and 287, [256, 5000, 32] 185 and 295, [64, 2000, 4], 500 waves, 34 and 43;
+// [300, 300, 3], 285 waves, 48 and 45, [128, 1000, 2], 252 waves, 58 and 42).
+bool folds(int b, int l, int d) {
+  const int64_t stretches = (l + kSteps - 1) / kSteps;
+  return d <= 32 && b * stretches > 16 * 256 && ((int64_t)b * d + 63) / 64 * stretches >= 384;
+}
+
+template <typename T, int V, bool FOLD>
 void run_fwd(const void* z, const void* f, void* y, float* h_last, float* starts, RecArgs p, void* ws,
              hipStream_t st) {
-  plan(p, V, ws);
+  plan(p, V, FOLD, ws);
   fill(p, V, st);
-  hipLaunchKernelGGL((pp_rec_fwd_kernel<T, V>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
+  hipLaunchKernelGGL((pp_rec_fwd_kernel<T, V, FOLD>), dim3((unsigned)p.nchunk * p.chains),
                      dim3(4 * p.chunk), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
                      static_cast<T*>(y), h_last, starts, p);
 }
-template <typename T, int V>
+template <typename T, int V, bool FOLD>
 void run_bwd(const void* z, const void* f, const float* starts, const void* gy, const float* gh,
              void* gz, void* gf, float* gh0, RecArgs p, void* ws, hipStream_t st) {
-  plan(p, V, ws);
+  plan(p, V, FOLD, ws);
   fill(p, V, st);
-  hipLaunchKernelGGL((pp_rec_bwd_kernel<T, V>), dim3((unsigned)p.nchunk * p.ngroup * p.b),
+  hipLaunchKernelGGL((pp_rec_bwd_kernel<T, V, FOLD>), dim3((unsigned)p.nchunk * p.chains),
                      dim3(4 * p.chunk), 0, st, static_cast<const T*>(z), static_cast<const T*>(f),
                      starts, static_cast<const T*>(gy), gh, static_cast<T*>(gz), static_cast<T*>(gf),
                      gh0, p);
@@ -731,14 +785,16 @@ hipError_t pp_launch_rec_fwd(const void* z, int64_t zb, int64_t zl, const void* 
                              int64_t fl, int dtype, const float* h0, const int32_t* lengths,
                              const uint8_t* reset, void* y, float* h_last, float* starts, void* ws,
                              int b, int l, int d, hipStream_t st) {
-  const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, 0, 0, 0, h0, lengths, reset, nullptr, nullptr, nullptr};
+  const RecArgs p = {zb, zl, fb, fl, 0, 0, b, l, d, 0, 0, 0, 0, h0, lengths, reset, nullptr, nullptr, nullptr};
   const bool two = pairs(dtype, b, l, d);
 #define PP_CALL(T)                                                                      \
   do {                                                                                  \
-    if (sizeof(T) == 2 && two)                                                          \
-      run_fwd<T, sizeof(T) == 2 ? 2 : 1>(z, f, y, h_last, starts, p, ws, st);           \
+    if (folds(b, l, d))                                                                 \
+      run_fwd<T, 1, true>(z, f, y, h_last, starts, p, ws, st);                          \
+    else if (sizeof(T) == 2 && two)                                                     \
+      run_fwd<T, sizeof(T) == 2 ? 2 : 1, false>(z, f, y, h_last, starts, p, ws, st);    \
     else                                                                                \
-      run_fwd<T, 1>(z, f, y, h_last, starts, p, ws, st);                                \
+      run_fwd<T, 1, false>(z, f, y, h_last, starts, p, ws, st);                         \
   } while (0)
   PP_REC_TYPES(PP_CALL);
 #undef PP_CALL
@@ -749,14 +805,16 @@ hipError_t pp_launch_rec_bwd(const void* z, int64_t zb, int64_t zl, const void* 
                              const float* starts, const void* gy, int64_t gb, int64_t gl,
                              const float* gh_last, void* gz, void* gf, float* gh0, void* ws, int b,
                              int l, int d, hipStream_t st) {
-  const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, 0, 0, 0, nullptr, lengths, reset, nullptr, nullptr, nullptr};
+  const RecArgs p = {zb, zl, fb, fl, gb, gl, b, l, d, 0, 0, 0, 0, nullptr, lengths, reset, nullptr, nullptr, nullptr};
   const bool two = pairs(dtype, b, l, d);
 #define PP_CALL(T)                                                           \
   do {                                                                       \
-    if (sizeof(T) == 2 && two)                                               \
-      run_bwd<T, sizeof(T) == 2 ? 2 : 1>(z, f, starts, gy, gh_last, gz, gf, gh0, p, ws, st); \
+    if (folds(b, l, d))                                                      \
+      run_bwd<T, 1, true>(z, f, starts, gy, gh_last, gz, gf, gh0, p, ws, st); \
+    else if (sizeof(T) == 2 && two)                                          \
+      run_bwd<T, sizeof(T) == 2 ? 2 : 1, false>(z, f, starts, gy, gh_last, gz, gf, gh0, p, ws, st); \
     else                                                                     \
-      run_bwd<T, 1>(z, f, starts, gy, gh_last, gz, gf, gh0, p, ws, st);      \
+      run_bwd<T, 1, false>(z, f, starts, gy, gh_last, gz, gf, gh0, p, ws, st); \
   } while (0)
   PP_REC_TYPES(PP_CALL);
 #undef PP_CALL

@@ -125,10 +125,12 @@ def test_strides_broadcasts_and_transposed_inputs():
     so.check(gf, ref["gf"], "gf of the state")
 
 
-# few and many (stretches of 16 steps) x (64 channels): one and two channels a lane in 16-bit types
-@pytest.mark.parametrize("dtype", [BF16, F16])
+# few and many (stretches of 16 steps) x (64 channels): one and two channels a lane in 16-bit types; narrow rows
+# that share a wave
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("shape", [(3, 300, 1), (3, 300, 2), (3, 300, 127), (120, 300, 129), (70, 300, 255), (65, 1025, 66),
-                                   (260, 16, 1031), (33, 257, 512)])
+                                   (260, 16, 1031), (33, 257, 512), (6500, 64, 1), (450, 304, 3), (4200, 16, 7),
+                                   (131, 513, 32), (5, 14000, 5)])
 def test_rows_at_any_element(dtype, shape):
     """16-bit rows of odd strides and addresses, cut and reset: pairs of channels start at any element."""
     from language_interpolation_amd import functional as PF
