@@ -1113,11 +1113,11 @@ class GatedRecurrenceFunction(torch.autograd.Function):
         h0 = None if h0 is None else h0.contiguous()
         starts = None
         if z.numel() == 0:  # no step: the state stays as it is
-            h = torch.zeros(b, d, device=z.device) if h0 is None else h0.clone()
+            h = torch.zeros(b, d, device=z.device, dtype=torch.float32) if h0 is None else h0.clone()
         else:
             h = torch.empty(b, d, device=z.device, dtype=torch.float32)
             if graded:
-                starts = torch.empty(b, lib.pp_gated_recurrence_starts(l), d, device=z.device)
+                starts = torch.empty(b, lib.pp_gated_recurrence_starts(l), d, device=z.device, dtype=torch.float32)
             nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
             ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
             _launch("pp_gated_recurrence_fwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
@@ -1139,7 +1139,7 @@ class GatedRecurrenceFunction(torch.autograd.Function):
         if z.numel() == 0:
             return gz, gf, gh if ctx.needs_input_grad[2] else None, None, None, None
         gy = torch.zeros_like(gz) if gy is None else _last_contiguous(gy)
-        gh0 = torch.empty(b, d, device=z.device) if ctx.needs_input_grad[2] else None
+        gh0 = torch.empty(b, d, device=z.device, dtype=torch.float32) if ctx.needs_input_grad[2] else None
         nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
         ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
         _launch("pp_gated_recurrence_bwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
@@ -1241,7 +1241,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
         b, t, v = logits.shape
         logits, lb, lt = _class_rows(logits)
         lp = torch.empty(b, t, device=logits.device, dtype=torch.float32)
-        stats = torch.empty(b, t, 2, device=logits.device) if graded else None
+        stats = torch.empty(b, t, 2, device=logits.device, dtype=torch.float32) if graded else None
         if lp.numel():
             _launch("pp_token_log_probs_fwd", logits.device, _at(logits), lb, lt,
                     _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(lp), _at(stats), b, t, v)
@@ -1296,8 +1296,8 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         stats = coef = grad = None
         gb = gt = 0
         if graded:
-            stats = torch.empty(b, t, 2, device=logits.device)
-            coef = torch.empty(b, t, device=logits.device)
+            stats = torch.empty(b, t, 2, device=logits.device, dtype=torch.float32)
+            coef = torch.empty(b, t, device=logits.device, dtype=torch.float32)
             grad, gb, gt = _class_grad(logits, lb, lt)
         if b * t:
             nbytes = lib.pp_clipped_policy_loss_workspace_bytes(b, t)

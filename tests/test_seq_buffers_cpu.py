@@ -1,0 +1,68 @@
+"""What the sequence-model operators hand to the library, without a GPU: the entries are replaced, tensors take the
+place of addresses."""
+import contextlib
+
+import pytest
+import torch
+
+from language_interpolation_amd import functional as PF
+
+F32 = torch.float32
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The calls made of the library: (entry, arguments with tensors for addresses)."""
+    made = []
+    monkeypatch.setattr(PF, "_at", lambda t: t)
+    monkeypatch.setattr(PF, "_launch", lambda name, device, *args: made.append((name, args)))
+    return made
+
+
+@contextlib.contextmanager
+def default_dtype(dtype):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        yield
+    finally:
+        torch.set_default_dtype(before)
+
+
+def _recurrence(b=2, l=40, d=3, dtype=F32, h0=True):
+    z, f = (torch.randn(b, l, d, dtype=F32).to(dtype).requires_grad_() for _ in range(2))
+    h0 = torch.zeros(b, d, dtype=F32, requires_grad=True) if h0 else None
+    y, h = PF.GatedRecurrenceFunction.apply(z, f, h0, None, None, True)
+    grads = torch.autograd.grad((y, h), [x for x in (z, f, h0) if x is not None],
+                                (torch.zeros_like(y), torch.zeros_like(h)))
+    return y, h, grads
+
+
+@pytest.mark.parametrize("default", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
+def test_buffers_of_floats_are_floats(calls, default):
+    """The kernels write 4-byte floats whatever the program's default dtype."""
+    b, l, d, t, v = 2, 40, 3, 5, 11
+    with default_dtype(default):
+        y, h, grads = _recurrence(b, l, d)
+        assert h.dtype == F32 and grads[2].dtype == F32
+        empty = PF.GatedRecurrenceFunction.apply(torch.zeros(b, 0, d, dtype=F32), torch.zeros(b, 0, d, dtype=F32), None, None,
+                                                 None, False)
+        assert empty[1].dtype == F32
+        x = torch.randn(b, t, v, dtype=F32, requires_grad=True)
+        tokens = torch.zeros(b, t, dtype=torch.int64)
+        lp = PF.TokenLogProbsFunction.apply(x, tokens, None, True)
+        torch.autograd.grad(lp, x, torch.zeros_like(lp))
+        old, adv = torch.zeros(b, t, dtype=F32), torch.zeros(b, t, dtype=F32)
+        loss, _, _ = PF.ClippedPolicyLossFunction.apply(x, tokens, None, old, adv, None, 0.2, 0.2, 0.0, 0, True)
+        torch.autograd.grad(loss, x, torch.ones((), dtype=F32))
+    steps = -(-l // 16)
+    floats = {"pp_gated_recurrence_fwd": {11: b * d, 12: b * steps * d},
+              "pp_gated_recurrence_bwd": {9: b * steps * d, 13: b * d, 16: b * d},
+              "pp_token_log_probs_fwd": {6: b * t, 7: b * t * 2},
+              "pp_token_log_probs_bwd": {6: b * t * 2, 7: b * t},
+              "pp_clipped_policy_loss_fwd": {15: 3, 16: b * t * 2, 17: b * t}}
+    assert {name for name, _ in calls} == set(floats)
+    for name, args in calls:
+        for at, count in floats[name].items():
+            if args[at] is not None:
+                assert args[at].dtype == F32 and args[at].numel() == count and args[at].is_contiguous(), (name, at)

@@ -1,0 +1,55 @@
+"""Calls of the sequence-model operators as larger programs make them: another default dtype, hooks on what a graph
+saves, checkpointing, many rows."""
+import contextlib
+
+import pytest
+import torch
+
+from language_interpolation_amd import functional as PF
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@contextlib.contextmanager
+def _default_dtype(dtype):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        yield
+    finally:
+        torch.set_default_dtype(before)
+
+
+def _trained(dtype, seed=0):
+    """One training call of each operator: all results, gradients and states."""
+    g = torch.Generator().manual_seed(seed)
+
+    def normal(*shape, dtype=F32):
+        return torch.randn(*shape, generator=g, dtype=F32).to(dtype).cuda()
+    z, f, gy = (normal(3, 70, 37, dtype=dtype) for _ in range(3))
+    h0, gh = normal(3, 37), normal(3, 37)
+    leaves = [x.requires_grad_() for x in (z, f, h0)]
+    y, h = PF.gated_recurrence(z, f, h0)
+    out = [y, h, *torch.autograd.grad((y, h), leaves, (gy, gh))]
+    x = normal(4, 9, 301, dtype=dtype).requires_grad_()
+    tokens = torch.randint(0, 301, (4, 9), generator=g).cuda()
+    lp = PF.token_log_probs(x, tokens)
+    out += [lp, *torch.autograd.grad(lp, x, normal(4, 9))]
+    loss, kl, cut = PF.clipped_policy_loss(x, tokens, lp.detach() - 0.1, normal(4, 9), lp.detach() + 0.1, kl_coef=0.1)
+    out += [loss, kl, cut, *torch.autograd.grad(loss, x, torch.tensor(0.5, dtype=F32, device="cuda"))]
+    p, grad = normal(5000, dtype=dtype), normal(5000, dtype=dtype)
+    master = None if dtype == F32 else [p.float()]
+    m, v = (torch.zeros(5000, dtype=F32, device="cuda") for _ in range(2))
+    PF.adamw_step([p], [grad], [m], [v], 1, lr=1e-2, masters=master)
+    return out + [p, m, v]
+
+
+@pytest.mark.parametrize("default", [BF16, F16, torch.float64])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_default_dtype_changes_nothing(dtype, default):
+    want = _trained(dtype)
+    with _default_dtype(default):
+        got = _trained(dtype)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and torch.equal(a, b)
