@@ -1225,6 +1225,12 @@ def _class_grad(logits, lb, lt):
     return buf.as_strided((b, t, v), (gb, gt, 1), off), gb, gt
 
 
+def _same_rows(logits, lb, lt, grad, gb, gt) -> bool:
+    """Every row of the gradient begins at its logits' offset within 16 bytes."""
+    vec = 16 // logits.element_size()
+    return (grad.data_ptr() - logits.data_ptr()) % 16 == 0 and (gb - lb) % vec == 0 and (gt - lt) % vec == 0
+
+
 def _check_classes(logits, tokens, mask):
     _require_element(logits, "logits")
     if logits.dim() != 3 or logits.shape[2] < 1:
@@ -1247,15 +1253,15 @@ class TokenLogProbsFunction(torch.autograd.Function):
                     _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(lp), _at(stats), b, t, v)
         if stats is not None:
             ctx.save_for_backward(logits, tokens, mask, stats)
-            ctx.strides = (lb, lt)
         return lp
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, glp):
         logits, tokens, mask, stats = ctx.saved_tensors
-        grad = _class_grad(logits, *ctx.strides)
-        _class_backward(logits, tokens, mask, stats, glp.float().contiguous(), None, 0, grad, ctx.strides)
+        logits, lb, lt = _class_rows(logits)  # (hooks on saved tensors may have laid them out anew)
+        grad = _class_grad(logits, lb, lt)
+        _class_backward(logits, tokens, mask, stats, glp.float().contiguous(), None, 0, grad, (lb, lt))
         return grad[0], None, None, None
 
 
@@ -1310,7 +1316,7 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
             out.zero_()
         if grad is not None:
             ctx.save_for_backward(logits, tokens, mask, stats, coef)
-            ctx.grad, ctx.strides = (grad, gb, gt), (lb, lt)
+            ctx.grad = (grad, gb, gt)
         # (no views of each other for autograd: `loss /= n` is allowed, and `kl += x` leaves the loss alone)
         loss, kl, clipped = (x.data for x in out.unbind())
         ctx.mark_non_differentiable(kl, clipped)
@@ -1320,12 +1326,13 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, gloss, _gkl, _gclipped):
         logits, tokens, mask, stats, coef = ctx.saved_tensors
+        logits, lb, lt = _class_rows(logits)
         grad, ctx.grad = ctx.grad, None
-        done = int(grad is not None)
-        if grad is None:
-            grad = _class_grad(logits, *ctx.strides)
+        done = grad is not None and _same_rows(logits, lb, lt, *grad)
+        if not done:
+            grad = _class_grad(logits, lb, lt)
         gout = gloss if gloss.dtype is torch.float32 else gloss.float()
-        _class_backward(logits, tokens, mask, stats, coef, gout, done, grad, ctx.strides)
+        _class_backward(logits, tokens, mask, stats, coef, gout, int(done), grad, (lb, lt))
         return (grad[0],) + (None,) * 10
 
 

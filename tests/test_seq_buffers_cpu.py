@@ -66,3 +66,35 @@ def test_buffers_of_floats_are_floats(calls, default):
         for at, count in floats[name].items():
             if args[at] is not None:
                 assert args[at].dtype == F32 and args[at].numel() == count and args[at].is_contiguous(), (name, at)
+
+
+def _inside(t, strides, shape):
+    """Elements shape[0] x shape[1] rows of shape[2] at these strides lie inside the storage of t."""
+    last = t.storage_offset() + sum((n - 1) * s for n, s in zip(shape, (*strides, 1)))
+    return last < t.untyped_storage().nbytes() // t.element_size()
+
+
+@pytest.mark.parametrize("policy", [False, True])
+def test_logits_laid_out_anew_by_a_hook(calls, policy):
+    """Hooks on saved tensors (save_on_cpu, compression) bring a slice of the logits back as a tensor of its own: the
+    backward goes by the strides of what it is given."""
+    b, t, v = 3, 6, 65
+    wide = torch.randn(b, t + 2, v + 7, dtype=F32, requires_grad=True)
+    tokens = torch.zeros(b, t, dtype=torch.int64)
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x.contiguous().clone(), lambda x: x):
+        x = wide[:, 1:t + 1, 3:v + 3]
+        if policy:
+            rows = torch.zeros(b, t)
+            out, _, _ = PF.ClippedPolicyLossFunction.apply(x, tokens, None, rows, rows, None, 0.2, 0.2, 0.0, 0, True)
+        else:
+            out = PF.TokenLogProbsFunction.apply(x, tokens, None, True)
+    for _ in range(2):
+        torch.autograd.grad(out, wide, torch.zeros_like(out), retain_graph=True)
+    backward = [args for name, args in calls if name == "pp_token_log_probs_bwd"]
+    assert len(backward) == 2
+    for a in backward:
+        assert a[0].shape == (b, t, v) and _inside(a[0], a[1:3], (b, t, v)) and a[0].stride() == (*a[1:3], 1)
+        grad, gb, gt = a[10:13]
+        vec = 16 // 4
+        assert _inside(grad, (gb, gt), (b, t, v)) and gt >= v and gb >= (t - 1) * gt + v
+        assert (gb - a[1]) % vec == 0 and (gt - a[2]) % vec == 0 and (grad.data_ptr() - a[0].data_ptr()) % 16 == 0

@@ -53,3 +53,32 @@ def test_the_default_dtype_changes_nothing(dtype, default):
         got = _trained(dtype)
     for a, b in zip(got, want):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [65, 6000])
+def test_saved_tensors_that_come_back_in_another_layout(v, dtype):
+    """A slice of the logits, kept by hooks as a tensor of its own: the gradients of the plain call, whatever the
+    upstream gradient and however often."""
+    g = torch.Generator().manual_seed(v)
+    wide = torch.randn(3, 8, v + 7, generator=g).to(dtype).cuda().requires_grad_()
+    tokens = torch.randint(0, v, (3, 6), generator=g).cuda()
+    old, adv = torch.full((3, 6), -7.0, device="cuda"), torch.randn(3, 6, generator=g).cuda()
+    z, f = (torch.randn(3, 40, 9, generator=g).to(dtype).cuda().requires_grad_() for _ in range(2))
+
+    def results(hooks):
+        out = []
+        for call in (lambda x: PF.token_log_probs(x, tokens).sum(), lambda x: PF.clipped_policy_loss(x, tokens, old, adv)[0]):
+            with hooks():
+                loss = call(wide[:, 1:7, 3:v + 3])
+            for scale in (1.0, 1.0, 3.0):
+                out += torch.autograd.grad(loss * scale, wide, retain_graph=True)
+        with hooks():
+            y, h = PF.gated_recurrence(z[..., 1:], f[..., :8])
+        return out + list(torch.autograd.grad(y.sum() + h.sum(), (z, f)))
+    want = results(contextlib.nullcontext)
+    for hooks in (torch.autograd.graph.save_on_cpu,
+                  lambda: torch.autograd.graph.saved_tensors_hooks(lambda x: x.contiguous().clone(), lambda x: x)):
+        for a, b in zip(results(hooks), want):
+            # (from registers or from kept statistics: a last bit apart where the gradient is made anew)
+            assert float((a - b).abs().max()) <= 4 * torch.finfo(dtype).eps * float(b.abs().max())
