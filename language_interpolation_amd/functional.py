@@ -1228,7 +1228,8 @@ def _class_grad(logits, lb, lt):
 def _same_rows(logits, lb, lt, grad, gb, gt) -> bool:
     """Every row of the gradient begins at its logits' offset within 16 bytes."""
     vec = 16 // logits.element_size()
-    return (grad.data_ptr() - logits.data_ptr()) % 16 == 0 and (gb - lb) % vec == 0 and (gt - lt) % vec == 0
+    return ((grad.data_ptr() - logits.data_ptr()) % 16 == 0 and (gb - lb) % vec == 0 and (gt - lt) % vec == 0 and
+            grad.stride(2) == 1)
 
 
 def _check_classes(logits, tokens, mask):
@@ -1315,8 +1316,8 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         else:
             out.zero_()
         if grad is not None:
-            ctx.save_for_backward(logits, tokens, mask, stats, coef)
-            ctx.grad = (grad, gb, gt)
+            ctx.save_for_backward(logits, tokens, mask, stats, coef, grad)
+            ctx.handed_out = False
         # (no views of each other for autograd: `loss /= n` is allowed, and `kl += x` leaves the loss alone)
         loss, kl, clipped = (x.data for x in out.unbind())
         ctx.mark_non_differentiable(kl, clipped)
@@ -1325,10 +1326,11 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, gloss, _gkl, _gclipped):
-        logits, tokens, mask, stats, coef = ctx.saved_tensors
+        logits, tokens, mask, stats, coef, grad = ctx.saved_tensors
         logits, lb, lt = _class_rows(logits)
-        grad, ctx.grad = ctx.grad, None
-        done = grad is not None and _same_rows(logits, lb, lt, *grad)
+        # (.data: what the program does to its gradient is no change of a saved tensor)
+        grad = (grad.data, grad.stride(0), grad.stride(1))
+        done, ctx.handed_out = not ctx.handed_out and _same_rows(logits, lb, lt, *grad), True
         if not done:
             grad = _class_grad(logits, lb, lt)
         gout = gloss if gloss.dtype is torch.float32 else gloss.float()

@@ -98,3 +98,47 @@ def test_logits_laid_out_anew_by_a_hook(calls, policy):
         vec = 16 // 4
         assert _inside(grad, (gb, gt), (b, t, v)) and gt >= v and gb >= (t - 1) * gt + v
         assert (gb - a[1]) % vec == 0 and (gt - a[2]) % vec == 0 and (grad.data_ptr() - a[0].data_ptr()) % 16 == 0
+
+
+def _policy(x, tokens):
+    rows = torch.zeros(tokens.shape)
+    return PF.ClippedPolicyLossFunction.apply(x, tokens, None, rows, rows, None, 0.2, 0.2, 0.0, 0, True)[0]
+
+
+def test_the_gradient_made_in_the_forward_is_a_saved_tensor(calls):
+    """Hooks see it (offloading moves it off the card), and the node holds no tensor beside what it saved."""
+    packed = []
+    tokens = torch.zeros(2, 5, dtype=torch.int64)
+    x = torch.randn(2, 5, 33, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t) or len(packed) - 1,
+                                                  lambda i: packed[i].clone()):
+        loss = _policy(x, tokens)
+    made = calls[0][1][18]
+    assert made.shape == x.shape and any(t.data_ptr() == made.data_ptr() for t in packed)
+    held = [v for value in vars(loss.grad_fn).values() for v in (value if isinstance(value, (tuple, list)) else [value])]
+    assert not any(isinstance(v, torch.Tensor) for v in held)
+
+
+def test_checkpointed_loss_hands_out_the_gradient_of_the_second_forward(calls):
+    from torch.utils.checkpoint import checkpoint
+    tokens = torch.zeros(2, 5, dtype=torch.int64)
+    x = torch.randn(2, 5, 33, requires_grad=True)
+    (g,) = torch.autograd.grad(checkpoint(_policy, x, tokens, use_reentrant=False), x)
+    forward = [a for name, a in calls if name == "pp_clipped_policy_loss_fwd"]
+    (back,) = [a for name, a in calls if name == "pp_token_log_probs_bwd"]
+    assert len(forward) == 2 and back[9] == 1  # done if the upstream gradient is 1
+    assert back[10].data_ptr() == forward[1][18].data_ptr() == g.data_ptr()
+
+
+def test_a_gradient_is_handed_out_once(calls):
+    """What was handed out belongs to the program, which may change it before it asks again."""
+    tokens = torch.zeros(2, 5, dtype=torch.int64)
+    x = torch.randn(2, 5, 33, requires_grad=True)
+    loss = _policy(x, tokens)
+    (first,) = torch.autograd.grad(loss, x, retain_graph=True)
+    assert first.data_ptr() == calls[0][1][18].data_ptr()
+    first.zero_()
+    for _ in range(2):
+        (again,) = torch.autograd.grad(loss, x, retain_graph=True)
+        assert again.data_ptr() != first.data_ptr()
+    assert [a[9] for name, a in calls if name == "pp_token_log_probs_bwd"] == [1, 0, 0]

@@ -82,3 +82,41 @@ def test_saved_tensors_that_come_back_in_another_layout(v, dtype):
         for a, b in zip(results(hooks), want):
             # (from registers or from kept statistics: a last bit apart where the gradient is made anew)
             assert float((a - b).abs().max()) <= 4 * torch.finfo(dtype).eps * float(b.abs().max())
+
+
+def test_a_checkpointed_or_offloaded_loss_keeps_no_gradient_on_the_card():
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(4, 64, 20000, generator=g).to(BF16).cuda().requires_grad_()
+    tokens = torch.randint(0, 20000, (4, 64), generator=g).cuda()
+    old, adv = torch.full((4, 64), -10.0, device="cuda"), torch.randn(4, 64, generator=g).cuda()
+
+    def loss(y):
+        return PF.clipped_policy_loss(y, tokens, old, adv)[0]
+    (want,) = torch.autograd.grad(loss(x), x)
+    size = x.numel() * x.element_size()
+    for kind in ("checkpoint", "offload"):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        if kind == "checkpoint":
+            out = checkpoint(loss, x, use_reentrant=False)
+        else:
+            with torch.autograd.graph.save_on_cpu():
+                out = loss(x)
+        assert torch.cuda.memory_allocated() - before < size // 4, kind
+        (got,) = torch.autograd.grad(out, x)
+        assert torch.equal(got, want)
+        del out, got
+
+
+def test_a_gradient_changed_by_the_program_is_made_anew():
+    x = torch.randn(3, 5, 700, device="cuda", requires_grad=True)
+    tokens = torch.randint(0, 700, (3, 5), device="cuda")
+    rows = torch.full((3, 5), -7.0, device="cuda")
+    loss = PF.clipped_policy_loss(x, tokens, rows, torch.ones(3, 5, device="cuda"))[0]
+    loss.backward(retain_graph=True)
+    want = x.grad.clone()
+    assert float(want.abs().max()) > 0
+    x.grad.zero_()
+    loss.backward(retain_graph=True)  # adds to the zeros
+    assert float((x.grad - want).abs().max()) <= 8 * torch.finfo(F32).eps * float(want.abs().max())
