@@ -1158,8 +1158,8 @@ def gated_recurrence(z, f, h0=None, lengths=None, reset=None):
     one projection are).  h0: the state before the first step, fp32 [b, d] (default zeros).
     lengths: int [b], the steps of each row that exist (y is 0 behind them, h_last is the state
     before them); reset: bool [b, l], steps before which the state is dropped (a new document in a
-    packed row).  y has z's dtype, h_last is fp32.  Differentiable in z, f and h0.  Formed as
-    z + a (h - z), which keeps the digits of a gate near 1: an infinite z gives NaN."""
+    packed row).  y has z's dtype, h_last is fp32.  Differentiable in z, f and h0.  a and 1 - a are
+    formed apart, each to its own digits: what a gate near 1 lets in of z is not lost."""
     _require_element(z, "z")
     _require_element(f, "f", like=z)
     if z.dim() != 3 or f.shape != z.shape:
