@@ -249,6 +249,12 @@ __device__ __forceinline__ uint32_t own_reset_bits(const uint8_t* reset, int64_t
   return bits;
 }
 
+template <bool FOLD>
+__device__ __forceinline__ uint32_t cuts(const RecArgs& p, int b, int t0, int n) {
+  if (FOLD) return own_reset_bits(p.reset, (int64_t)b * p.l + t0, n);
+  return n > 0 ? reset_bits(p.reset, (int64_t)b * p.l, t0, n) : 0u;
+}
+
 // this workgroup's chunk (counted along the chain), channel group and row
 __device__ __forceinline__ void draw_tile(const RecArgs& p, int* shared, int& c, int& g, int& b) {
   int id = blockIdx.x;
@@ -494,15 +500,13 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_fwd_kernel(const T*
     P[v] = 1.0f;
     H[v] = 0.0f;
   }
-  uint32_t cut = 0;
-  bool fast = false;
-  if (FOLD ? rows > 0 : n > 0) {
-    cut = FOLD ? own_reset_bits(p.reset, row0, n) : reset_bits(p.reset, (int64_t)b * p.l, t0, n);
+  const uint32_t cut = cuts<FOLD>(p, b, t0, n);
+  const bool fast = n == kSteps && cut == 0;
+  const bool straight = FOLD ? __all(fast || n == 0) : fast;  // (the same way for all lanes of a wave)
+  if (n > 0) {
     const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
     const T* fp = f + b * p.fb + t0 * p.fl;
-    fast = n == kSteps && cut == 0;
-    if (FOLD) fast = __all(fast);
-    if (fast)
+    if (straight)
       first_walk<true, T, V>(zp, p.zl, fp, p.fl, ch, n, cut, hl, pl, P, H);
     else
       first_walk<false, T, V>(zp, p.zl, fp, p.fl, ch, n, cut, hl, pl, P, H);
@@ -602,10 +606,10 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
     P[v] = 1.0f;
     G[v] = 0.0f;
   }
-  uint32_t cut = 0;
-  bool fast = false;
-  if (FOLD ? rows > 0 : n > 0) {
-    cut = FOLD ? own_reset_bits(p.reset, row0, n) : reset_bits(p.reset, (int64_t)b * p.l, t0, n);
+  const uint32_t cut = cuts<FOLD>(p, b, t0, n);
+  const bool fast = n == kSteps && cut == 0;
+  const bool straight = FOLD ? __all(fast || n == 0) : fast;
+  if (n > 0) {
     const T* zp = z + b * p.zb + t0 * p.zl;  // (the same for all lanes: scalar addresses)
     const T* fp = f + b * p.fb + t0 * p.fl;
     const T* gp = gy + b * p.gb + t0 * p.gl;
@@ -613,9 +617,7 @@ __global__ __launch_bounds__(64 * kMostWaves, 4) void pp_rec_bwd_kernel(
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = sp[ch + v];
-    fast = n == kSteps && cut == 0;
-    if (FOLD) fast = __all(fast);
-    if (fast)
+    if (straight)
       first_walk_back<true, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, ch, n, cut, h, q, gap, gr, P, G);
     else
       first_walk_back<false, T, V>(zp, p.zl, fp, p.fl, gp, p.gl, ch, n, cut, h, q, gap, gr, P, G);

@@ -120,3 +120,26 @@ def test_a_gradient_changed_by_the_program_is_made_anew():
     x.grad.zero_()
     loss.backward(retain_graph=True)  # adds to the zeros
     assert float((x.grad - want).abs().max()) <= 8 * torch.finfo(F32).eps * float(want.abs().max())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("b,l,d", [(6500, 64, 1), (450, 304, 3), (4200, 16, 7), (131, 513, 32)])
+def test_behind_the_ends_of_rows_that_share_waves(b, l, d, dtype):
+    """Rows of a few channels that end at different steps, NaN behind the ends of inputs and gradient, with and without resets."""
+    import seq_oracle as so
+    g = torch.Generator().manual_seed(l + d)
+    z, f, gy = (torch.randn(b, l, d, generator=g).to(dtype) for _ in range(3))
+    h0, gh = torch.randn(b, d, generator=g), torch.randn(b, d, generator=g)
+    lengths = torch.randint(0, l + 1, (b,), generator=g, dtype=torch.int32)
+    lengths[:70] = l  # a wave of whole rows
+    lengths[70:140] = 0
+    lengths[-1] = 1
+    behind = torch.arange(l)[None] >= lengths[:, None]
+    for reset in (None, torch.rand(b, l, generator=g) < 0.02):
+        want = so.recurrence(z, f, h0, lengths, reset, gy, gh)
+        bad = [x.masked_fill(behind[..., None], float("nan")).cuda() for x in (z, f, gy)]
+        leaves = [bad[0].requires_grad_(), bad[1].requires_grad_(), h0.cuda().requires_grad_()]
+        y, h = PF.gated_recurrence(*leaves, lengths=lengths.cuda(), reset=None if reset is None else reset.cuda())
+        grads = torch.autograd.grad((y, h), leaves, (bad[2], gh.cuda()))
+        for name, x in zip(("y", "h", "gz", "gf", "gh0"), (y, h) + grads):
+            so.check(x, want[name], name)
