@@ -8,7 +8,7 @@
 // The sum of exp(x - max) is taken in fp32 a lane and in 64 bits over the lanes; lp = (x - max) - log sum
 // and its differences to old and ref are formed in 64 bits (a few operations a row: the log is that of the
 // mantissa in fp32, and the exponent times log 2), since a ratio is the exponential of a small difference of
-// numbers around -10, whose fp32 spacing alone would be 1e-6 of it.  The backward keeps (max, log sum) in fp32.
+// numbers around -10, whose fp32 spacing alone would be 1e-6 of it.  The backward keeps (max, sum) in fp32.
 // A masked token's logits, token, old, ref and advantage are not read; its gradient row is zeros.
 //
 // Bound: the logits are read once and the gradient written once.  A row that fits is therefore held
@@ -132,11 +132,13 @@ __device__ __forceinline__ double log_of(double sum) {
   return low == low ? l + (double)low : l;
 }
 
-// A row's max and the log of the sum of exp(x - max).
+// A row's max, the sum of exp(x - max) and its log.
 struct RowStats {
-  float max;
+  float max, sum;
   double log_sum;
-  __device__ __forceinline__ float2 kept() const { return make_float2(max, (float)log_sum); }
+  __device__ __forceinline__ explicit RowStats(const MaxSum& r) : max(r.max), sum((float)r.sum), log_sum(log_of(r.sum)) {}
+  // (the sum, not its log: a share from a log around 10 that is rounded to fp32 would be off by 8 such roundings)
+  __device__ __forceinline__ float2 kept() const { return make_float2(max, sum); }
   __device__ __forceinline__ double lp(float x) const { return ((double)x - (double)max) - log_sum; }
 };
 
@@ -207,8 +209,7 @@ __device__ __forceinline__ RowStats stream_stats(const T* __restrict__ x, int v,
     run.add(e);
   }
   if (tid < s.edge) run.add((float)x[s.edge_at(tid)]);
-  const MaxSum all = join_lanes<THREADS>(run, red);
-  return {all.max, log_of(all.sum)};
+  return RowStats(join_lanes<THREADS>(run, red));
 }
 
 // stats and lp, or stats, terms and coef, of each row.  THREADS lanes a row, 256 a workgroup.
@@ -284,7 +285,7 @@ __global__ __launch_bounds__(256) void pp_row_grad_kernel(const T* __restrict__ 
     }
     const float c = coef[row] * go;
     const float2 st = stats[row];
-    const float k = -c * exp_of(-st.y);
+    const float k = -c / st.y;
     const int64_t tok = p.tokens[row];
     const int token = tok >= 0 && tok < p.v ? (int)tok : -1 - kVec;
     const Span<T> s(x, p.v);
@@ -363,27 +364,26 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, NV <= 8 ? 8 : 4) voi
     }
   }
   keep_raw(r);
-  const MaxSum all = join_lanes<THREADS>(run, red);
-  const RowStats st = {all.max, log_of(all.sum)};
+  const RowStats st(join_lanes<THREADS>(run, red));
   const float c = policy_terms(p, q, row, st.lp(xt), tid == 0);
   if (tid == 0) {
     if (stats) stats[row] = st.kept();
     if (coef) coef[row] = c;
   }
   if (!g) return;
-  const float k = -c / (float)all.sum;
+  const float k = -c / st.sum;
   const int token = tok >= 0 && tok < p.v ? (int)tok : -1 - kVec;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int n = i * THREADS + tid;
     if (n < s.vecs) {
       const int e = s.head + n * kVec;
-      E::stream(g + e, grad_vec<T>(r[i], all.max, k, c, token - e));
+      E::stream(g + e, grad_vec<T>(r[i], st.max, k, c, token - e));
     }
   }
   if (tid < s.edge) {
     const int e = s.edge_at(tid);
-    g[e] = (T)(k * exp_of(edge - all.max) + (e == token ? c : 0.0f));
+    g[e] = (T)(k * exp_of(edge - st.max) + (e == token ? c : 0.0f));
   }
 }
 
