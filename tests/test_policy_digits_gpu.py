@@ -29,3 +29,27 @@ def test_the_share_of_equal_classes(v):
     (one,) = torch.autograd.grad(loss, x, retain_graph=True)
     (two,) = torch.autograd.grad(loss, x, torch.tensor(2.0, device="cuda"))  # made anew from what was kept
     assert bool(((two - 2 * one)[..., :-1].abs() <= 8 * U * two[..., :-1].abs()).all())
+
+
+@pytest.mark.parametrize("v", [5, 130, 3001, 40001, 70001])
+@pytest.mark.parametrize("anew", [False, True])
+def test_shares_of_unlikely_classes(v, anew):
+    """fp32: two classes' gradients are to each other as exp of their logits' difference, however unlikely.  An exponential
+    2 U, a product U on either side: 8 U counted, and the exact quotient's own rounding."""
+    g = torch.Generator().manual_seed(v)
+    x = -80.0 * torch.rand(1, 4, v, generator=g)
+    x[..., 0], tokens = 0.0, torch.full((1, 4), v - 1)
+    xd = x.cuda().requires_grad_()
+    if anew:
+        (got,) = torch.autograd.grad(PF.token_log_probs(xd, tokens.cuda()).sum(), xd)
+    else:
+        rows = torch.full((1, 4), -40.0, device="cuda")
+        ref = rows + 0.5
+        loss = PF.clipped_policy_loss(xd, tokens.cuda(), rows, torch.zeros(1, 4, device="cuda"), ref, kl_coef=0.5)[0]
+        (got,) = torch.autograd.grad(loss, xd)
+    got = got.cpu().double()[..., :-1]
+    ratio, want = got / got[..., :1], x.double()[..., :-1].exp()
+    # (a gradient of fp32's subnormals has fewer bits)
+    fine = got.abs() > 2.0 ** -120
+    assert float(fine.double().mean()) > 0.5
+    assert bool(((ratio - want).abs() <= 8 * U * want)[fine].all()), float(((ratio / want - 1).abs()[fine]).max() / U)
