@@ -22,6 +22,7 @@
 // load and store a row needs two exponentials an entry, which is 40 % of the time and hides only behind
 // the other rows of the CU: two at up to 65536 entries, one above.
 #include <algorithm>
+#include <cmath>
 
 #include "pp_device.h"
 #include "pp_lowp.h"
@@ -44,6 +45,7 @@ struct PolTerms {
   const float* ref;
   int64_t ab, at;       // strides of adv
   float low, high, beta;
+  double log_low, log_high;  // of 1 - low (NaN above 1: no ratio is below) and 1 + high
   const float* weight;  // of a token, by sequence; NULL: `every`
   float every;
   float* terms;         // [3][padded rows]: weighted loss, kl, clipped
@@ -161,9 +163,11 @@ __device__ __forceinline__ float policy_terms(const PolArgs& p, const PolTerms& 
                                               bool writer) {
   const int b = row / p.t, t = row % p.t;
   const float w = q.weight ? q.weight[b] : q.every, adv = q.adv[b * q.ab + t * q.at];
-  const float rho = expf((float)(lp - (double)q.old[row]));
+  const double step = lp - (double)q.old[row];
+  const float rho = expf((float)step);
   const float border = adv >= 0.0f ? 1.0f + q.high : 1.0f - q.low;
-  const bool clipped = adv >= 0.0f ? rho > border : rho < border;
+  // (in 64 bits: a ratio of fp32 lies on a border that it is beyond by half a unit)
+  const bool clipped = adv >= 0.0f ? step > q.log_high : step < q.log_low;
   float loss = -(clipped ? border : rho) * adv, c = clipped ? 0.0f : -adv * rho, kl = 0.0f;
   if (q.ref) {
     const float delta = (float)((double)q.ref[row] - lp), grow = expm1f(delta);
@@ -578,8 +582,8 @@ hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtyp
   const PolArgs p = {tokens, mask, lb, lt, gb, gt, 0, b * t, t, v};
   float* weight = static_cast<float*>(ws);
   // (without a mask both means are the mean over all tokens)
-  const PolTerms q = {old, adv, ref, ab, at, low, high, beta, mask ? weight : nullptr,
-                      1.0f / ((float)b * (float)t), weight + ((b + 3) & ~3), padded_rows(b, t)};
+  const PolTerms q = {old, adv, ref, ab, at, low, high, beta, std::log1p(-(double)low), std::log1p((double)high),
+                      mask ? weight : nullptr, 1.0f / ((float)b * (float)t), weight + ((b + 3) & ~3), padded_rows(b, t)};
   if (mask)
     hipLaunchKernelGGL(pp_policy_weight_kernel, dim3(1), dim3(1024), 0, st, mask, b, t, by_sequence,
                        weight);

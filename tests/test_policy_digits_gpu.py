@@ -53,3 +53,28 @@ def test_shares_of_unlikely_classes(v, anew):
     fine = got.abs() > 2.0 ** -120
     assert float(fine.double().mean()) > 0.5
     assert bool(((ratio - want).abs() <= 8 * U * want)[fine].all()), float(((ratio / want - 1).abs()[fine]).max() / U)
+
+
+@pytest.mark.parametrize("below", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_ratios_next_to_a_border(dtype, below):
+    """Two equal logits, lp = -log 2: borders one fp32 step apart on both sides of a ratio.  lp comes from a sum of 2 exactly, so
+    it is as exact as the logarithm (2^-27 counted); a ratio further than that from the border is clipped or not."""
+    f = np.float32
+    cases = []
+    for old in np.linspace(-1.1, -0.8, 40).astype(f) if not below else np.linspace(-0.6, -0.3, 40).astype(f):
+        d = -math.log(2.0) - float(old)
+        exact = abs(math.expm1(d))
+        for clip in (f(exact), np.nextafter(f(exact), f(0)), np.nextafter(f(exact), f(1))):
+            gap = d - math.log1p(-float(clip) if below else float(clip))
+            if abs(gap) > 2.0 ** -27:
+                cases.append((old, float(clip), gap < 0 if below else gap > 0))
+    assert len(cases) > 60 and 10 < sum(c for _, _, c in cases) < len(cases) - 10
+    # (an fp32 ratio falls on the border itself in some of them: those are what this is about)
+    x = torch.zeros(1, 1, 2, dtype=dtype, device="cuda", requires_grad=True)
+    token, adv = torch.zeros(1, 1, dtype=torch.int64, device="cuda"), torch.full((1, 1), -1.0 if below else 1.0, device="cuda")
+    for old, clip, cut in cases:
+        kw = {"clip_low": clip} if below else {"clip_high": clip}
+        loss, _, clipped = PF.clipped_policy_loss(x, token, torch.full((1, 1), float(old), device="cuda"), adv, **kw)
+        (g,) = torch.autograd.grad(loss, x)
+        assert bool(clipped == 1.0) == cut and bool((g == 0).all()) == cut, (old, clip)
