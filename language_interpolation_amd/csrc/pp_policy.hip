@@ -133,12 +133,18 @@ __device__ __forceinline__ MaxSum join_lanes(const Running& run, MaxSum* red) {
   return r;
 }
 
-// log of a sum: exponent and mantissa apart
+// log of a sum: exponent and mantissa apart, the mantissa between sqrt(1/2) and sqrt(2), so that nothing cancels where the
+// sum is near 1 (a certain token: 0 for 1, and never less)
 __device__ __forceinline__ double log_of(double sum) {
   const float f = (float)sum;
   const float low = (float)((sum - (double)f) / sum);  // what fp32 rounds off (NaN for 0 and infinity)
-  const double l = (double)__builtin_amdgcn_frexp_expf(f) * 0.69314718055994531 +
-                   (double)logf(__builtin_amdgcn_frexp_mantf(f));
+  int e = __builtin_amdgcn_frexp_expf(f);
+  float m = __builtin_amdgcn_frexp_mantf(f);
+  if (m < 0.707106781f) {
+    m *= 2.0f;
+    e -= 1;
+  }
+  const double l = (double)e * 0.69314718055994531 + (double)logf(m);
   return low == low ? l + (double)low : l;
 }
 

@@ -78,3 +78,34 @@ def test_ratios_next_to_a_border(dtype, below):
         loss, _, clipped = PF.clipped_policy_loss(x, token, torch.full((1, 1), float(old), device="cuda"), adv, **kw)
         (g,) = torch.autograd.grad(loss, x)
         assert bool(clipped == 1.0) == cut and bool((g == 0).all()) == cut, (old, clip)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_a_certain_token_is_not_more_than_certain(dtype):
+    """Sums of 1 and just above: log-probabilities are 0 or below, 0 where nothing but the token has a share."""
+    one = torch.tensor([[[3.5]]], dtype=dtype, device="cuda")
+    zero = torch.zeros(1, 1, dtype=torch.int64, device="cuda")
+    assert float(PF.token_log_probs(one, zero)) == 0.0
+    for v in (2, 64, 300, 5000, 150000):
+        x = torch.full((1, 1, v), -60000.0 if dtype != F16 else -300.0, dtype=dtype, device="cuda")
+        x[..., v - 1] = 0.0
+        assert float(PF.token_log_probs(x, zero + v - 1)) == 0.0
+        # another class behind a distance of n: 1 + e^-n, its log e^-n to first order.  The sum of a lane is fp32 (U), that
+        # of a row 16 such (16 U), the log of a number near 1 is off by a unit of itself
+        for n in (6, 9, 12, 15, 18, 25):
+            x[..., 0] = -float(n)
+            lp = float(PF.token_log_probs(x, zero + v - 1))
+            want = -math.log1p(math.exp(-n))
+            assert lp <= 0.0 and abs(lp - want) <= 17 * U * 2, (v, n)
+
+
+def test_the_log_of_a_sum_near_one_keeps_its_digits():
+    """The share of the likeliest class comes in a lane of another wave than the second's, whose sum is exact: nothing but
+    the logarithm rounds, to 2 U of itself (4 U with the exponential and 3 U of the fp32 result: 12 U counted)."""
+    v = 4096  # 1024 vectors of 4 in 256 threads
+    for n in (5.0, 9.0, 13.0, 17.0, 21.0):
+        x = torch.full((1, 1, v), float("-inf"), device="cuda")
+        x[..., 0], x[..., 64 * 4 * 3] = 0.0, -n
+        lp = float(PF.token_log_probs(x, torch.zeros(1, 1, dtype=torch.int64, device="cuda")))
+        want = -math.log1p(math.exp(-n))
+        assert abs(lp - want) <= (12 + n) * U * abs(want), n
