@@ -285,7 +285,8 @@ class AdamW(torch.optim.Optimizer):
     capturable: the step numbers are device counters, so that a captured step counts its replays.
     step(grad_scale=t): gradients are multiplied by the device scalar t first.
     16-bit weights follow their masters: who sets them from outside after the first step sets
-    state[p]["master"] too.  State dicts of torch.optim.Adam and AdamW can be loaded."""
+    state[p]["master"] too.  State dicts of torch.optim.AdamW can be loaded, and those of torch.optim.Adam
+    without a (coupled) weight decay; one of another rule (amsgrad, maximize) is refused."""
 
     MIN_8BIT = 4096
 
@@ -356,9 +357,23 @@ class AdamW(torch.optim.Optimizer):
                     seed=group["seed"] + 8191 * index + k, grad_scale=grad_scale)
         return loss
 
+    @staticmethod
+    def _check_rule(group):
+        """A saved group whose steps were not this class's is refused."""
+        if "moment_bits" not in group and "amsgrad" not in group:
+            raise ValueError("AdamW: the checkpoint is none of AdamW or torch.optim.Adam")
+        for name in ("maximize", "amsgrad"):
+            if group.get(name):
+                raise ValueError(f"AdamW: the checkpoint was made with {name}=True, which this class does not do")
+        if "moment_bits" not in group and group["weight_decay"] != 0 and not group.get("decoupled_weight_decay"):
+            raise ValueError("AdamW: the checkpoint's weight decay is coupled (torch.optim.Adam), this class's is not; if it "
+                             "is one of torch.optim.AdamW, set decoupled_weight_decay=True in its groups")
+
     def load_state_dict(self, state_dict):
         """As the base class, but the state keeps its own types (the base class would cast codes,
         moments and masters to the parameter's) and its own order of the entries."""
+        for group in state_dict["param_groups"]:
+            self._check_rule(group)
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = []
