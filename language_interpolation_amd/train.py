@@ -369,13 +369,29 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: the checkpoint's weight decay is coupled (torch.optim.Adam), this class's is not; if it "
                              "is one of torch.optim.AdamW, set decoupled_weight_decay=True in its groups")
 
+    @staticmethod
+    def _check_state(p, old):
+        """A parameter's saved state is that of a tensor like it."""
+        for name in ("exp_avg", "exp_avg_sq", "master"):
+            x = old.get(name)
+            if x is not None and x.shape != p.shape:
+                raise ValueError(f"AdamW: {name} of shape {tuple(x.shape)} in the checkpoint, the parameter has {tuple(p.shape)}")
+            if x is not None and name != "master" and x.dtype == torch.uint8:
+                e = old.get(name + "_exponent")
+                if e is None or e.dtype != torch.uint8 or e.shape != (PF.moment_blocks(p.numel()),):
+                    raise ValueError(f"AdamW: the exponents of {name} do not fit a parameter of {p.numel()} entries")
+                if x.stride() != p.stride():
+                    raise ValueError("AdamW: 8-bit moments belong to another order of the entries")
+
     def load_state_dict(self, state_dict):
         """As the base class, but the state keeps its own types (the base class would cast codes,
         moments and masters to the parameter's) and its own order of the entries."""
         for group in state_dict["param_groups"]:
             self._check_rule(group)
-        super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            self._check_state(p, state_dict["state"].get(i, {}))
+        super().load_state_dict(state_dict)
         mine = []
         for group in self.param_groups:
             for name, value in self.defaults.items():  # a torch.optim group has no moment_bits and seed
@@ -390,8 +406,6 @@ class AdamW(torch.optim.Optimizer):
             for name in ("exp_avg", "exp_avg_sq"):
                 x = old[name]
                 if x.dtype == torch.uint8:
-                    if x.stride() != p.stride():
-                        raise ValueError("AdamW: 8-bit moments belong to another order of the entries")
                     st[name + "_exponent"] = old[name + "_exponent"].to(p.device, copy=True)
                 st[name] = torch.empty_like(p, dtype=torch.uint8 if x.dtype == torch.uint8 else torch.float32).copy_(x)
             if p.dtype != torch.float32:

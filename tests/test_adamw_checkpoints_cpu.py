@@ -72,3 +72,38 @@ def test_the_same_rule_is_loaded():
         again = AdamW(_params())
         again.load_state_dict(opt.state_dict())
         assert again.param_groups[0]["seed"] == 9
+
+
+def test_moments_of_another_shape_are_refused():
+    """A moment that could be spread over the weight is not, and the optimizer keeps what it had."""
+    for name in ("exp_avg", "exp_avg_sq"):
+        for shape in ((1, 5), (), (5, 6), (30,)):
+            state = _checkpoint(torch.optim.AdamW)
+            state["state"][0][name] = torch.ones(shape)
+            _refused(state, "shape")
+
+
+def test_codes_that_do_not_fit_are_refused():
+    ps = [torch.zeros(100, 50).requires_grad_()]
+
+    def state(p, shape=(100, 50), blocks=20, **kw):
+        entry = {"step": 3}
+        for name in ("exp_avg", "exp_avg_sq"):
+            entry[name] = torch.zeros(shape, dtype=torch.uint8)
+            entry[name + "_exponent"] = torch.zeros(blocks, dtype=torch.uint8)
+        entry.update(kw)
+        return {"state": {0: entry}, "param_groups": AdamW([p], moment_bits=8).state_dict()["param_groups"]}
+    for kw, match in ((dict(shape=(100, 1)), "shape"), (dict(blocks=19), "exponents"), (dict(blocks=1), "exponents"),
+                      (dict(exp_avg=torch.zeros(50, 100, dtype=torch.uint8).t()), "order"),
+                      (dict(exp_avg_exponent=torch.zeros(20)), "exponents")):
+        opt = AdamW(ps, lr=0.25)
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(state(ps[0], **kw))
+        assert not opt.state and opt.param_groups[0]["lr"] == 0.25
+    half = [torch.zeros(100, 50, dtype=torch.bfloat16).requires_grad_()]
+    opt = AdamW(half)
+    with pytest.raises(ValueError, match="shape"):
+        opt.load_state_dict(state(half[0], master=torch.zeros(50)))
+    opt.load_state_dict(state(half[0], master=torch.ones(100, 50)))
+    assert float(opt.state[half[0]]["master"].sum()) == 5000
+    assert opt.state[half[0]]["exp_avg"].dtype == torch.uint8
