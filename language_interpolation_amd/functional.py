@@ -1408,8 +1408,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     [moment_blocks(numel)] (all zero at first); their rounding is stochastic, drawn from `seed`, the
     step and the place.  Every tensor has the strides of its param, which may be any dense order.
     steps: the number of this step (1, 2, ...) or a device int64 counter that is advanced by the call
-    (under graph capture), for all or a list of one each.  grad_scale: device fp32 scalar that the
-    gradients are multiplied by."""
+    (under graph capture), for all or a list of one each.  lr, betas, eps and weight_decay are numbers:
+    a captured step keeps those of its capture.  grad_scale: device fp32 scalar that the gradients
+    are multiplied by."""
+    if isinstance(lr, torch.Tensor) and lr.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_step: a learning rate on the device would be read once, at the capture; pass a number, and "
+                           "capture again when it changes")
     params = list(params)
     n = len(params)
     eight = avg_exponents is not None or sq_exponents is not None

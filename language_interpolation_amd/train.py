@@ -283,6 +283,8 @@ class AdamW(torch.optim.Optimizer):
     moment_bits=8 keeps both moments in one byte an entry (tensors under MIN_8BIT entries stay in 32
     bits: they are most of the tensors and none of the memory); `seed` is that of their rounding.
     capturable: the step numbers are device counters, so that a captured step counts its replays.
+    Nothing else is: replays go on with the lr, betas, eps and weight decay of the capture, so a
+    scheduler's new lr needs a new capture.
     step(grad_scale=t): gradients are multiplied by the device scalar t first.
     16-bit weights follow their masters: who sets them from outside after the first step sets
     state[p]["master"] too.  State dicts of torch.optim.AdamW can be loaded, and those of torch.optim.Adam
@@ -587,6 +589,9 @@ class GraphedTrainStep:
     is a few hundred short launches, and the host cannot issue them as fast as the GPU retires
     them.  The library allocates nothing and never synchronises, so the whole step is
     capturable; torch's allocations inside the capture come from the graph's private pool.
+
+    Numbers go into the graph by value: replays keep the optimizer's lr of the capture (any of the
+    optimizers here), a new lr needs a new GraphedTrainStep.
 
     The warm-up iterations PyTorch asks for before a capture run real steps, so parameters are
     restored and the optimizer state is zeroed in place afterwards (state tensors must exist

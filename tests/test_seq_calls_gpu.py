@@ -143,3 +143,25 @@ def test_behind_the_ends_of_rows_that_share_waves(b, l, d, dtype):
         grads = torch.autograd.grad((y, h), leaves, (bad[2], gh.cuda()))
         for name, x in zip(("y", "h", "gz", "gf", "gh0"), (y, h) + grads):
             so.check(x, want[name], name)
+
+
+def test_a_learning_rate_on_the_device_is_refused_under_capture():
+    """It would be read once, by the host, at the capture; eagerly it is a number like any other."""
+    from language_interpolation_amd.train import AdamW
+    p = torch.ones(300, device="cuda", requires_grad=True)
+    q = torch.ones(300, device="cuda", requires_grad=True)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    rate = torch.tensor(0.25, device="cuda")
+    opt, plain = AdamW([p], lr=rate, capturable=True), AdamW([q], lr=0.25)
+    opt.step()
+    plain.step()
+    assert torch.equal(p, q)
+    before, step = p.detach().clone(), int(opt.state[p]["step"])
+    with pytest.raises(RuntimeError, match="learning rate"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p, before) and int(opt.state[p]["step"]) == step == 1
+    opt.step()
+    plain.step()
+    assert torch.equal(p, q)
