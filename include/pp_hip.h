@@ -464,7 +464,9 @@ enum { PP_F32 = 0, PP_BF16 = 1, PP_F16 = 2 };
  * Backward: gy [b][l][d] with strides (gb, gl), gh_last [b][d] or NULL (zeros); writes gz, gf
  * [b][l][d] contiguous and gh0 [b][d] unless NULL.  Scratch: pp_gated_recurrence_workspace_bytes
  * for either direction (0: none needed), contents undefined on entry and exit; calls that may run
- * at the same time need one each.  b <= 65535.  Bitwise reproducible.
+ * at the same time need one each.  b <= 65535, and 64 threads for every 16 steps (above 256 steps: 1024 for
+ * every 256) of every 64 channels of a row come to fewer than 2^32 (PP_ERR_RANGE): split larger batches, rows are
+ * independent.  Bitwise reproducible.
  * The step form takes one token for b running sequences: z, f [b][d] with row strides zb, fb; h
  * [b][d] fp32 with row stride hb is replaced by the new state, y [b][d] contiguous receives it. */
 #define PP_RECURRENCE_STEPS 16

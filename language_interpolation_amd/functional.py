@@ -12,6 +12,7 @@ import ctypes
 import math
 from array import array
 from dataclasses import dataclass, field
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -1099,6 +1100,23 @@ def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+@lru_cache(maxsize=256)
+def _rows_of_a_launch(l: int, d: int) -> int:
+    """Rows of l steps of d channels that a call of pp_gated_recurrence_* takes."""
+    threads = 64 * -(-l // 16) if l <= 256 else 1024 * -(-l // 256)
+    return max(1, min(65535, ((1 << 31) - 1) // l, ((1 << 32) // threads - 1) // -(-d // 64)))
+
+
+def _row_slices(b: int, l: int, d: int, *tensors):
+    """The tensors (or None) in slices of their rows, as few and as equal as the launches allow."""
+    most = _rows_of_a_launch(l, d)
+    if b <= most:
+        return (tensors,)
+    count = -(-b // most)
+    cuts = [b * i // count for i in range(count + 1)]
+    return [[None if t is None else t[lo:hi] for t in tensors] for lo, hi in zip(cuts, cuts[1:])]
+
+
 class GatedRecurrenceFunction(torch.autograd.Function):
     """(y, h_last) of gated_recurrence; keeps z, f and the state at the start of every
     PP_RECURRENCE_STEPS steps, the backward recomputes the states in between."""
@@ -1118,11 +1136,13 @@ class GatedRecurrenceFunction(torch.autograd.Function):
             h = torch.empty(b, d, device=z.device, dtype=torch.float32)
             if graded:
                 starts = torch.empty(b, lib.pp_gated_recurrence_starts(l), d, device=z.device, dtype=torch.float32)
-            nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
-            ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
-            _launch("pp_gated_recurrence_fwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
-                    f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(h0), _at(lengths), _at(reset),
-                    _at(y), _at(h), _at(starts), _at(ws), nbytes, b, l, d)
+            for pz, pf, ph0, pn, pr, py, ph, ps in _row_slices(b, l, d, z, f, h0, lengths, reset, y, h, starts):
+                rows = pz.shape[0]
+                nbytes = lib.pp_gated_recurrence_workspace_bytes(rows, l, d)
+                ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
+                _launch("pp_gated_recurrence_fwd", z.device, _at(pz), z.stride(0), z.stride(1), _at(pf),
+                        f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(ph0), _at(pn), _at(pr),
+                        _at(py), _at(ph), _at(ps), _at(ws), nbytes, rows, l, d)
         if graded:
             ctx.save_for_backward(z, f, starts, lengths, reset)
         return y, h
@@ -1140,12 +1160,15 @@ class GatedRecurrenceFunction(torch.autograd.Function):
             return gz, gf, gh if ctx.needs_input_grad[2] else None, None, None, None
         gy = torch.zeros_like(gz) if gy is None else _last_contiguous(gy)
         gh0 = torch.empty(b, d, device=z.device, dtype=torch.float32) if ctx.needs_input_grad[2] else None
-        nbytes = lib.pp_gated_recurrence_workspace_bytes(b, l, d)
-        ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
-        _launch("pp_gated_recurrence_bwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
-                f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(lengths), _at(reset), _at(starts),
-                _at(gy), gy.stride(0), gy.stride(1), _at(gh), _at(gz), _at(gf), _at(gh0), _at(ws),
-                nbytes, b, l, d)
+        for pz, pf, pn, pr, ps, py, ph, pgz, pgf, pgh0 in _row_slices(b, l, d, z, f, lengths, reset, starts, gy, gh,
+                                                                      gz, gf, gh0):
+            rows = pz.shape[0]
+            nbytes = lib.pp_gated_recurrence_workspace_bytes(rows, l, d)
+            ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
+            _launch("pp_gated_recurrence_bwd", z.device, _at(pz), z.stride(0), z.stride(1), _at(pf),
+                    f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(pn), _at(pr), _at(ps),
+                    _at(py), gy.stride(0), gy.stride(1), _at(ph), _at(pgz), _at(pgf), _at(pgh0), _at(ws),
+                    nbytes, rows, l, d)
         return gz, gf, gh0, None, None, None
 
 
@@ -1158,7 +1181,7 @@ def gated_recurrence(z, f, h0=None, lengths=None, reset=None):
     one projection are).  h0: the state before the first step, fp32 [b, d] (default zeros).
     lengths: int [b], the steps of each row that exist (y is 0 behind them, h_last is the state
     before them); reset: bool [b, l], steps before which the state is dropped (a new document in a
-    packed row).  y has z's dtype, h_last is fp32.  Differentiable in z, f and h0.  a and 1 - a are
+    packed row).  Above 65535 rows (less for long ones) the batch takes several launches.  y has z's dtype, h_last is fp32.  Differentiable in z, f and h0.  a and 1 - a are
     formed apart, each to its own digits: what a gate near 1 lets in of z is not lost."""
     _require_element(z, "z")
     _require_element(f, "f", like=z)
@@ -1195,8 +1218,13 @@ def gated_recurrence_step(z, f, h):
     if z.numel() == 0:
         return y
     z, f = _last_contiguous(z), _last_contiguous(f)
-    _launch("pp_gated_recurrence_step", z.device, _at(z), z.stride(0), _at(f), f.stride(0),
-            _ELEMENT[z.dtype], _at(h), max(h.stride(0), d), _at(y), b, d)
+    if b <= _rows_of_a_launch(1, d):
+        _launch("pp_gated_recurrence_step", z.device, _at(z), z.stride(0), _at(f), f.stride(0),
+                _ELEMENT[z.dtype], _at(h), max(h.stride(0), d), _at(y), b, d)
+    else:
+        for pz, pf, ph, py in _row_slices(b, 1, d, z, f, h, y):
+            _launch("pp_gated_recurrence_step", z.device, _at(pz), z.stride(0), _at(pf), f.stride(0),
+                    _ELEMENT[z.dtype], _at(ph), max(h.stride(0), d), _at(py), pz.shape[0], d)
     _written([h])
     return y
 

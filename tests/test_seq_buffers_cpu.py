@@ -142,3 +142,47 @@ def test_a_gradient_is_handed_out_once(calls):
         (again,) = torch.autograd.grad(loss, x, retain_graph=True)
         assert again.data_ptr() != first.data_ptr()
     assert [a[9] for name, a in calls if name == "pp_token_log_probs_bwd"] == [1, 0, 0]
+
+
+def test_many_rows_are_taken_in_slices(calls):
+    """A launch takes 65535 rows: more are several launches over the rows' own parts of every tensor."""
+    b, l, d = 150001, 2, 1
+    z, f = (torch.randn(b, l, 2 * d)[..., :d].requires_grad_() for _ in range(2))
+    h0 = torch.randn(b, d, requires_grad=True)
+    lengths, reset = torch.ones(b, dtype=torch.int32), torch.zeros(b, l, dtype=torch.uint8)
+    y, h = PF.GatedRecurrenceFunction.apply(z, f, h0, lengths, reset, True)
+    gz, gf, gh0 = torch.autograd.grad((y, h), (z, f, h0), (torch.zeros(b, l, d), torch.zeros(b, d)))
+    fwd = [a for name, a in calls if name.endswith("_fwd")]
+    bwd = [a for name, a in calls if name.endswith("_bwd")]
+    for made, whole in ((fwd, {0: z, 3: f, 7: h0, 8: lengths, 9: reset, 10: y, 11: h, 12: None}),
+                        (bwd, {0: z, 3: f, 7: lengths, 8: reset, 9: None, 10: None, 13: None, 14: gz, 15: gf, 16: gh0})):
+        rows = [a[-3] for a in made]
+        assert len(rows) == 3 and sum(rows) == b and max(rows) <= 65535 and max(rows) - min(rows) < 3
+        first = 0
+        for a in made:
+            assert a[-2:] == (l, d)
+            for at, t in whole.items():
+                part = a[at]
+                assert part.shape[0] == a[-3]
+                if t is not None:
+                    assert part.data_ptr() == t[first:].data_ptr() and part.stride() == t.stride()
+            first += a[-3]
+    assert [a[12].data_ptr() for a in fwd] == [a[9].data_ptr() for a in bwd]  # the kept states
+    assert fwd[1][12].data_ptr() - fwd[0][12].data_ptr() == 4 * fwd[0][-3] * d
+
+
+def test_rows_of_a_launch_are_what_the_entry_takes():
+    """The entries say so themselves, before they look at addresses (an odd one here) or launch anything."""
+    import ctypes
+    from language_interpolation_amd import _lib
+    lib, odd = _lib.load(), ctypes.c_void_p(4097)
+
+    def entry(b, l, d):
+        return lib.pp_gated_recurrence_fwd(odd, 1, 1, odd, 1, 1, 0, None, None, None, odd, odd, None, None, 0, b, l, d, None)
+    for l in (1, 16, 17, 256, 257, 5000, 32767, 131072, 1 << 24):
+        for d in (1, 64, 65, 2048, 1 << 20):
+            most = PF._rows_of_a_launch(l, d)
+            assert most >= 1
+            if most > 1:
+                assert entry(most, l, d) == -3, (l, d)  # only the address is wrong
+                assert entry(most + 1, l, d) in (-2, -6), (l, d)

@@ -165,3 +165,35 @@ def test_a_learning_rate_on_the_device_is_refused_under_capture():
     opt.step()
     plain.step()
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("b,l,d", [(65536, 3, 5), (70000, 20, 3), (66001, 260, 1), (140003, 1, 2)])
+def test_more_rows_than_a_launch_takes(b, l, d):
+    import seq_oracle as so
+    g = torch.Generator().manual_seed(l)
+    z, f, gy = (torch.randn(b, l, d, generator=g) for _ in range(3))
+    h0, gh = torch.randn(b, d, generator=g), torch.randn(b, d, generator=g)
+    lengths = torch.randint(0, l + 1, (b,), generator=g, dtype=torch.int32)
+    reset = torch.rand(b, l, generator=g) < 0.05
+    want = so.recurrence(z, f, h0, lengths, reset, gy, gh)
+    leaves = [x.cuda().requires_grad_() for x in (z, f, h0)]
+    y, h = PF.gated_recurrence(*leaves, lengths=lengths.cuda(), reset=reset.cuda())
+    grads = torch.autograd.grad((y, h), leaves, (gy.cuda(), gh.cuda()))
+    for name, x in zip(("y", "h", "gz", "gf", "gh0"), (y, h) + grads):
+        so.check(x, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_token_for_more_sequences_than_a_launch_takes(dtype):
+    import seq_oracle as so
+    b, d = 131073, 5
+    g = torch.Generator().manual_seed(1)
+    z, f = (torch.randn(b, 1, d, generator=g).to(dtype) for _ in range(2))
+    h0 = torch.randn(b, d, generator=g)
+    pool = torch.full((b, d + 2), 7.0, device="cuda")
+    pool[:, :d] = h0.cuda()
+    y = PF.gated_recurrence_step(z.cuda()[:, 0], f.cuda()[:, 0], pool[:, :d])
+    want = so.recurrence(z, f, h0)
+    so.check(y, tuple(x[:, 0] for x in want["y"]), "y")
+    so.check(pool[:, :d], want["h"], "h")
+    assert bool((pool[:, d:] == 7).all())
