@@ -706,11 +706,14 @@ bool fits(int v, size_t size, std::initializer_list<const void*> at, std::initia
   return true;
 }
 
+// groups of 64 v channels: of a row, or of all rows together where they share waves
+int groups(int b, int d, int v, bool fold) { return (int)(((fold ? (int64_t)b * d : d) + 64 * v - 1) / (64 * v)); }
+
 // A short row is one chunk, others are cut into chunks of kMostWaves stretches: with half of that the
 // long chains wait twice as often (bf16 [1, 100003, 640] forward + backward 289 against 241 us, fp32
 // [4, 1024, 2048] 75 against 64), and where nothing waits little is gained ([2, 8192, 2048] 129, 131).
 void plan(RecArgs& p, int v, bool fold, void* ws) {
-  p.ngroup = ((fold ? p.b * p.d : p.d) + 64 * v - 1) / (64 * v);
+  p.ngroup = groups(p.b, p.d, v, fold);
   p.chains = fold ? p.ngroup : p.ngroup * p.b;
   p.chunk = kSteps * std::min(kMostWaves, (p.l + kSteps - 1) / kSteps);
   p.nchunk = (p.l + p.chunk - 1) / p.chunk;
@@ -787,7 +790,9 @@ void run_step(const void* z, int64_t zb, const void* f, int64_t fb, float* h, in
 size_t pp_rec_workspace_bytes(int b, int l, int d) {
   if (l <= kMostWaves * kSteps) return 0;
   const size_t chunk = kMostWaves * kSteps, nchunk = ((size_t)l + chunk - 1) / chunk;
-  return 16 + (size_t)b * nchunk * (((size_t)d + 127) / 128 * 128) * 12;
+  // (without the type: room for two channels a lane)
+  const size_t lanes = folds(b, l, d) ? 64 * (size_t)groups(b, d, 1, true) : 128 * (size_t)groups(b, d, 2, false) * b;
+  return 16 + lanes * nchunk * 12;
 }
 
 hipError_t pp_launch_rec_fwd(const void* z, int64_t zb, int64_t zl, const void* f, int64_t fb,

@@ -186,3 +186,16 @@ def test_rows_of_a_launch_are_what_the_entry_takes():
             if most > 1:
                 assert entry(most, l, d) == -3, (l, d)  # only the address is wrong
                 assert entry(most + 1, l, d) in (-2, -6), (l, d)
+
+
+def test_the_workspace_of_shared_rows_is_what_they_use():
+    """Rows of up to 32 channels that share waves: 12 bytes for each of a chunk's lanes, not for 128 channels a row."""
+    from language_interpolation_amd import _lib
+    need = _lib.load().pp_gated_recurrence_workspace_bytes
+    chunks = -(-131072 // 256)
+    assert need(457, 131072, 1) == 16 + 12 * 64 * -(-457 // 64) * chunks
+    assert need(450, 304, 3) == 16 + 12 * 64 * -(-1350 // 64) * 2
+    assert need(131, 513, 32) == 16 + 12 * 64 * -(-131 * 32 // 64) * 3
+    # a wave or more a row: one or two channels a lane, whichever the type takes
+    assert need(1, 1000, 64) >= 16 + 12 * 64 * 4 and need(8, 2048, 2048) == 16 + 12 * 8 * 2048 * 8
+    assert need(3, 256, 40) == 0
