@@ -525,7 +525,7 @@ int pp_clipped_policy_loss_fwd(const void* logits, int64_t lb, int64_t lt, int d
  * w is p and master is NULL, 16-bit: w is master[t] (fp32) and p receives w rounded to nearest.
  * moment_bits 32: m, v fp32, m_exp and v_exp NULL.  8: codes of one byte and one exponent byte for
  * every 256 entries (pp_moment_blocks), all zero at first; stochastic rounding from (seed, s,
- * first_index + t, entry).  pp_decode_moment: their values as `dtype`.
+ * first_index + t, entry), by 8 random bits: betas above 1 - 2^-12 are refused (PP_ERR_RANGE).  pp_decode_moment: their values as `dtype`.
  * step: host array of step numbers s >= 1; or step_dev, an array of device counters of which s is
  * read when the kernel runs (pp_count_step adds 1 to each; a graph that holds both calls counts its
  * replays).  Host arrays of `count` entries; tensors are `numel[t]` elements in one order, updated

@@ -14,9 +14,13 @@
 // bits (top 30); the all-ones code is a value that was not finite.
 // Rounding is stochastic: b2 = 0.999 moves v by 0.1 % a step and the codes are 6 to 12 % apart, so
 // rounding to nearest would hold v where it is for ever; rounding up with the probability that the
-// remainder stands for keeps the expected value exact.  The bits come from a hash of (seed, step,
-// tensor, entry), so a step can be repeated.  A positive v never becomes zero: the step m / eps that
-// would follow is unbounded.
+// remainder stands for keeps the expected value.  An entry has 8 random bits for that, so the probability is a
+// multiple of 1/256, and what is under 1/512 of a unit is rounded away: a code has 8 to 16 units, so a step has to move
+// the moment by 2^-12 of it at least.  At b2 = 0.999 v falls by b2^n to a few per cent, and rests while g^2 stays within
+// 12 to 24 % of it; with b above 1 - 2^-12 it would stand still, and is refused.  (More random bits: two more hashes for every
+// four entries, in a step that the vector units bound, and other codes for the same seed.)  The bits come from a
+// hash of (seed, step, tensor, entry), so a step can be repeated.  A positive v never becomes zero: the step
+// m / eps that would follow is unbounded.
 //
 // Bound: HBM.  Everything is read and written once, in 16-byte accesses (4 bytes of codes) that pass the caches
 // by: nothing is used again before the next step, and 92 M fp32 weights take 432 us (6.0 TB/s) that way, 478

@@ -1043,6 +1043,7 @@ int pp_adamw_step(int count, int dtype, int moment_bits, void* const* p, const v
   if (!p || !g || !m || !v || !numel || (!step && !step_dev)) return PP_ERR_NULL;
   if ((dtype != PP_F32 && !master) || (moment_bits == 8 && (!m_exp || !v_exp))) return PP_ERR_NULL;
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return PP_ERR_SHAPE;
+  if (moment_bits == 8 && (beta1 > 1.0 - 0x1p-12 || beta2 > 1.0 - 0x1p-12)) return PP_ERR_RANGE;  // moments would stand still
   const size_t s = elem_size(dtype), ms = moment_bits / 8;
   int64_t blocks = 0;
   if (!aligned_to(grad_scale, 4)) return PP_ERR_ALIGN;

@@ -1420,6 +1420,16 @@ def moment_blocks(numel: int) -> int:
     return _lib.load().pp_moment_blocks(numel)
 
 
+MOST_BETA_8BIT = 1 - 2.0 ** -12
+
+
+def check_betas_8bit(betas) -> None:
+    """A code is one of 8 to 16 units; a change under 1/512 of a unit is rounded away, with 8 random bits."""
+    if not max(betas) <= MOST_BETA_8BIT:
+        raise ValueError(f"betas {tuple(betas)} are too near 1 for 8-bit moments: above {MOST_BETA_8BIT} a step changes "
+                         "less than their rounding can carry, and they stand still")
+
+
 @torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0.999), eps=1e-8,
                weight_decay=1e-2, masters=None, avg_exponents=None, sq_exponents=None, seed=0,
@@ -1434,7 +1444,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     bf16 and fp16 params need `masters`, fp32 tensors that hold the weights, and receive them
     rounded.  exp_avgs, exp_avg_sqs: fp32, or uint8 codes with avg_exponents and sq_exponents, uint8
     [moment_blocks(numel)] (all zero at first); their rounding is stochastic, drawn from `seed`, the
-    step and the place.  Every tensor has the strides of its param, which may be any dense order.
+    step and the place, with 8 random bits (betas above 1 - 2^-12 are refused there).  Every tensor has the strides of its param, which may be any dense order.
     steps: the number of this step (1, 2, ...) or a device int64 counter that is advanced by the call
     (under graph capture), for all or a list of one each.  lr, betas, eps and weight_decay are numbers:
     a captured step keeps those of its capture.  grad_scale: device fp32 scalar that the gradients
@@ -1450,6 +1460,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, *, lr, betas=(0.9, 0
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
         raise ValueError(f"adamw_step: betas must lie in [0, 1), got {betas}")
+    if eight:
+        check_betas_8bit(betas)
     lists = {"grads": list(grads), "exp_avgs": list(exp_avgs), "exp_avg_sqs": list(exp_avg_sqs)}
     for name, x in (("masters", masters), ("avg_exponents", avg_exponents), ("sq_exponents", sq_exponents)):
         if x is not None:

@@ -281,7 +281,9 @@ class AdamW(torch.optim.Optimizer):
     an fp32 master in the state; dense in any order (the layers' parameters are permuted leaves).
 
     moment_bits=8 keeps both moments in one byte an entry (tensors under MIN_8BIT entries stay in 32
-    bits: they are most of the tensors and none of the memory); `seed` is that of their rounding.
+    bits: they are most of the tensors and none of the memory); `seed` is that of their rounding.  It has
+    8 random bits: at beta2 = 0.999 a second moment may rest while the squares of the gradients stay
+    within a quarter of it; betas above 1 - 2^-12, where it could not even fall, are refused.
     capturable: the step numbers are device counters, so that a captured step counts its replays.
     Nothing else is: replays go on with the lr, betas, eps and weight decay of the capture, so a
     scheduler's new lr needs a new capture.
@@ -300,6 +302,16 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       moment_bits=moment_bits, capturable=capturable, seed=seed))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        if group["moment_bits"] == 8 and any(p.numel() >= self.MIN_8BIT for p in group["params"]):
+            try:
+                PF.check_betas_8bit(group["betas"])
+            except ValueError:
+                self.param_groups.pop()
+                raise
 
     def _init_state(self, p, group):
         st = self.state[p]
