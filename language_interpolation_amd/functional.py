@@ -1107,14 +1107,29 @@ def _rows_of_a_launch(l: int, d: int) -> int:
     return max(1, min(65535, ((1 << 31) - 1) // l, ((1 << 32) // threads - 1) // -(-d // 64)))
 
 
-def _row_slices(b: int, l: int, d: int, *tensors):
-    """The tensors (or None) in slices of their rows, as few and as equal as the launches allow."""
-    most = _rows_of_a_launch(l, d)
-    if b <= most:
-        return (tensors,)
-    count = -(-b // most)
+def _in_slices(launch, b: int, l: int, d: int, *tensors):
+    """The launch for slices of the rows of the tensors (or None), as few and as equal as it allows."""
+    count = -(-b // _rows_of_a_launch(l, d))
     cuts = [b * i // count for i in range(count + 1)]
-    return [[None if t is None else t[lo:hi] for t in tensors] for lo, hi in zip(cuts, cuts[1:])]
+    for lo, hi in zip(cuts, cuts[1:]):
+        launch(hi - lo, l, d, *(None if t is None else t[lo:hi] for t in tensors))
+
+
+def _recurrence_fwd(b, l, d, z, f, h0, lengths, reset, y, h, starts):
+    nbytes = _lib.load().pp_gated_recurrence_workspace_bytes(b, l, d)
+    ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
+    _launch("pp_gated_recurrence_fwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
+            f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(h0), _at(lengths), _at(reset),
+            _at(y), _at(h), _at(starts), _at(ws), nbytes, b, l, d)
+
+
+def _recurrence_bwd(b, l, d, z, f, lengths, reset, starts, gy, gh, gz, gf, gh0):
+    nbytes = _lib.load().pp_gated_recurrence_workspace_bytes(b, l, d)
+    ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
+    _launch("pp_gated_recurrence_bwd", z.device, _at(z), z.stride(0), z.stride(1), _at(f),
+            f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(lengths), _at(reset), _at(starts),
+            _at(gy), gy.stride(0), gy.stride(1), _at(gh), _at(gz), _at(gf), _at(gh0), _at(ws),
+            nbytes, b, l, d)
 
 
 class GatedRecurrenceFunction(torch.autograd.Function):
@@ -1136,13 +1151,10 @@ class GatedRecurrenceFunction(torch.autograd.Function):
             h = torch.empty(b, d, device=z.device, dtype=torch.float32)
             if graded:
                 starts = torch.empty(b, lib.pp_gated_recurrence_starts(l), d, device=z.device, dtype=torch.float32)
-            for pz, pf, ph0, pn, pr, py, ph, ps in _row_slices(b, l, d, z, f, h0, lengths, reset, y, h, starts):
-                rows = pz.shape[0]
-                nbytes = lib.pp_gated_recurrence_workspace_bytes(rows, l, d)
-                ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
-                _launch("pp_gated_recurrence_fwd", z.device, _at(pz), z.stride(0), z.stride(1), _at(pf),
-                        f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(ph0), _at(pn), _at(pr),
-                        _at(py), _at(ph), _at(ps), _at(ws), nbytes, rows, l, d)
+            if b <= _rows_of_a_launch(l, d):
+                _recurrence_fwd(b, l, d, z, f, h0, lengths, reset, y, h, starts)
+            else:
+                _in_slices(_recurrence_fwd, b, l, d, z, f, h0, lengths, reset, y, h, starts)
         if graded:
             ctx.save_for_backward(z, f, starts, lengths, reset)
         return y, h
@@ -1150,7 +1162,6 @@ class GatedRecurrenceFunction(torch.autograd.Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, gy, gh):
-        lib = _lib.load()
         z, f, starts, lengths, reset = ctx.saved_tensors
         b, l, d = z.shape
         gz = torch.empty(b, l, d, device=z.device, dtype=z.dtype)
@@ -1160,15 +1171,10 @@ class GatedRecurrenceFunction(torch.autograd.Function):
             return gz, gf, gh if ctx.needs_input_grad[2] else None, None, None, None
         gy = torch.zeros_like(gz) if gy is None else _last_contiguous(gy)
         gh0 = torch.empty(b, d, device=z.device, dtype=torch.float32) if ctx.needs_input_grad[2] else None
-        for pz, pf, pn, pr, ps, py, ph, pgz, pgf, pgh0 in _row_slices(b, l, d, z, f, lengths, reset, starts, gy, gh,
-                                                                      gz, gf, gh0):
-            rows = pz.shape[0]
-            nbytes = lib.pp_gated_recurrence_workspace_bytes(rows, l, d)
-            ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8) if nbytes else None
-            _launch("pp_gated_recurrence_bwd", z.device, _at(pz), z.stride(0), z.stride(1), _at(pf),
-                    f.stride(0), f.stride(1), _ELEMENT[z.dtype], _at(pn), _at(pr), _at(ps),
-                    _at(py), gy.stride(0), gy.stride(1), _at(ph), _at(pgz), _at(pgf), _at(pgh0), _at(ws),
-                    nbytes, rows, l, d)
+        if b <= _rows_of_a_launch(l, d):
+            _recurrence_bwd(b, l, d, z, f, lengths, reset, starts, gy, gh, gz, gf, gh0)
+        else:
+            _in_slices(_recurrence_bwd, b, l, d, z, f, lengths, reset, starts, gy, gh, gz, gf, gh0)
         return gz, gf, gh0, None, None, None
 
 
@@ -1200,6 +1206,11 @@ def gated_recurrence(z, f, h0=None, lengths=None, reset=None):
     return GatedRecurrenceFunction.apply(z, f, h0, lengths, reset, _graded(z, f, h0))
 
 
+def _recurrence_step(b, l, d, z, f, h, y):
+    _launch("pp_gated_recurrence_step", z.device, _at(z), z.stride(0), _at(f), f.stride(0),
+            _ELEMENT[z.dtype], _at(h), max(h.stride(0), d), _at(y), b, d)
+
+
 def gated_recurrence_step(z, f, h):
     """One token of b running sequences: z, f [b, d]; h [b, d] fp32 is replaced by the new state,
     which is returned in z's dtype.  No backward: gated_recurrence has one."""
@@ -1219,12 +1230,9 @@ def gated_recurrence_step(z, f, h):
         return y
     z, f = _last_contiguous(z), _last_contiguous(f)
     if b <= _rows_of_a_launch(1, d):
-        _launch("pp_gated_recurrence_step", z.device, _at(z), z.stride(0), _at(f), f.stride(0),
-                _ELEMENT[z.dtype], _at(h), max(h.stride(0), d), _at(y), b, d)
+        _recurrence_step(b, 1, d, z, f, h, y)
     else:
-        for pz, pf, ph, py in _row_slices(b, 1, d, z, f, h, y):
-            _launch("pp_gated_recurrence_step", z.device, _at(pz), z.stride(0), _at(pf), f.stride(0),
-                    _ELEMENT[z.dtype], _at(ph), max(h.stride(0), d), _at(py), pz.shape[0], d)
+        _in_slices(_recurrence_step, b, 1, d, z, f, h, y)
     _written([h])
     return y
 
@@ -1345,7 +1353,7 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
             out.zero_()
         if grad is not None:
             ctx.save_for_backward(logits, tokens, mask, stats, coef, grad)
-            ctx.handed_out = False
+            ctx.rows, ctx.handed_out = (logits.stride(), lb, lt, (gb, gt, 1)), False
         # (no views of each other for autograd: `loss /= n` is allowed, and `kl += x` leaves the loss alone)
         loss, kl, clipped = (x.data for x in out.unbind())
         ctx.mark_non_differentiable(kl, clipped)
@@ -1355,12 +1363,14 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     @_once_differentiable
     def backward(ctx, gloss, _gkl, _gclipped):
         logits, tokens, mask, stats, coef, grad = ctx.saved_tensors
-        logits, lb, lt = _class_rows(logits)
+        strides, lb, lt, gstrides = ctx.rows
+        done, ctx.handed_out = not ctx.handed_out, True
+        if logits.stride() != strides or grad.stride() != gstrides or (grad.data_ptr() - logits.data_ptr()) % 16:
+            logits, lb, lt = _class_rows(logits)  # hooks on saved tensors have laid them out anew
+            gstrides = grad.stride()
+            done = done and _same_rows(logits, lb, lt, grad, gstrides[0], gstrides[1])
         # (.data: what the program does to its gradient is no change of a saved tensor)
-        grad = (grad.data, grad.stride(0), grad.stride(1))
-        done, ctx.handed_out = not ctx.handed_out and _same_rows(logits, lb, lt, *grad), True
-        if not done:
-            grad = _class_grad(logits, lb, lt)
+        grad = (grad.data, gstrides[0], gstrides[1]) if done else _class_grad(logits, lb, lt)
         gout = gloss if gloss.dtype is torch.float32 else gloss.float()
         _class_backward(logits, tokens, mask, stats, coef, gout, int(done), grad, (lb, lt))
         return (grad[0],) + (None,) * 10
