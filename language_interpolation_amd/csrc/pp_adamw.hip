@@ -126,7 +126,7 @@ __device__ __forceinline__ uint32_t encode8(float x, int E, uint32_t byte) {
 }
 
 // Square root of 0 or of x >= 2^-96, correctly rounded: the instruction is off by at most one step, and the sign
-// of x - s (s -+ step) tells on which side of the halfway point to either neighbour x lies.
+// of x - s (s -+ step) tells on which side of the halfway point to either neighbour x lies (Tuckerman's test).
 __device__ __forceinline__ float sqrt_plain(float x) {
   const float s = __builtin_amdgcn_sqrtf(x);
   const float less = __uint_as_float(__float_as_uint(s) - 1u), more = __uint_as_float(__float_as_uint(s) + 1u);

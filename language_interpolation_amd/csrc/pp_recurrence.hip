@@ -21,7 +21,8 @@
 // workgroup are consecutive stretches, joined through LDS; the workgroups of a row (chunks) are
 // joined through global memory: each publishes its (P, H) as soon as it has it, then looks back for
 // the nearest chunk whose final state is known and applies the (P, H) of those in between, in
-// order -- the same fma of each chunk whoever applies it, so results do not depend on timing.
+// order -- the same fma of each chunk whoever applies it, so results do not depend on timing.  (The single-pass
+// scan with decoupled look-back of Merrill and Garland, 2016, for the composition of affine maps.)
 //   Waiting is safe: a workgroup draws its chunk from a counter, chunks in the order of the chain,
 // so it waits only for workgroups that are running already and that publish before they wait.
 //   The published words carry their own readiness (all ones = not yet, the fill before the launch),
