@@ -1071,7 +1071,7 @@ def _require_aux(t, name: str, shape, dtypes, device) -> None:
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, expected {device}")
@@ -1084,7 +1084,11 @@ def _bytes_of(mask: Optional[torch.Tensor]):
 
 def _graded(*tensors) -> bool:
     """A backward may follow.  (A Function's needs_input_grad is also set under no_grad.)"""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _once_differentiable(backward):
@@ -1094,6 +1098,17 @@ def _once_differentiable(backward):
     def run(ctx, *grads):
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
     return run
+
+
+def _hooked() -> bool:
+    """Hooks are in force on what a node saves, and may bring it back in another layout.  (Asked in the forward: in the
+    backward's thread every look at a tensor costs the host two or three times as much.)"""
+    return torch._C._autograd._top_saved_tensors_default_hooks(True) is not None
+
+
+def _kept(*tensors):
+    """Tensors that were saved contiguous (or None)."""
+    return [t if t is None or t.is_contiguous() else t.contiguous() for t in tensors]
 
 
 def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
@@ -1157,12 +1172,16 @@ class GatedRecurrenceFunction(torch.autograd.Function):
                 _in_slices(_recurrence_fwd, b, l, d, z, f, h0, lengths, reset, y, h, starts)
         if graded:
             ctx.save_for_backward(z, f, starts, lengths, reset)
+            ctx.hooked = _hooked()
         return y, h
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, gy, gh):
         z, f, starts, lengths, reset = ctx.saved_tensors
+        if ctx.hooked:
+            z, f = _last_contiguous(z), _last_contiguous(f)
+            starts, lengths, reset = _kept(starts, lengths, reset)
         b, l, d = z.shape
         gz = torch.empty(b, l, d, device=z.device, dtype=z.dtype)
         gf = torch.empty_like(gz)
@@ -1290,13 +1309,17 @@ class TokenLogProbsFunction(torch.autograd.Function):
                     _ELEMENT[logits.dtype], _at(tokens), _at(mask), _at(lp), _at(stats), b, t, v)
         if stats is not None:
             ctx.save_for_backward(logits, tokens, mask, stats)
+            ctx.rows, ctx.hooked = (lb, lt), _hooked()
         return lp
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, glp):
         logits, tokens, mask, stats = ctx.saved_tensors
-        logits, lb, lt = _class_rows(logits)  # (hooks on saved tensors may have laid them out anew)
+        lb, lt = ctx.rows
+        if ctx.hooked:
+            logits, lb, lt = _class_rows(logits)
+            tokens, mask, stats = _kept(tokens, mask, stats)
         grad = _class_grad(logits, lb, lt)
         _class_backward(logits, tokens, mask, stats, glp.float().contiguous(), None, 0, grad, (lb, lt))
         return grad[0], None, None, None
@@ -1352,8 +1375,8 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         else:
             out.zero_()
         if grad is not None:
-            ctx.save_for_backward(logits, tokens, mask, stats, coef, grad)
-            ctx.rows, ctx.handed_out = (logits.stride(), lb, lt, (gb, gt, 1)), False
+            ctx.save_for_backward(logits, grad, tokens, mask, stats, coef)
+            ctx.rows, ctx.hooked, ctx.handed_out = (lb, lt, gb, gt), _hooked(), False
         # (no views of each other for autograd: `loss /= n` is allowed, and `kl += x` leaves the loss alone)
         loss, kl, clipped = (x.data for x in out.unbind())
         ctx.mark_non_differentiable(kl, clipped)
@@ -1362,15 +1385,16 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, gloss, _gkl, _gclipped):
-        logits, tokens, mask, stats, coef, grad = ctx.saved_tensors
-        strides, lb, lt, gstrides = ctx.rows
+        logits, grad, tokens, mask, stats, coef = ctx.saved_tensors
+        lb, lt, gb, gt = ctx.rows
         done, ctx.handed_out = not ctx.handed_out, True
-        if logits.stride() != strides or grad.stride() != gstrides or (grad.data_ptr() - logits.data_ptr()) % 16:
-            logits, lb, lt = _class_rows(logits)  # hooks on saved tensors have laid them out anew
-            gstrides = grad.stride()
-            done = done and _same_rows(logits, lb, lt, grad, gstrides[0], gstrides[1])
+        if ctx.hooked:
+            logits, lb, lt = _class_rows(logits)
+            tokens, mask, stats, coef = _kept(tokens, mask, stats, coef)
+            gb, gt, _ = grad.stride()
+            done = done and _same_rows(logits, lb, lt, grad, gb, gt)
         # (.data: what the program does to its gradient is no change of a saved tensor)
-        grad = (grad.data, gstrides[0], gstrides[1]) if done else _class_grad(logits, lb, lt)
+        grad = (grad.data, gb, gt) if done else _class_grad(logits, lb, lt)
         gout = gloss if gloss.dtype is torch.float32 else gloss.float()
         _class_backward(logits, tokens, mask, stats, coef, gout, int(done), grad, (lb, lt))
         return (grad[0],) + (None,) * 10

@@ -199,3 +199,41 @@ def test_the_workspace_of_shared_rows_is_what_they_use():
     # a wave or more a row: one or two channels a lane, whichever the type takes
     assert need(1, 1000, 64) >= 16 + 12 * 64 * 4 and need(8, 2048, 2048) == 16 + 12 * 8 * 2048 * 8
     assert need(3, 256, 40) == 0
+
+
+def test_saved_tensors_that_come_back_turned(calls):
+    """A hook may keep a tensor in another order of its elements: what the entries take as contiguous is made so."""
+    def turned(x):
+        return x.transpose(0, -1).contiguous().transpose(0, -1) if x.dim() > 1 else x
+    b, l, d, t, v = 3, 40, 5, 6, 17
+    with torch.autograd.graph.saved_tensors_hooks(turned, lambda x: x):
+        z, f = (torch.randn(b, l, d, requires_grad=True) for _ in range(2))
+        lengths, reset = torch.ones(b, dtype=torch.int32), torch.zeros(b, l, dtype=torch.uint8)
+        y, h = PF.GatedRecurrenceFunction.apply(z, f, None, lengths, reset, True)
+        x, tokens, mask = torch.randn(b, t, v, requires_grad=True), torch.zeros(b, t, dtype=torch.int64), torch.ones(b, t, dtype=torch.uint8)
+        lp = PF.TokenLogProbsFunction.apply(x, tokens, mask, True)
+        rows = torch.zeros(b, t)
+        loss = PF.ClippedPolicyLossFunction.apply(x, tokens, mask, rows, rows, None, 0.2, 0.2, 0.0, 0, True)[0]
+    torch.autograd.grad((y, h), (z, f), (torch.zeros(b, l, d), torch.zeros(b, d)))
+    torch.autograd.grad(lp, x, torch.zeros(b, t))
+    torch.autograd.grad(loss, x)
+    (rec,) = [a for name, a in calls if name == "pp_gated_recurrence_bwd"]
+    assert rec[0].stride() == (rec[1], rec[2], 1) and rec[3].stride() == (rec[4], rec[5], 1)
+    assert all(rec[i].is_contiguous() for i in (7, 8, 9))
+    classes = [a for name, a in calls if name == "pp_token_log_probs_bwd"]
+    assert len(classes) == 2
+    for a in classes:
+        assert a[0].stride() == (a[1], a[2], 1) and a[10].stride() == (a[11], a[12], 1)
+        assert all(a[i].is_contiguous() for i in (4, 5, 6, 7))
+
+
+def test_empty_batches_have_empty_gradients(calls):
+    for b, t in ((0, 5), (3, 0)):
+        x = torch.zeros(b, t, 9, requires_grad=True)
+        tokens, rows = torch.zeros(b, t, dtype=torch.int64), torch.zeros(b, t)
+        lp = PF.TokenLogProbsFunction.apply(x, tokens, None, True)
+        assert torch.autograd.grad(lp, x, rows)[0].shape == x.shape
+        loss = PF.ClippedPolicyLossFunction.apply(x, tokens, None, rows, rows, None, 0.2, 0.2, 0.0, 0, True)[0]
+        for _ in range(2):
+            assert torch.autograd.grad(loss, x, retain_graph=True)[0].shape == x.shape
+    assert not calls

@@ -197,3 +197,27 @@ def test_a_token_for_more_sequences_than_a_launch_takes(dtype):
     so.check(y, tuple(x[:, 0] for x in want["y"]), "y")
     so.check(pool[:, :d], want["h"], "h")
     assert bool((pool[:, d:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_saved_tensors_that_come_back_turned(dtype):
+    """Hooks that keep every tensor with its first and last dimensions exchanged: the gradients of the plain call."""
+    def turned(x):
+        return x.transpose(0, -1).contiguous().transpose(0, -1) if x.dim() > 1 else x
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(3, 6, 301, generator=g).to(dtype).cuda().requires_grad_()
+    z, f = (torch.randn(3, 300, 9, generator=g).to(dtype).cuda().requires_grad_() for _ in range(2))
+    tokens = torch.randint(0, 301, (3, 6), generator=g).cuda()
+    mask, reset = (torch.rand(3, n, generator=g).cuda() < 0.8 for n in (6, 300))
+    old, adv = torch.full((3, 6), -6.0, device="cuda"), torch.randn(3, 6, generator=g).cuda()
+
+    def results(hooks):
+        with hooks:
+            y, h = PF.gated_recurrence(z, f, reset=~reset)
+            lp = PF.token_log_probs(x, tokens, mask)
+            loss = PF.clipped_policy_loss(x, tokens, old, adv, mask=mask)[0]
+        return [*torch.autograd.grad(y.sum() + h.sum(), (z, f)), *torch.autograd.grad(lp.sum(), x),
+                *torch.autograd.grad(loss, x, retain_graph=True), *torch.autograd.grad(loss * 3, x)]
+    want = results(contextlib.nullcontext())
+    for a, b in zip(results(torch.autograd.graph.saved_tensors_hooks(turned, lambda t: t)), want):
+        assert float((a - b).abs().max()) <= 4 * torch.finfo(dtype).eps * float(b.abs().max())
