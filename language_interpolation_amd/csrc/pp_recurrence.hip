@@ -33,8 +33,8 @@
 // between are recomputed from it; y, rounded to 16 bits, would not do for the differences).
 //
 // Bound: forward 3 and backward 5 values an entry through HBM, each once.  Measured (MI355X, bf16):
-// [8, 2048, 2048] forward 50 us (4.2 TB/s with the kept states), backward 73 us (4.7); [1, 100003, 640] 101
-// and 144 us.  The rest is the shape of a workgroup: 16 waves of 113 registers are all that a CU holds, so
+// [8, 2048, 2048] forward 50 us (4.2 TB/s with the kept states), backward 74 us (4.6); [1, 100003, 640] 103
+// and 148 us.  The rest is the shape of a workgroup: 16 waves of 113 registers are all that a CU holds, so
 // its loads, its walks and its waits follow one another.  Counter and look-back are 5 to 10 %, the gates
 // nothing (measured without them).  Rows of few channels share waves (folds).
 #include <algorithm>
