@@ -29,7 +29,7 @@
 
 namespace {
 
-constexpr float kLog2e = 1.44269502f, kLn2 = 0.693147182f, kLn2Rest = -1.90465421e-9f;
+constexpr float kLog2e = 1.44269502f, kLog2eAbove = 1.44269514f, kLn2 = 0.693147182f, kLn2Rest = -1.90465421e-9f;
 
 struct PolArgs {
   const int64_t* tokens;
@@ -67,9 +67,14 @@ struct Span {
   __device__ __forceinline__ int edge_at(int i) const { return i < head ? i : i + vecs * kVec; }
 };
 
-// e^d, off by up to 2^-24 |d| of itself (the product is rounded, and log2(e) too).  A sum over classes hardly sees it: those
-// far below the max add little; one of normal logits is off by 6e-8 of itself.
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+// e^d, off by up to 2^-24 |d| of itself (the product is rounded, and log2(e) too).
+__device__ __forceinline__ float exp_of(float d, float log2e = kLog2e) { return __builtin_amdgcn_exp2f(d * log2e); }
+// In a sum over classes the products' roundings cancel, that of log2(e) does not (sums of normal logits were off by 6e-8 of
+// themselves, all to one side).  So a sixth of the lanes take the next number above: 10 of 64 of them bring the mean
+// of all to log2(e) within 5e-10 of it, at no instruction a class.
+__device__ __forceinline__ float lane_log2e() {
+  return (threadIdx.x & 63) % 6 == 5 ? kLog2eAbove : kLog2e;
+}
 // The same to 2 units of its own size: an fp32 gradient has a value for each class.
 __device__ __forceinline__ float exp_digits(float d) {
   d = __builtin_elementwise_maximum(d, -200.0f);  // (0 from there on; a NaN stays one)
@@ -80,15 +85,16 @@ __device__ __forceinline__ float exp_digits(float d) {
 // What a lane has seen: the max, and the sum of exp(x - max), brought to a new max by one factor a vector.
 struct Running {
   float max = -3.40282347e38f, sum = 0.0f;  // (finite, so that -inf - max is -inf and not NaN)
+  const float log2e = lane_log2e();
   template <int N>
   __device__ __forceinline__ void add(const float (&e)[N]) {
     float top = max;
 #pragma unroll
     for (int j = 0; j < N; ++j) top = fmaxf(top, e[j]);
-    sum *= exp_of(max - top);
+    sum *= exp_of(max - top, log2e);
     max = top;
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum += exp_of(e[j] - top);
+    for (int j = 0; j < N; ++j) sum += exp_of(e[j] - top, log2e);
   }
   __device__ __forceinline__ void add(float e) {
     const float one[1] = {e};
@@ -113,7 +119,7 @@ template <int THREADS>
 __device__ __forceinline__ MaxSum join_lanes(const Running& run, MaxSum* red) {
   MaxSum r;
   r.max = wave_max(run.max);
-  float v = run.sum * exp_of(run.max - r.max);
+  float v = run.sum * exp_digits(run.max - r.max);
   v = pp_dpp_add<0x128>(v);
   v = pp_dpp_add<0x124>(v);
   v = pp_dpp_add<0x122>(v);
@@ -126,7 +132,7 @@ __device__ __forceinline__ MaxSum join_lanes(const Running& run, MaxSum* red) {
     __syncthreads();
     const MaxSum mine = red[threadIdx.x % kWaves];
     r.max = wave_max(mine.max);
-    r.sum = mine.sum * (double)exp_of(mine.max - r.max);
+    r.sum = mine.sum * (double)exp_digits(mine.max - r.max);
 #pragma unroll
     for (int o = kWaves / 2; o; o >>= 1) r.sum += __shfl_xor(r.sum, o);
   }
@@ -263,7 +269,7 @@ __global__ __launch_bounds__(256) void pp_row_terms_kernel(const T* __restrict__
 
 // exp(x - max) for a gradient in T: fp32 keeps the digits, 16 bits have no room for them.  That costs fp32 up to 2 %
 // ([8, 512, v]: v = 4000 37.4 -> 38.1 us, 9001 65.5 -> 65.6, 50021 333 -> 337, 65536 405 -> 410).  In the sums it would
-// cost another 2 to 4 %, there in 16 bits 2 to 30 %, for one unit of the sum.
+// cost another 2 to 4 %, there in 16 bits 2 to 30 %: lane_log2e instead.
 template <typename T>
 __device__ __forceinline__ float share_of(float d) {
   return sizeof(T) == 4 ? exp_digits(d) : exp_of(d);

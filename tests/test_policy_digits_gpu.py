@@ -109,3 +109,24 @@ def test_the_log_of_a_sum_near_one_keeps_its_digits():
         lp = float(PF.token_log_probs(x, torch.zeros(1, 1, dtype=torch.int64, device="cuda")))
         want = -math.log1p(math.exp(-n))
         assert abs(lp - want) <= (12 + n) * U * abs(want), n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v", [128, 1001, 5001, 50021])
+def test_errors_of_the_sums_do_not_add_up(dtype, v):
+    """Ratios far from the borders, all advantages 1: the loss is the mean ratio, so an error of one sign in the sums of a
+    vocabulary is the loss's.  What is left is rounding: a loss is rounded by at most U of itself and by chance (a
+    deviation of U / sqrt 3), so the mean over 100 losses has one of 0.06 U: 5 of those, and as much for ratios and sums of
+    512 tokens, whose own roundings (under 16 U) have a mean deviation below 16 U / sqrt(51200) = 0.07 U."""
+    g = torch.Generator(device="cuda").manual_seed(v)
+    n = 512 if v < 10000 else 128
+    tokens = torch.randint(0, v, (1, n), generator=g, device="cuda")
+    off = []
+    for _ in range(100):
+        x = (torch.randn(1, n, v, generator=g, device="cuda") * 2.0).to(dtype)
+        lp = torch.cat([torch.log_softmax(part.double(), -1) for part in x.split(64, 1)], 1).gather(-1, tokens[..., None])[..., 0]
+        old = (lp - 0.3 - 0.2 * torch.rand(1, n, generator=g, device="cuda")).float()
+        loss = PF.clipped_policy_loss(x, tokens, old, torch.ones(1, n, device="cuda"), clip_high=10.0)[0]
+        off.append(float(loss) / -float(torch.exp(lp - old.double()).mean()) - 1)
+    bound = 5 * U * (1 / math.sqrt(3 * 100) + 16 / math.sqrt(100 * n))
+    assert abs(sum(off) / len(off)) <= bound, (sum(off) / len(off) / U, bound / U)
