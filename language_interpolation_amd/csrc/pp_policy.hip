@@ -44,11 +44,13 @@ struct PolTerms {
   const float* adv;
   const float* ref;
   int64_t ab, at;       // strides of adv
-  float low, high, beta;
-  double log_low, log_high;  // of 1 - low (NaN above 1: no ratio is below) and 1 + high
+  float beta;
+  double low, high;          // 1 - clip_low, 1 + clip_high
+  double log_low, log_high;  // their logarithms (NaN of a negative: no ratio is below)
   const float* weight;  // of a token, by sequence; NULL: `every`
   float every;
-  float* terms;         // [3][padded rows]: weighted loss, kl, clipped
+  double* loss;         // [padded rows]: weighted
+  float* figures;       // [2][padded rows]: weighted kl, clipped
   int padded;
 };
 
@@ -73,7 +75,7 @@ __device__ __forceinline__ float exp_of(float d, float log2e = kLog2e) { return 
 // themselves, all to one side).  So a sixth of the lanes take the next number above: 10 of 64 of them bring the mean
 // of all to log2(e) within 5e-10 of it, at no instruction a class.
 __device__ __forceinline__ float lane_log2e() {
-  return (threadIdx.x & 63) % 6 == 5 ? kLog2eAbove : kLog2e;
+  return (0x0820820820820820ull >> (threadIdx.x & 63)) & 1 ? kLog2eAbove : kLog2e;  // lanes 5, 11, ... 59
 }
 // The same to 2 units of its own size: an fp32 gradient has a value for each class.
 __device__ __forceinline__ float exp_digits(float d) {
@@ -177,10 +179,10 @@ __device__ __forceinline__ float policy_terms(const PolArgs& p, const PolTerms& 
   const float w = q.weight ? q.weight[b] : q.every, adv = q.adv[b * q.ab + t * q.at];
   const double step = lp - (double)q.old[row];
   const float rho = expf((float)step);
-  const float border = adv >= 0.0f ? 1.0f + q.high : 1.0f - q.low;
   // (in 64 bits: a ratio of fp32 lies on a border that it is beyond by half a unit)
   const bool clipped = adv >= 0.0f ? step > q.log_high : step < q.log_low;
-  float loss = -(clipped ? border : rho) * adv, c = clipped ? 0.0f : -adv * rho, kl = 0.0f;
+  float c = clipped ? 0.0f : -adv * rho, kl = 0.0f;
+  float loss = c;  // (of a clipped token: without its ratio)
   if (q.ref) {
     const float delta = (float)((double)q.ref[row] - lp), grow = expm1f(delta);
     kl = grow - delta;
@@ -188,14 +190,19 @@ __device__ __forceinline__ float policy_terms(const PolArgs& p, const PolTerms& 
     c -= q.beta * grow;
   }
   if (writer) {
-    q.terms[row] = loss * w;
-    q.terms[q.padded + row] = kl * w;
-    q.terms[2 * (int64_t)q.padded + row] = clipped ? w : 0.0f;
+    // Ratios are rounded by chance; a border is the same for all the tokens it holds, and advantages repeat: their product in
+    // 64 bits, or all would be off alike, by 2e-8 of it, which a loss shows where its terms cancel.
+    double term = (double)(loss * w);
+    if (clipped) term -= (adv >= 0.0f ? q.high : q.low) * (double)adv * (double)w;
+    q.loss[row] = term;
+    q.figures[row] = kl * w;
+    q.figures[q.padded + row] = clipped ? w : 0.0f;
   }
   return c * w;
 }
 __device__ __forceinline__ void no_terms(const PolTerms& q, int row) {
-  q.terms[row] = q.terms[q.padded + row] = q.terms[2 * (int64_t)q.padded + row] = 0.0f;
+  q.loss[row] = 0.0;
+  q.figures[row] = q.figures[q.padded + row] = 0.0f;
 }
 
 template <typename T, int THREADS>
@@ -456,15 +463,28 @@ __global__ __launch_bounds__(1024) void pp_policy_weight_kernel(const uint8_t* _
   }
 }
 
+// 16 bytes of a list of terms, as one number of 64 bits
+__device__ __forceinline__ double sum_of(const double2& x) { return x.x + x.y; }
+__device__ __forceinline__ double sum_of(const float4& x) { return ((double)x.x + (double)x.y) + ((double)x.z + (double)x.w); }
+template <typename V, typename T>
+__device__ __forceinline__ double sum_list(const T* x, int rows) {
+  constexpr int kVec = sizeof(V) / sizeof(T);
+  const V* v = reinterpret_cast<const V*>(x);  // (lists begin at multiples of 16 bytes)
+  double s = 0.0;
+#pragma unroll 16
+  for (int i = threadIdx.x; i < rows / kVec; i += 1024) s += sum_of(v[i]);
+  if ((int)threadIdx.x < rows % kVec) s += (double)x[rows - rows % kVec + threadIdx.x];
+  return s;
+}
+
 // Sum of each of the three lists, in 64 bits and in a fixed order.
-__global__ __launch_bounds__(1024) void pp_policy_finish_kernel(const float* __restrict__ terms,
+__global__ __launch_bounds__(1024) void pp_policy_finish_kernel(const double* __restrict__ loss,
+                                                                const float* __restrict__ figures,
                                                                 int rows, int padded,
                                                                 float* __restrict__ out) {
   __shared__ double red[16];
-  const float* x = terms + (int64_t)blockIdx.x * padded;
-  double s = 0.0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < rows; i += 1024) s += (double)x[i];
+  double s = blockIdx.x == 0 ? sum_list<double2>(loss, rows)
+                             : sum_list<float4>(figures + (int64_t)(blockIdx.x - 1) * padded, rows);
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -582,7 +602,8 @@ hipError_t pp_launch_token_lp_bwd(const void* logits, int64_t lb, int64_t lt, in
 static int padded_rows(int b, int t) { return (b * t + 3) & ~3; }
 
 size_t pp_policy_workspace_bytes(int b, int t) {
-  return ((((size_t)b + 3) & ~(size_t)3) + 3 * (size_t)padded_rows(b, t)) * sizeof(float);
+  return (((size_t)b + 3) & ~(size_t)3) * sizeof(float) +
+         (size_t)padded_rows(b, t) * (sizeof(double) + 2 * sizeof(float));
 }
 
 hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtype,
@@ -594,8 +615,11 @@ hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtyp
   const PolArgs p = {tokens, mask, lb, lt, gb, gt, 0, b * t, t, v};
   float* weight = static_cast<float*>(ws);
   // (without a mask both means are the mean over all tokens)
-  const PolTerms q = {old, adv, ref, ab, at, low, high, beta, std::log1p(-(double)low), std::log1p((double)high),
-                      mask ? weight : nullptr, 1.0f / ((float)b * (float)t), weight + ((b + 3) & ~3), padded_rows(b, t)};
+  const int padded = padded_rows(b, t);
+  double* loss = reinterpret_cast<double*>(weight + ((b + 3) & ~3));
+  const PolTerms q = {old, adv, ref, ab, at, beta, 1.0 - (double)low, 1.0 + (double)high, std::log1p(-(double)low),
+                      std::log1p((double)high), mask ? weight : nullptr, 1.0f / ((float)b * (float)t), loss,
+                      reinterpret_cast<float*>(loss + padded), padded};
   if (mask)
     hipLaunchKernelGGL(pp_policy_weight_kernel, dim3(1), dim3(1024), 0, st, mask, b, t, by_sequence,
                        weight);
@@ -604,6 +628,6 @@ hipError_t pp_launch_policy(const void* logits, int64_t lb, int64_t lt, int dtyp
                 static_cast<T*>(grad), st)
   PP_POL_TYPES(PP_CALL);
 #undef PP_CALL
-  hipLaunchKernelGGL(pp_policy_finish_kernel, dim3(3), dim3(1024), 0, st, q.terms, p.rows, q.padded, out);
+  hipLaunchKernelGGL(pp_policy_finish_kernel, dim3(3), dim3(1024), 0, st, q.loss, q.figures, p.rows, q.padded, out);
   return hipGetLastError();
 }

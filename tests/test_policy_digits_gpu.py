@@ -130,3 +130,23 @@ def test_errors_of_the_sums_do_not_add_up(dtype, v):
         off.append(float(loss) / -float(torch.exp(lp - old.double()).mean()) - 1)
     bound = 5 * U * (1 / math.sqrt(3 * 100) + 16 / math.sqrt(100 * n))
     assert abs(sum(off) / len(off)) <= bound, (sum(off) / len(off) / U, bound / U)
+
+
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_a_border_is_not_rounded_for_all_tokens_alike(reduction):
+    """Every token clipped, half at either border, so that the loss nearly cancels.  A term is rounded to fp32 once, by chance
+    (a deviation of U / sqrt 3 of itself), so the mean of n is off by U rms / sqrt(3 n): 6 of those, and the result's rounding."""
+    g = torch.Generator().manual_seed(2)
+    b, t, high, low = 256, 256, float(np.float32(0.28)), float(np.float32(0.2))
+    up = torch.rand(b, t // 2, generator=g)
+    adv = torch.cat([up, -1.6 * up], 1)
+    old = torch.cat([torch.full((b, t // 2), math.log(0.5) - 1.0), torch.full((b, t // 2), math.log(0.5) + 1.0)], 1)
+    up64 = torch.ones(b, t, dtype=torch.float64)
+    terms = -torch.where(adv >= 0, (1 + high) * up64, (1 - low) * up64) * adv.double()
+    loss, _, clipped = PF.clipped_policy_loss(torch.zeros(b, t, 2, device="cuda"), torch.zeros(b, t, dtype=torch.int64, device="cuda"),
+                                              old.cuda(), adv.cuda(), mask=torch.ones(b, t, dtype=torch.bool, device="cuda"),
+                                              clip_high=high, clip_low=low, reduction=reduction)
+    want = float(terms.mean())
+    assert float(clipped) == 1.0 and abs(want) < 1e-6
+    bound = 6 * U * float(terms.square().mean().sqrt()) / math.sqrt(3 * b * t) + U * abs(want)
+    assert abs(float(loss) - want) <= bound, (float(loss) - want, bound)
